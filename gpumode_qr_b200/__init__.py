@@ -19,6 +19,11 @@ __all__ = [
     "geqrf_host",
     "gram",
     "gram_geqrf",
+    "linear",
+    "linear_backward",
+    "pack_activation",
+    "unpack_activation",
+    "PackedActivation",
     "VARIANTS",
     "VARIANT_INFO",
     "CHAMPION",
@@ -32,7 +37,8 @@ from .variants import CHAMPION, VARIANT_INFO, VARIANTS  # noqa: E402
 
 def __getattr__(name):  # lazy: keep `import gpumode_qr_b200` torch-free
     if name in ("geqrf", "impl", "hh_fused_qr", "hh_panel_qr", "larfb", "householder_product",
-                "ormqr", "geqrf_host", "gram", "gram_geqrf"):
+                "ormqr", "geqrf_host", "gram", "gram_geqrf", "linear", "linear_backward",
+                "pack_activation", "unpack_activation", "PackedActivation"):
         from . import api
 
         return getattr(api, name)

@@ -41,6 +41,17 @@ SIGNATURES: dict[str, tuple] = {
     "qrb_get_config": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_I64)]),
 }
 
+# The linear-layer operators (include/qrb200_linear.h); the argument structs
+# are passed by address.
+LINEAR_SIGNATURES: dict[str, tuple] = {
+    "qrbl_linear_workspace_bytes": (_SZ, [_P]),
+    "qrbl_linear": (ctypes.c_int, [_P, _P, _SZ, _P]),
+    "qrbl_linear_backward_workspace_bytes": (_SZ, [_P]),
+    "qrbl_linear_backward": (ctypes.c_int, [_P, _P, _SZ, _P]),
+    "qrbl_pack": (ctypes.c_int, [_I32, _P, _I64, _I64, _I64, _P, _P, _P]),
+    "qrbl_unpack": (ctypes.c_int, [_I32, _P, _P, _I64, _I64, _P, _I64, _P]),
+}
+
 
 class QRBError(RuntimeError):
     """A libqrb200 entry point returned a non-zero status."""
@@ -69,7 +80,7 @@ def lib() -> ctypes.CDLL:
                 f"libqrb200.so not found at {LIB_PATH}; run `python -m gpumode_qr_b200.build`"
             )
         handle = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **LINEAR_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args

@@ -12,6 +12,9 @@
   (``src/qrbench/variants.py:800-804``).
 * :func:`gram`, :func:`gram_geqrf` — the statistics ``G @ G.mT`` that the
   reference's workload factors, alone or followed by the factorization.
+* :func:`linear`, :func:`linear_backward` — the layer whose weight gradient is
+  that G, and :func:`pack_activation`, :func:`unpack_activation` — its
+  activations kept in 8 bits for the backward pass (:mod:`.layers`).
 
 Every function runs the CUDA library on the caller's current stream. Inputs
 that the library cannot take (CPU tensors, other dtypes, non-square shapes)
@@ -25,6 +28,13 @@ import math
 import torch
 
 from . import _lib
+from .layers import (  # noqa: F401  (entry points of their own module)
+    PackedActivation,
+    linear,
+    linear_backward,
+    pack_activation,
+    unpack_activation,
+)
 
 
 def _require_cuda_f32(name: str, t: torch.Tensor) -> None:

@@ -1,0 +1,635 @@
+"""GPU tests of the linear-layer operators against 64-bit formulas.
+
+Tolerances, elementwise, from arithmetic (u = half a step of the output type):
+
+* a product's FP32 accumulation over k terms, S the sum of |x_i w_i|: the tensor
+  core truncates, so every add costs at most one FP32 step 2^-23 of a partial
+  sum (at most S). 16-bit layers: k / 16 adds per chain and fewer than 16 within
+  an MMA; FP32 layers: chains of 256 values (4 x 4 adds, counted with their
+  small products as 24), k / 256 adds of chains, and three dropped products of
+  2^-24: ``ACC * S``.
+* an activation: slope at most 1.13, its own evaluation below 1e-6 |z| + 1e-7.
+* dz is rounded once more to the layer's type (u relative, and for float16 half
+  a subnormal step 2^-25): u * (|dz| @ |w|) in dx, likewise in dW; its
+  derivative factor is exact to 2e-6 (at most 1.13, so 2e-6 |dy| absolute).
+* packing: half a step 2^e (a whole step at the largest exponent).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import itertools
+import math
+import threading
+
+import pytest
+import torch
+
+from gpumode_qr_b200 import _lib, api, checker, layers
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF, HF, FP]
+IDS = ["bf16", "fp16", "fp32"]
+ACTS = list(layers.ACTIVATIONS)
+STEP = 2.0**-23
+SUB = {BF: 2.0**-134, HF: 2.0**-25, FP: 2.0**-150}  # half a subnormal step
+
+
+def u(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def acc(dt, k):
+    return STEP * ((24 + k / 256 + 2) if dt == FP else (k / 16 + 18))
+
+
+def rnd(shape, seed, dt, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g)).to(dt).to(DEV)
+
+
+def act64(z, act):
+    """(act(z), act'(z)) in the precision of z."""
+    if act == "none":
+        return z, torch.ones_like(z)
+    if act == "relu":
+        return z.clamp_min(0), (z > 0).to(z.dtype)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * (1 - s)
+    if act == "gelu":
+        p = 0.5 * torch.erfc(-z * math.sqrt(0.5))
+        return z * p, p + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    c = math.sqrt(2 / math.pi)
+    t = torch.tanh(c * (z + 0.044715 * z**3))
+    return 0.5 * z * (1 + t), 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+
+
+def near(got, want, tol, what=""):
+    assert got.shape == want.shape
+    d = (got.double() - want).abs() - tol
+    assert torch.isfinite(got.double()).all(), what
+    worst = d.max().item() if d.numel() else -1.0
+    assert worst <= 0, f"{what}: over the bound by {worst:.3g} of {tol.flatten()[d.argmax()]:.3g}"
+
+
+def check_forward(x, w, b, r, act, y, z=None, dt=None):
+    dt = dt or x.dtype
+    x, w = x.double(), w.double()
+    z64 = x @ w.mT
+    s = x.abs() @ w.abs().mT
+    if b is not None:
+        z64, s = z64 + b.double(), s + b.double().abs()
+    za = acc(dt, x.shape[-1]) * s
+    y64 = act64(z64, act)[0]
+    ya = 1.13 * za + (1e-6 * z64.abs() + 1e-7 if act not in ("none", "relu") else 0)
+    if r is not None:
+        y64 = y64 + r.double()
+        ya = ya + 2.0**-23 * (y64.abs() + r.double().abs())
+    near(y, y64, u(dt) * y64.abs() * 1.0001 + ya * (1 + u(dt)) + SUB[dt], "y")
+    if z is not None:
+        near(z, z64, u(dt) * z64.abs() * 1.0001 + za * (1 + u(dt)) + SUB[dt], "z")
+    return z64, za
+
+
+# ---------------------------------------------------------------------------
+# forward
+# ---------------------------------------------------------------------------
+# one row, one column, one value; odd sizes; edges of every tile width; a long
+# reduction with few tiles (split); tall and wide
+SHAPES = [(1, 1, 1), (1, 4096, 512), (2, 33, 7), (3, 64, 64), (5, 200, 1000), (16, 512, 512),
+          (33, 65, 129), (128, 256, 64), (129, 257, 72), (200, 96, 4096), (300, 1000, 40),
+          (777, 130, 355), (1024, 513, 136), (8, 8, 8192), (64, 2048, 2048)]
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear_sizes(m, n, k, dt):
+    x, w = rnd((m, k), 1, dt), rnd((n, k), 2, dt, k**-0.5)
+    b, r = rnd((n,), 3, dt), rnd((m, n), 4, dt)
+    y = api.linear(x, w, b, r, "silu")
+    check_forward(x, w, b, r, "silu", y)
+    check_forward(x, w, None, None, "none", api.linear(x, w))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,n,k", [(3, 96, 64), (150, 264, 96), (20, 64, 4096)])
+def test_linear_activations(m, n, k, act, dt):
+    x, w, b = rnd((m, k), 5, dt), rnd((n, k), 6, dt, 3 * k**-0.5), rnd((n,), 7, dt)
+    y, z = api.linear(x, w, b, None, act, keep="plain")
+    check_forward(x, w, b, None, act, y, z)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(1, 32, 16), (3, 40, 64), (130, 264, 96), (257, 77, 64),
+                                   (20, 65, 4096), (6, 4096, 1024)])
+def test_linear_keeps_z_packed(m, n, k, dt):
+    x, w, b, r = rnd((m, k), 8, dt), rnd((n, k), 9, dt, k**-0.5), rnd((n,), 10, dt), rnd((m, n), 11, dt)
+    y, p = api.linear(x, w, b, r, "gelu", keep="packed")
+    z64, za = check_forward(x, w, b, r, "gelu", y)
+    assert p.codes.shape == (m, n) and p.exponents.shape == (m, -(-n // 32)) and p.dtype == dt
+    s = torch.ldexp(torch.ones(p.exponents.shape, dtype=torch.float64, device=DEV), p.exponents.int())
+    step = s.repeat_interleave(32, dim=1)[:, :n]
+    got = api.unpack_activation(p)
+    near(got, z64, 0.5 * step + za, "packed z")
+    # the step is the smallest that holds the block's largest value
+    amax = torch.nn.functional.pad(z64.abs(), (0, -n % 32)).view(m, -1, 32).amax(-1)
+    slack = torch.nn.functional.pad(za, (0, -n % 32)).view(m, -1, 32).amax(-1)
+    assert (amax - slack <= 127 * s).all() and (amax + slack > 63.5 * s).all()
+
+
+def test_packed_saturates_beyond_float16():
+    # z = 1e5 is finite in FP32 but not in float16: kept as the largest value
+    # the packed form has there, not as Inf
+    x, w = torch.full((2, 16), 250.0, device=DEV, dtype=HF), torch.full((32, 16), 25.0, device=DEV, dtype=HF)
+    y, p = api.linear(x, w, activation="gelu", keep="packed")
+    assert torch.isinf(y).all()
+    assert (api.unpack_activation(p) == 63 * 1024).all()
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_linear_strides_and_leading_dimensions(dt):
+    m, n, k = 37, 48, 80
+    big = rnd((m, 3 * k + 5), 12, dt)
+    wbig = rnd((n + 3, k + 9), 13, dt, k**-0.5)
+    rbig = rnd((m, n + 7), 14, dt)
+    bbig = rnd((2 * n,), 15, dt)
+    for x, w in ((big[:, 3:3 + k], wbig[1:1 + n, 2:2 + k]),          # rows not 16-byte aligned
+                 (big[:, 8:8 + k], wbig[:n, :k]),
+                 (big[:, ::3][:, :k], wbig[:n, :k]),                 # column stride 3
+                 (big[:, :k].t().contiguous().t(), wbig[:n, :k]),    # column-major
+                 (big[:1, :k].expand(m, k), wbig[:n, :k])):          # one row broadcast
+        for b, r in ((bbig[1:1 + n], rbig[:, 1:1 + n]), (bbig[::2], rbig[:, :n])):
+            y = api.linear(x, w, b, r, "relu")
+            check_forward(x, w, b, r, "relu", y)
+    x4 = rnd((2, 3, 5, k), 16, dt)
+    y4 = api.linear(x4, wbig[:n, :k])
+    assert y4.shape == (2, 3, 5, n)
+    assert torch.equal(y4.reshape(30, n), api.linear(x4.reshape(30, k), wbig[:n, :k]))
+    y1 = api.linear(x4[0, 0, 0], wbig[:n, :k], residual=y4[0, 0, 0])
+    assert y1.shape == (n,)
+    perm = x4.permute(2, 0, 1, 3)
+    assert torch.equal(api.linear(perm, wbig[:n, :k]), y4.permute(2, 0, 1, 3))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_linear_empty(dt):
+    w = rnd((6, 8), 17, dt)
+    assert api.linear(torch.empty(0, 8, device=DEV, dtype=dt), w).shape == (0, 6)
+    assert api.linear(rnd((3, 8), 1, dt), torch.empty(0, 8, device=DEV, dtype=dt)).shape == (3, 0)
+    x0, w0 = torch.empty(3, 0, device=DEV, dtype=dt), torch.empty(70, 0, device=DEV, dtype=dt)
+    b, r = rnd((70,), 18, dt), rnd((3, 70), 19, dt)
+    y, z = api.linear(x0, w0, b, r, "silu", keep="plain")
+    assert torch.equal(z, b.expand(3, 70))
+    check_forward(x0, w0, b, r, "silu", y, z)
+    y, p = api.linear(x0, w0, b, r, "silu", keep="packed")
+    assert torch.equal(api.unpack_activation(p), api.unpack_activation(api.pack_activation(b.expand(3, 70))))
+
+
+def test_linear_non_finite_rows_stay_in_their_row():
+    for dt in TYPES:
+        x, w = rnd((70, 96), 20, dt), rnd((130, 96), 21, dt, 0.1)
+        clean = api.linear(x, w, activation="gelu")
+        x[3, 5], x[40, 7] = float("nan"), float("inf")
+        y, p = api.linear(x, w, activation="gelu", keep="packed")
+        rows = torch.ones(70, dtype=torch.bool, device=DEV)
+        rows[3] = rows[40] = False
+        assert torch.equal(y[rows], clean[rows])
+        assert y[3].isnan().all()
+        assert not torch.isfinite(y[40][(w[:, 7] > 0)]).any()
+        back = api.unpack_activation(p)
+        assert back[3].isnan().all() and back[rows].isfinite().all()
+
+
+def test_linear_in_place_residual():
+    x, w = rnd((100, 64), 22, BF), rnd((72, 64), 23, BF, 0.1)
+    r = rnd((100, 72), 24, BF)
+    want = api.linear(x, w, None, r, "gelu")
+    out = r.clone()
+    a = layers._LinearArgs(2, 2, 100, 72, 64, x.data_ptr(), 64, w.data_ptr(), 64, None,
+                           out.data_ptr(), 72, out.data_ptr(), 72)
+    assert _lib.lib().qrbl_linear(ctypes.byref(a), None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(3, 40, 64), (130, 100, 72), (16, 48, 4096)])
+def test_rows_and_columns_outside_stay_as_they_were(m, n, k, dt):
+    # outputs inside larger buffers: only [m, n] is written
+    L, s = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    x, w = rnd((m, k), 25, dt), rnd((n, k), 26, dt, 0.1)
+    want = api.linear(x, w)
+    for ldy in (n, n + 8, n + 3):
+        y = torch.full((m + 200, ldy), 7.0, device=DEV, dtype=dt)
+        a = layers._LinearArgs(layers._DTYPES[dt], 0, m, n, k, x.data_ptr(), k, w.data_ptr(), k,
+                               None, None, 0, y.data_ptr(), ldy)
+        need = L.qrbl_linear_workspace_bytes(ctypes.byref(a))
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+        assert L.qrbl_linear(ctypes.byref(a), ws.data_ptr(), need, s) == 0
+        assert torch.equal(y[:m, :n], want)
+        assert (y[m:] == 7).all() and (y[:, n:] == 7).all()
+
+
+# ---------------------------------------------------------------------------
+# backward
+# ---------------------------------------------------------------------------
+def check_backward(dy, x64, w, z64, act, dx, dw, db):
+    dt, m = dy.dtype, dy.shape[0]
+    dy, w = dy.double(), w.double()
+    dz = dy * act64(z64, act)[1] if act != "none" else dy
+    # dz as the products see it: rounded (or, FP32, split), its factor off by 2e-6
+    e = (0 if act == "none" else u(dt) if dt != FP else 0) * dz.abs()
+    e = e + (0 if act == "none" else 2e-6 * dy.abs() + SUB[dt])
+    if dx is not None:
+        s = dz.abs() @ w.abs()
+        tol = (e @ w.abs()) + acc(dt, dy.shape[1]) * s
+        want = dz @ w
+        near(dx, want, u(dt) * want.abs() * 1.0001 + tol * (1 + u(dt)) + SUB[dt], "dx")
+    if dw is not None:
+        s = dz.abs().mT @ x64.abs()
+        tol = (e.mT @ x64.abs()) + acc(dt, m) * s
+        want = dz.mT @ x64
+        near(dw, want, u(dt) * want.abs() * 1.0001 + tol * (1 + u(dt)) + SUB[dt], "dw")
+    if db is not None:  # FP32 sums of 64 rows and of the blocks
+        want = dz.sum(0)
+        tol = (2e-6 * dy.abs()).sum(0) + 2.0**-24 * (80 + m / 64) * dz.abs().sum(0)
+        near(db, want, u(dt) * want.abs() * 1.0001 + tol * (1 + u(dt)) + SUB[dt], "db")
+
+
+BSHAPES = [(1, 1, 1), (2, 33, 70), (64, 64, 64), (129, 257, 72), (999, 177, 530), (5, 1000, 16),
+           (4096, 32, 48), (300, 513, 1024)]
+
+
+@pytest.mark.parametrize("kept", ["plain", "packed"])
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", BSHAPES)
+def test_backward_sizes(m, n, k, dt, kept):
+    dy, x, w, z = (rnd((m, n), 30, dt), rnd((m, k), 31, dt), rnd((n, k), 32, dt, n**-0.5),
+                   rnd((m, n), 33, dt, 1.5))
+    if kept == "packed":
+        x, z = api.pack_activation(x), api.pack_activation(z)
+        x64, z64 = api.unpack_activation(x).double(), api.unpack_activation(z).double()
+    else:
+        x64, z64 = x.double(), z.double()
+    for act in ("gelu", "none"):
+        dx, dw, db = api.linear_backward(dy, x, w, z if act != "none" else None, act)
+        check_backward(dy, x64, w, z64, act, dx, dw, db)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("act,kept", [(a, p) for a in ACTS for p in ("plain", "packed")
+                                      if (a, p) not in (("relu", "packed"), ("none", "packed"))])
+def test_backward_activations(act, kept, dt):
+    m, n, k = 70, 96, 40
+    dy, x, w, z = rnd((m, n), 34, dt), rnd((m, k), 35, dt), rnd((n, k), 36, dt), rnd((m, n), 37, dt, 3.0)
+    if kept == "packed":
+        zp = api.pack_activation(z)
+        z64 = api.unpack_activation(zp).double()
+    else:
+        zp, z64 = z, z.double()
+    check_backward(dy, x.double(), w, z64, act, *api.linear_backward(dy, x, w, zp, act))
+
+
+def test_backward_far_pre_activations():
+    # saturated and overflowing z: the derivative is 0 or 1, never NaN
+    z = torch.tensor([-3e38, -1e20, -1e4, -200.0, -90.0, -30.0, 0.0, 30.0, 90.0, 1e4, 1e20, 3e38],
+                     device=DEV)
+    want = (z > 0).float() + 0.5 * (z == 0).float()
+    for dt in (FP, BF):
+        zz = z.to(dt).reshape(1, -1)
+        dy = torch.ones_like(zz)
+        eye = torch.eye(12, device=DEV, dtype=dt)
+        for act in ("gelu", "gelu_tanh", "silu"):
+            dx, _, db = api.linear_backward(dy, None, eye, zz, act, need=("x", "bias"))
+            assert (dx.float()[0] - want).abs().max() < 1e-9
+            assert (db.float() - want).abs().max() < 1e-9
+            y = api.linear(zz, eye, activation=act)
+            # z * 1 is a product with zeros beside it: finite z only
+            assert (y.float()[0, 3:10] - (z * want)[3:10].to(dt).float()).abs().max() < 1e-9
+
+
+@pytest.mark.parametrize("need", [c for r in range(4) for c in itertools.combinations(
+    ("x", "weight", "bias"), r)])
+def test_backward_computes_what_is_needed(need):
+    m, n, k = 130, 72, 100
+    dy, x, w, z = rnd((m, n), 38, BF), rnd((m, k), 39, BF), rnd((n, k), 40, BF), rnd((m, n), 41, BF)
+    full = dict(zip(("x", "weight", "bias"), api.linear_backward(dy, x, w, z, "silu")))
+    got = dict(zip(("x", "weight", "bias"),
+                   api.linear_backward(dy, x if "weight" in need else None, w, z, "silu", need=need)))
+    for name in full:
+        assert torch.equal(got[name], full[name]) if name in need else got[name] is None
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_backward_strides(dt):
+    m, n, k = 65, 40, 56
+    big = rnd((m, 400), 42, dt)
+    wbig = rnd((n, k + 5), 43, dt)
+    for dy, x, z, w in ((big[:, 1:1 + n], big[:, 100:100 + k], big[:, 203:203 + n], wbig[:, 3:3 + k]),
+                        (big[:, :2 * n:2], big[:, 96:96 + k], big[:, 200:200 + n], wbig[:, :k]),
+                        (big[:1, :n].expand(m, n), big[:, 96:96 + k], big[:, 200:200 + n], wbig[:, :k])):
+        check_backward(dy, x.double(), w, z.double(), "gelu_tanh",
+                       *api.linear_backward(dy, x, w, z, "gelu_tanh"))
+        check_backward(dy, x.double(), w, z.double(), "none", *api.linear_backward(dy, x, w))
+    dy3, x3 = rnd((3, 4, n), 44, dt), rnd((3, 4, k), 45, dt)
+    dx, dw, db = api.linear_backward(dy3, x3, wbig[:, :k])
+    assert dx.shape == (3, 4, k) and dw.shape == (n, k) and db.shape == (n,)
+    check_backward(dy3.reshape(12, n), x3.reshape(12, k).double(), wbig[:, :k], None, "none",
+                   dx.reshape(12, k), dw, db)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_backward_empty(dt):
+    w = rnd((6, 8), 46, dt)
+    e = lambda *s: torch.empty(*s, device=DEV, dtype=dt)  # noqa: E731
+    dx, dw, db = api.linear_backward(e(0, 6), e(0, 8), w, e(0, 6), "gelu")
+    assert dx.shape == (0, 8) and (dw == 0).all() and (db == 0).all()
+    dx, dw, db = api.linear_backward(e(3, 0), e(3, 8), e(0, 8), e(3, 0), "gelu")
+    assert (dx == 0).all() and dx.shape == (3, 8) and dw.shape == (0, 8) and db.shape == (0,)
+    dy = rnd((3, 6), 47, dt)
+    dx, dw, db = api.linear_backward(dy, e(3, 0), e(6, 0))
+    assert dx.shape == (3, 0) and dw.shape == (6, 0)
+    near(db, dy.double().sum(0), 2e-6 * dy.double().abs().sum(0) + u(dt) * dy.double().sum(0).abs())
+    xp, zp = api.pack_activation(e(0, 8)), api.pack_activation(e(0, 6))
+    dx, dw, db = api.linear_backward(e(0, 6), xp, w, zp, "silu")
+    assert (dw == 0).all() and (db == 0).all()
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_gradients_against_differences(act):
+    # central differences of the FP64 formula's loss sum(y * c) around the FP32 inputs
+    m, n, k = 4, 5, 6
+    x, w, b, c = rnd((m, k), 50, FP), rnd((n, k), 51, FP), rnd((n,), 52, FP), rnd((m, n), 53, FP)
+    _, z = api.linear(x, w, b, None, act, keep="plain")
+    dx, dw, db = api.linear_backward(c, x, w, z, act)
+
+    def loss(x, w, b):
+        return (act64(x @ w.mT + b, act)[0] * c.double()).sum()
+
+    args = [t.double() for t in (x, w, b)]
+    for i, g in enumerate((dx, dw, db)):
+        for j in range(g.numel()):
+            h = 1e-5
+            vals = []
+            for sgn in (1, -1):
+                moved = [t.clone() for t in args]
+                moved[i].view(-1)[j] += sgn * h
+                vals.append(loss(*moved).item())
+            # h^2 / 6 * |third derivative| and cancellation are below 1e-8; FP32 results 1e-5
+            assert abs((vals[0] - vals[1]) / (2 * h) - g.view(-1)[j].item()) < 3e-5
+
+
+# ---------------------------------------------------------------------------
+# packed form
+# ---------------------------------------------------------------------------
+def pack64(x):
+    """Codes and exponents from the definition, in 64 bits on the CPU."""
+    lo, hi = (-24, 10) if x.dtype == HF else (-126, 122)
+    v = x.detach().cpu().double().reshape(-1, x.shape[-1])
+    rows, c = v.shape
+    v = torch.nn.functional.pad(v, (0, -c % 32)).view(rows, -1, 32)
+    fin = torch.isfinite(v)
+    amax = torch.where(fin, v, 0.0).abs().amax(-1)
+    e = torch.full(amax.shape, lo)
+    for p in range(lo, hi):  # the smallest step that holds amax
+        e = torch.where(amax > 127 * 2.0**p, p + 1, e)
+    e = e.clamp(lo, hi)
+    most = torch.where(e == hi, 63.0, 127.0)[..., None]
+    q = torch.where(fin, v, 0.0) / torch.ldexp(torch.ones(e.shape, dtype=torch.float64), e)[..., None]
+    q = torch.minimum(torch.maximum(q.round(), -most), most)
+    q = torch.where(fin, q, -128.0)
+    return (q.view(rows, -1)[:, :c].to(torch.int8).reshape(x.shape),
+            e.to(torch.int8).reshape(*x.shape[:-1], -1))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 31), (5, 32), (2, 33), (7, 64), (4, 200), (1, 5000),
+                                   (1000, 40), (130, 257), (2, 3, 48), (17,)])
+def test_pack_is_the_definition(shape, dt):
+    x = rnd(shape, 60, dt) * torch.exp(2 * rnd((*shape[:-1], 1), 61, FP)).to(dt)
+    p = api.pack_activation(x)
+    q, e = pack64(x)
+    assert torch.equal(p.codes.cpu(), q) and torch.equal(p.exponents.cpu(), e)
+    back = api.unpack_activation(p)
+    want = torch.ldexp(q.double(), e.int().repeat_interleave(32, dim=-1)[..., :shape[-1]])
+    assert back.dtype == dt and torch.equal(back.double().cpu(), want)
+    assert torch.equal(api.unpack_activation(api.pack_activation(back)), back)  # nothing lost twice
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_pack_special_values(dt):
+    big, tiny = torch.finfo(dt).max, torch.finfo(dt).smallest_normal
+    rows = torch.zeros(12, 64, dtype=dt)
+    rows[1] = big
+    rows[2, ::2] = -big
+    rows[3] = tiny
+    rows[4, 3], rows[4, 4], rows[4, 5], rows[4, 6] = float("nan"), float("inf"), -float("inf"), 1.0
+    rows[5] = float("inf")
+    rows[6] = 127.0
+    rows[7, :32] = torch.arange(32) * 0.5 + 0.25
+    rows[7, 32] = 127 * 2.0**-7
+    rows[8] = tiny / 4
+    rows[9, 0], rows[9, 1:32] = 1.0, 2.0**-8  # half a step: to even, zero
+    rows[10, 0], rows[10, 1:32] = 1.0, 3 * 2.0**-8
+    rows[11] = -0.0
+    p = api.pack_activation(rows.to(DEV))
+    q, e = pack64(rows)
+    assert torch.equal(p.codes.cpu(), q) and torch.equal(p.exponents.cpu(), e)
+    back = api.unpack_activation(p).cpu()
+    assert torch.equal(back.isnan(), ~rows.isfinite())
+    assert not back.isinf().any()
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_pack_strides(dt):
+    big = rnd((40, 300), 62, dt)
+    for x in (big[:, 1:100], big[:, ::3], big.t(), big[:1].expand(40, 300), big[:, 8:136]):
+        p = api.pack_activation(x)
+        q, e = pack64(x)
+        assert torch.equal(p.codes.cpu(), q) and torch.equal(p.exponents.cpu(), e)
+    p = api.pack_activation(big)
+    # codes and exponents that are views
+    wide = api.PackedActivation(p.codes.repeat(1, 2)[:, :300], p.exponents.repeat(1, 2)[:, :10], dt)
+    assert torch.equal(api.unpack_activation(wide), api.unpack_activation(p))
+    assert api.pack_activation(torch.empty(0, 5, device=DEV, dtype=dt)).codes.shape == (0, 5)
+    assert api.unpack_activation(api.pack_activation(torch.empty(3, 0, device=DEV, dtype=dt))).shape == (3, 0)
+
+
+def test_offsets_beyond_32_bits():
+    rows, cols = 70_001, 32_768  # 2.29e9 values
+    x = torch.empty(rows, cols, device=DEV, dtype=BF)
+    x.copy_(rnd((1, cols), 63, BF).expand(rows, cols))
+    x[-1] = rnd((cols,), 64, BF)
+    p = api.pack_activation(x)
+    del x
+    back = api.unpack_activation(p)
+    for r in (0, 65_536, rows - 2, rows - 1):
+        want = rnd((1, cols), 64 if r == rows - 1 else 63, BF)
+        assert torch.equal(back[r:r + 1], api.unpack_activation(api.pack_activation(want)))
+    del p, back
+    m, n, k = 600_011, 4096, 64  # y and dy: 2.46e9 values
+    xs, w = rnd((m, k), 65, BF), rnd((n, k), 66, BF, 0.125)
+    y = api.linear(xs, w)
+    for r in (slice(0, 200), slice(m - 200, m)):
+        check_forward(xs[r], w, None, None, "none", y[r].contiguous())
+    dx, _, _ = api.linear_backward(y, None, w, need=("x",))
+    for r in (slice(0, 100), slice(m - 100, m)):
+        check_backward(y[r].contiguous(), None, w, None, "none", dx[r].contiguous(), None, None)
+
+
+# ---------------------------------------------------------------------------
+# together, streams, graphs, refusals
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("kept", ["plain", "packed"])
+def test_two_layers_and_the_statistics_of_their_gradient(kept):
+    # x -> gelu(x W1^T + b1) -> (. W2^T + b2) + x, backward, S = dW1 dW1^T, its QR
+    m, d, h = 256, 96, 192
+    x, w1, b1 = rnd((m, d), 70, FP), rnd((h, d), 71, FP, d**-0.5), rnd((h,), 72, FP, 0.1)
+    w2, b2, dy = rnd((d, h), 73, FP, h**-0.5), rnd((d,), 74, FP, 0.1), rnd((m, d), 75, FP)
+    a, z = api.linear(x, w1, b1, None, "gelu", keep=kept)
+    y = api.linear(a, w2, b2, x)
+    ka, kx = (api.pack_activation(a), api.pack_activation(x)) if kept == "packed" else (a, x)
+    da, dw2, db2 = api.linear_backward(dy, ka, w2)
+    dx, dw1, db1 = api.linear_backward(da, kx, w1, z, "gelu")
+    dx = dx + dy
+
+    t = [v.double().requires_grad_() for v in (x, w1, b1, w2, b2)]
+    a64 = torch.nn.functional.gelu(t[0] @ t[1].mT + t[2])
+    y64 = a64 @ t[3].mT + t[4] + t[0]
+    grads = torch.autograd.grad((y64 * dy.double()).sum(), t)
+    assert (y - y64).abs().max() < 2e-5 * y64.abs().max()
+    # packed: a kept value is off by half a step at most, and a step is at most 1/63.5 of the
+    # block's largest, so the root mean square error is below amax / (127 sqrt(3)) = amax / 220.
+    # The largest of 32 normal values is 2.5 at most in the root mean square over blocks: 0.0114,
+    # 1.2 % of x (rms 1) and 1.8 % of gelu(z) (rms 0.65). gelu' changes by at most 0.8 of z's
+    # error, 0.0091, of its rms 0.67: 1.4 % of dz. dw1 has x's and dz's: 2.6 % in sum.
+    tol = 2e-5 if kept == "plain" else 0.026
+    for got, want in zip((dx, dw1, db1, dw2, db2), grads):
+        assert (got - want).norm() <= tol * want.norm()
+    H, tau = api.gram_geqrf(dw1)
+    assert checker.check(api.gram(dw1), H, tau).passed
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_same_bits_every_time(dt):
+    x, w, b = rnd((200, 1000), 80, dt), rnd((130, 1000), 81, dt, 0.03), rnd((130,), 82, dt)
+    dy = rnd((200, 130), 83, dt)
+    runs = []
+    for _ in range(3):
+        y, z = api.linear(x, w, b, None, "silu", keep="plain")
+        runs.append((y, z, *api.linear_backward(dy, x, w, z, "silu")))
+    for r in runs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(runs[0], r))
+
+
+def _step(x, w, b, dy):
+    y, z = api.linear(x, w, b, x[:, :w.shape[0]], "gelu", keep="packed")
+    return (y, *api.linear_backward(dy, api.pack_activation(x), w, z, "gelu"))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_captured_and_replayed(dt):
+    m, n, k = 70, 48, 520
+    new = [(rnd((m, k), 90 + i, dt), rnd((n, k), 95 + i, dt, 0.05), rnd((n,), 100 + i, dt),
+            rnd((m, n), 105 + i, dt)) for i in range(3)]
+    want = [_step(*a) for a in new]
+    held = [t.clone() for t in new[0]]
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs over the same inputs, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _step(*held)
+        graphs.append((g, out))
+    for i in (1, 2, 0):
+        for t, s in zip(held, new[i]):
+            t.copy_(s)
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want[i]))
+
+
+def test_other_streams_and_threads():
+    dt = BF
+    data = [(rnd((300, 256), 110 + i, dt), rnd((192, 256), 120 + i, dt, 0.05), rnd((192,), 130 + i, dt),
+             rnd((300, 192), 140 + i, dt)) for i in range(4)]
+    want = [_step(*a) for a in data]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(10):
+                got[i] = _step(*data[i])
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for p, q in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(p, q))
+
+
+def test_refusals():
+    x, w = rnd((4, 8), 150, BF), rnd((6, 8), 151, BF)
+    dy, z = rnd((4, 6), 152, BF), rnd((4, 6), 153, BF)
+    pk = api.pack_activation
+    cases = [
+        (TypeError, lambda: api.linear(x, w.half())),
+        (TypeError, lambda: api.linear(x, w, rnd((6,), 1, FP))),
+        (ValueError, lambda: api.linear(x, w[:, :7])),
+        (ValueError, lambda: api.linear(x, w[0])),
+        (ValueError, lambda: api.linear(x, w, rnd((5,), 1, BF))),
+        (ValueError, lambda: api.linear(x, w, None, rnd((4, 5), 1, BF))),
+        (ValueError, lambda: api.linear(x, w, activation="tanh")),
+        (ValueError, lambda: api.linear(x, w, activation=None)),
+        (ValueError, lambda: api.linear(x, w, keep="fp8")),
+        (ValueError, lambda: api.linear(x, w.cpu())),
+        (ValueError, lambda: api.linear_backward(dy, x, w, None, "silu")),
+        (ValueError, lambda: api.linear_backward(dy, None, w)),
+        (ValueError, lambda: api.linear_backward(dy, x[:3], w)),
+        (ValueError, lambda: api.linear_backward(dy[:, :5], x, w)),
+        (ValueError, lambda: api.linear_backward(dy, x, w, z[:, :5], "silu")),
+        (ValueError, lambda: api.linear_backward(dy, x, w, pk(z), "relu")),
+        (ValueError, lambda: api.linear_backward(dy, pk(x[:, :7]), w)),
+        (TypeError, lambda: api.linear_backward(dy, pk(x.half()), w)),
+        (ValueError, lambda: api.linear_backward(dy, x, w, need=("y",))),
+        (ValueError, lambda: api.linear_backward(dy, x, w, need="x")),
+        (ValueError, lambda: api.unpack_activation(pk(x)._replace(exponents=pk(x).exponents[:3]))),
+        (TypeError, lambda: api.unpack_activation(pk(x)._replace(codes=x))),
+    ]
+    for exc, call in cases:
+        with pytest.raises(exc):
+            call()
+    wg = w.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient"):
+        api.linear(x, wg)
+    with torch.no_grad():
+        assert torch.equal(api.linear(x, wg), api.linear(x, w))
+
+
+def test_withheld_products_time_out_and_the_next_call_works():
+    x, w = rnd((300, 512), 160, BF), rnd((300, 512), 161, BF)
+    want = api.linear(x, w)
+    torch.cuda.synchronize()
+    hooks = {"wait_limit": 2_000_000, "test_skip_mma": 1, "sync_check": 1}
+    old = {k: _lib.get_config(k) for k in hooks}
+    try:
+        for k, v in hooks.items():
+            _lib.set_config(k, v)
+        with pytest.raises(_lib.QRBError) as ei:
+            api.linear(x, w)
+        assert ei.value.status == 7
+    finally:
+        for k, v in old.items():
+            _lib.set_config(k, v)
+        _lib.set_config("device_error", 0)
+    assert torch.equal(api.linear(x, w), want)
