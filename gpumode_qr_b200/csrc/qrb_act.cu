@@ -10,7 +10,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kVals = 8;     // values per thread and row
-constexpr int kSumRows = 64; // rows of one block's column sums
 
 // Threads tx over the columns (8 each), 256 / tx over the rows.
 struct Grid2 {
@@ -31,15 +30,23 @@ Grid2 grid2(int64_t rows, int64_t cols, int rows_per_thread, bool* ok) {
   return g;
 }
 
-template <int V>
-__device__ __forceinline__ void load_codes(const int8_t* p, bool vec, int valid, int (&q)[V]) {
-  if (vec && valid >= V) {
-    const Vec<int8_t, V> u = *reinterpret_cast<const Vec<int8_t, V>*>(p);
+// Eight codes: one access where they are all there and aligned.
+__device__ __forceinline__ uint2 load_codes(const int8_t* p, bool vec, int valid) {
+  if (vec && valid >= kVals) return *reinterpret_cast<const uint2*>(p);
+  uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < V; ++i) q[i] = u.v[i];
-  } else {
+  for (int i = 0; i < kVals; ++i)
+    if (i < valid) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void decode8(uint2 q, float step, float (&out)[kVals]) {
+  float lo[4], hi[4];
+  decode4(q.x, step, lo);
+  decode4(q.y, step, hi);
 #pragma unroll
-    for (int i = 0; i < V; ++i) q[i] = i < valid ? p[i] : 0;
+  for (int i = 0; i < 4; ++i) {
+    out[i] = lo[i];
+    out[4 + i] = hi[i];
   }
 }
 
@@ -54,6 +61,7 @@ __global__ void __launch_bounds__(kThreads)
            int8_t* __restrict__ codes, int8_t* __restrict__ exps, int vin, int vout) {
   const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * kVals;
   const int64_t r0 = (int64_t)blockIdx.x * blockDim.y * ROWS + threadIdx.y;
+  constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
   float v[ROWS][kVals];
   const int valid = (int)(cols - c < kVals ? (cols > c ? cols - c : 0) : kVals);
 #pragma unroll
@@ -64,24 +72,41 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int j = 0; j < ROWS; ++j) {
     const int64_t r = r0 + (int64_t)j * blockDim.y;
-    float a = 0.f;
+    float a = fabsf(v[j][0]);
 #pragma unroll
-    for (int i = 0; i < kVals; ++i) a = fmaxf(a, finite_f(v[j][i]) ? fabsf(v[j][i]) : 0.f);
-    a = fmaxf(a, __shfl_xor_sync(kFull, a, 1));
-    a = fmaxf(a, __shfl_xor_sync(kFull, a, 2));
-    const int e = block_exponent(a, ExpRange<T>::lo, ExpRange<T>::hi);
-    const float scale = pow2f(-e), most = e == ExpRange<T>::hi ? 63.f : 127.f;
+    for (int i = 1; i < kVals; ++i) a = max_abs_nan(a, v[j][i]);
+    a = max_abs_nan(a, __shfl_xor_sync(kFull, a, 1));
+    a = max_abs_nan(a, __shfl_xor_sync(kFull, a, 2));
+    if (__any_sync(kFull, !finite_f(a))) {
+      const bool fine = finite_f(a);
+      float f = finite_amax(v[j]);
+      f = fmaxf(f, __shfl_xor_sync(kFull, f, 1));
+      f = fmaxf(f, __shfl_xor_sync(kFull, f, 2));
+      if (!fine) {  // Inf or NaN in this block: its exponent from the rest
+        const int e = block_exponent(f, lo, hi);
+        uint32_t w[2];
+        encode(v[j], e, false, e == hi ? 63.f : 127.f, w);
+        if (r < rows && valid > 0) {
+          int8_t* out = codes + r * cols + c;
+#pragma unroll
+          for (int i = 0; i < kVals; ++i)
+            if (i < valid) out[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+          if ((threadIdx.x & 3) == 0) exps[r * nblk + c / kBlk] = (int8_t)e;
+        }
+        continue;
+      }
+    }
+    const int e = block_exponent(a, lo, hi);
+    uint32_t w[2];
+    encode(v[j], e, plain_block(a, e, hi), 63.f, w);
     if (r >= rows || valid == 0) continue;
-    Vec<int8_t, kVals> q;
-#pragma unroll
-    for (int i = 0; i < kVals; ++i) q.v[i] = (int8_t)code_of(v[j][i], scale, most);
     int8_t* out = codes + r * cols + c;
     if (vout && valid >= kVals) {
-      *reinterpret_cast<Vec<int8_t, kVals>*>(out) = q;
+      *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
     } else {
 #pragma unroll
       for (int i = 0; i < kVals; ++i)
-        if (i < valid) out[i] = q.v[i];
+        if (i < valid) out[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
     }
     if ((threadIdx.x & 3) == 0) exps[r * nblk + c / kBlk] = (int8_t)e;
   }
@@ -103,11 +128,8 @@ __global__ void __launch_bounds__(kThreads)
   for (int j = 0; j < ROWS; ++j) {
     const int64_t r = r0 + (int64_t)j * blockDim.y;
     if constexpr (PACKED) {
-      int q[kVals];
-      load_codes<kVals>(codes + r * cols + c, vin, r < rows ? valid : 0, q);
-      const float step = r < rows ? pow2f(exps[r * nblk + c / kBlk]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < kVals; ++i) v[j][i] = value_of(q[i], step);
+      const uint2 q = load_codes(codes + r * cols + c, vin, r < rows ? valid : 0);
+      decode8(q, r < rows ? pow2f(exps[r * nblk + c / kBlk]) : 0.f, v[j]);
     } else {
       load_n<T, kVals>(x + r * ld + c, vin, r < rows ? valid : 0, v[j]);
     }
@@ -133,69 +155,95 @@ __global__ void __launch_bounds__(kThreads)
 // ---------------------------------------------------------------------------
 // dz = dy act'(z), and its column sums
 // ---------------------------------------------------------------------------
-// A block takes kSumRows rows of its columns; each thread sums its rows in
-// order, then the block's row groups are added in order: the same bits every
-// time. part[blockIdx.x][col].
+// Warps of 256 columns (8 per lane), 8 warps over the rows; a block takes `rows`
+// rows of them, 2 per warp at a time so that their loads are in flight
+// together. Each thread sums its rows in order, then the block's warps are
+// added in order: the same bits every time. part[blockIdx.x][col].
+constexpr int kDzRows = 2;
+template <bool EXACT, int ACT>
+__device__ __forceinline__ void dz8(float (&d)[kVals], const float (&z)[kVals]) {
+#pragma unroll
+  for (int i = 0; i < kVals; ++i) d[i] *= act_grad_fn<EXACT>(z[i], ACT);
+}
 template <typename T, bool PACKED, bool PLANES>
-__global__ void __launch_bounds__(kThreads)
-    k_dz(DzArgs a, int64_t nblk, int vdy, int vz, int vdst) {
-  __shared__ float sums[kThreads * kVals];
-  const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * kVals;
-  const int64_t rb = (int64_t)blockIdx.x * kSumRows;
-  const int64_t rend = rb + kSumRows < a.m ? rb + kSumRows : a.m;
-  const int valid = (int)(a.n - c < kVals ? (a.n > c ? a.n - c : 0) : kVals);
+__global__ void __launch_bounds__(kThreads, 3)
+    k_dz(DzArgs a, int64_t nblk, int rows, int vdy, int vz, int vdst) {
+  __shared__ float sums[8][32 * kVals];
   constexpr bool EXACT = sizeof(T) == 4;
+  const int lane = threadIdx.x, warp = threadIdx.y;
+  const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * kVals;
+  const int64_t rb = (int64_t)blockIdx.x * rows;
+  const int64_t rend = rb + rows < a.m ? rb + rows : a.m;
+  const int valid = (int)(a.n - c < kVals ? (a.n > c ? a.n - c : 0) : kVals);
   float acc[kVals];
 #pragma unroll
   for (int i = 0; i < kVals; ++i) acc[i] = 0.f;
   if (valid > 0) {
-#pragma unroll 2
-    for (int64_t r = rb + threadIdx.y; r < rend; r += blockDim.y) {
-      float g[kVals];
-      load_n<T, kVals>(reinterpret_cast<const T*>(a.dy) + r * a.lddy + c, vdy, valid, g);
-      if (a.act != QRBL_ACT_NONE) {
-        float z[kVals];
-        if constexpr (PACKED) {
-          int q[kVals];
-          load_codes<kVals>(a.z_codes + r * a.n + c, vz, valid, q);
-          const float step = pow2f(a.z_exps[r * nblk + c / kBlk]);
+    for (int64_t r0 = rb + warp; r0 < rend; r0 += 8 * kDzRows) {
+      Raw8<T> g[kDzRows], z[kDzRows];
+      uint2 q[kDzRows];
+      int e[kDzRows];
 #pragma unroll
-          for (int i = 0; i < kVals; ++i) z[i] = value_of(q[i], step);
-        } else {
-          load_n<T, kVals>(reinterpret_cast<const T*>(a.z) + r * a.ldz + c, vz, valid, z);
+      for (int j = 0; j < kDzRows; ++j) {
+        const int64_t r = r0 + 8 * j;
+        const int have = r < rend ? valid : 0;
+        g[j] = load_raw8<T>(reinterpret_cast<const T*>(a.dy) + r * a.lddy + c, vdy, have);
+        if (a.act != QRBL_ACT_NONE) {
+          if constexpr (PACKED) {
+            q[j] = load_codes(a.z_codes + r * a.n + c, vz, have);
+            e[j] = have > 0 ? a.z_exps[r * nblk + c / kBlk] : 0;
+          } else {
+            z[j] = load_raw8<T>(reinterpret_cast<const T*>(a.z) + r * a.ldz + c, vz, have);
+          }
         }
-#pragma unroll
-        for (int i = 0; i < kVals; ++i) g[i] *= act_grad_fn<EXACT>(z[i], a.act);
       }
 #pragma unroll
-      for (int i = 0; i < kVals; ++i) acc[i] += g[i];
-      if (a.dst != nullptr) {
+      for (int j = 0; j < kDzRows; ++j) {
+        const int64_t r = r0 + 8 * j;
+        if (r >= rend) break;
+        float d[kVals];
+        values8<T>(g[j], d);
+        if (a.act != QRBL_ACT_NONE) {
+          float f[kVals];
+          if constexpr (PACKED) {
+            decode8(q[j], pow2f(e[j]), f);
+          } else {
+            values8<T>(z[j], f);
+          }
+          switch (a.act) {
+            case QRBL_ACT_RELU: dz8<EXACT, QRBL_ACT_RELU>(d, f); break;
+            case QRBL_ACT_GELU: dz8<EXACT, QRBL_ACT_GELU>(d, f); break;
+            case QRBL_ACT_GELU_TANH: dz8<EXACT, QRBL_ACT_GELU_TANH>(d, f); break;
+            case QRBL_ACT_SILU: dz8<EXACT, QRBL_ACT_SILU>(d, f); break;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) acc[i] += d[i];
+        if (a.dst == nullptr) continue;
         if constexpr (PLANES) {
-          bf16* d = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + c;
+          bf16* out = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + c;
           Vec<bf16, kVals> p[3];
 #pragma unroll
-          for (int i = 0; i < kVals; ++i) split3(g[i], p[0].v[i], p[1].v[i], p[2].v[i]);
+          for (int i = 0; i < kVals; ++i) split3(d[i], p[0].v[i], p[1].v[i], p[2].v[i]);
 #pragma unroll
           for (int k = 0; k < 3; ++k)
-            *reinterpret_cast<Vec<bf16, kVals>*>(d + k * a.plane) = p[k];
+            *reinterpret_cast<Vec<bf16, kVals>*>(out + k * a.plane) = p[k];
         } else {
-          store_n<T, kVals>(reinterpret_cast<T*>(a.dst) + r * a.ldd + c, vdst, valid, g);
+          store_n<T, kVals>(reinterpret_cast<T*>(a.dst) + r * a.ldd + c, vdst, valid, d);
         }
       }
     }
   }
   if (a.part == nullptr) return;
-  const int t = threadIdx.y * blockDim.x + threadIdx.x;
 #pragma unroll
-  for (int i = 0; i < kVals; ++i) sums[t * kVals + i] = acc[i];
+  for (int i = 0; i < kVals; ++i) sums[warp][lane + 32 * i] = acc[i];
   __syncthreads();
-  const int cols = blockDim.x * kVals;  // this block's columns
-  for (int j = t; j < cols; j += kThreads) {
-    float s = 0.f;
-    for (int y = 0; y < (int)blockDim.y; ++y) s += sums[y * cols + j];
-    const int64_t col = (int64_t)blockIdx.y * cols + j;
-    if (col < a.n) a.part[(int64_t)blockIdx.x * a.n + col] = s;
-  }
+  const int t = warp * 32 + lane;  // one column each: lane t / 8, value t % 8
+  float s = 0.f;
+#pragma unroll
+  for (int y = 0; y < 8; ++y) s += sums[y][t / kVals + 32 * (t % kVals)];
+  const int64_t col = (int64_t)blockIdx.y * 256 + t;
+  if (col < a.n) a.part[(int64_t)blockIdx.x * a.n + col] = s;
 }
 
 // out[col] = sum over the blocks of part[block][col]: 32 columns and 8 groups
@@ -248,20 +296,24 @@ __global__ void __launch_bounds__(kThreads)
     if (e.z != nullptr)
       store_n<T, 4>(reinterpret_cast<T*>(e.z) + r * e.ldz + c, e.vec, valid, v);
   }
-  if (e.z_codes != nullptr) {
-    float a = 0.f;
+  if (e.z_codes != nullptr) {  // (the values beyond the row are 0)
+    constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
+    float f = finite_amax(v), a = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      a = fmaxf(a, i < valid && finite_f(v[i]) ? fabsf(v[i]) : 0.f);
+    for (int i = 0; i < 4; ++i) a = max_abs_nan(a, v[i]);
 #pragma unroll
-    for (int o = 1; o < 8; o *= 2) a = fmaxf(a, __shfl_xor_sync(kFull, a, o));
-    const int ex = block_exponent(a, ExpRange<T>::lo, ExpRange<T>::hi);
-    const float scale = pow2f(-ex), most = ex == ExpRange<T>::hi ? 63.f : 127.f;
+    for (int o = 1; o < 8; o *= 2) {
+      f = fmaxf(f, __shfl_xor_sync(kFull, f, o));
+      a = max_abs_nan(a, __shfl_xor_sync(kFull, a, o));
+    }
+    const int ex = block_exponent(f, lo, hi);
+    uint32_t w[1];
+    encode(v, ex, plain_block(a, ex, hi), ex == hi ? 63.f : 127.f, w);
     if (valid > 0) {
       int8_t* out = e.z_codes + r * n + c;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i < valid) out[i] = (int8_t)code_of(v[i], scale, most);
+        if (i < valid) out[i] = (int8_t)(w[0] >> (8 * i));
       if ((threadIdx.x & 7) == 0) e.z_exps[r * ((n + kBlk - 1) / kBlk) + c / kBlk] = (int8_t)ex;
     }
   }
@@ -321,19 +373,18 @@ int stage_t(const void* src, int64_t lds, const int8_t* codes, const int8_t* exp
 template <typename T>
 int dz_t(const DzArgs& a, cudaStream_t s) {
   constexpr bool PLANES = sizeof(T) == 4;
-  bool ok;
-  Grid2 g = grid2(a.m, a.n, 1, &ok);
-  const int64_t gx = (a.m + kSumRows - 1) / kSumRows;
-  if (!ok || gx > 0x7fffffffLL) return QRB_ERR_UNSUPPORTED;
-  g.grid.x = (unsigned)gx;
+  const int rows = colsum_rows(a.m, a.n);
+  const int64_t gx = (a.m + rows - 1) / rows, gy = (a.n + 255) / 256;
+  if (gx > 0x7fffffffLL || gy > 65535) return QRB_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)gx, (unsigned)gy), block(32, 8);
   const int vdy = rows_aligned(a.dy, a.lddy, sizeof(T), 16);
   const int vdst = rows_aligned(a.dst, a.ldd, sizeof(T), 16);
   if (a.z_codes != nullptr)
-    k_dz<T, true, PLANES><<<g.grid, g.block, 0, s>>>(a, blocks_of(a.n), vdy,
-                                                     rows_aligned(a.z_codes, a.n, 1, 8), vdst);
+    k_dz<T, true, PLANES><<<grid, block, 0, s>>>(a, blocks_of(a.n), rows, vdy,
+                                                 rows_aligned(a.z_codes, a.n, 1, 8), vdst);
   else
-    k_dz<T, false, PLANES><<<g.grid, g.block, 0, s>>>(
-        a, blocks_of(a.n), vdy, rows_aligned(a.z, a.ldz, sizeof(T), 16), vdst);
+    k_dz<T, false, PLANES><<<grid, block, 0, s>>>(
+        a, blocks_of(a.n), rows, vdy, rows_aligned(a.z, a.ldz, sizeof(T), 16), vdst);
   return launched();
 }
 
@@ -377,7 +428,11 @@ int launch_stage(int dtype, const void* src, int64_t lds, const int8_t* codes, c
                                                          ldd, plane, s)));
 }
 
-int colsum_rows() { return kSumRows; }
+// 128 rows where that leaves four blocks or more per SM (fewer partial sums to
+// write and add), else 32.
+int colsum_rows(int64_t m, int64_t n) {
+  return ((m + 127) / 128) * ((n + 255) / 256) >= 592 ? 128 : 32;
+}
 
 int launch_dz(int dtype, const DzArgs& a, cudaStream_t s) {
   QRBL_BY_TYPE(dtype, return dz_t<T>(a, s));

@@ -95,6 +95,7 @@ struct Forward {
   Source xs, ws;
   Operand x, w;
   bool stage_x = false, stage_w = false;
+  ProductSize size;
   ProductPlan plan;
   float* part = nullptr;
 };
@@ -104,8 +105,9 @@ Forward plan_forward(const qrbl_linear_args& a, Carve* c) {
   f.ws.p = a.w; f.ws.ld = a.ldw; f.ws.rows = a.n; f.ws.cols = a.k;
   f.x = operand_of(a.dtype, f.xs, c, &f.stage_x);
   f.w = operand_of(a.dtype, f.ws, c, &f.stage_w);
-  f.plan = plan_product(a.dtype, kForward, a.m, a.n, a.k);
-  f.part = reinterpret_cast<float*>(c->take(f.plan.part_bytes));
+  f.size.m = a.m; f.size.n = a.n; f.size.k = a.k;
+  f.plan = plan_products(a.dtype, &f.size, 1);
+  f.part = reinterpret_cast<float*>(c->take(f.plan.part_bytes[0]));
   return f;
 }
 
@@ -133,7 +135,13 @@ int forward(const qrbl_linear_args& a, void* workspace, size_t bytes, cudaStream
   if (c.used > 0 && !aligned16(workspace)) return QRB_ERR_INVALID_ARG;
   if (f.stage_x && (rc = fill(a.dtype, f.xs, f.x, s)) != QRB_OK) return rc;
   if (f.stage_w && (rc = fill(a.dtype, f.ws, f.w, s)) != QRB_OK) return rc;
-  return launch_product(a.dtype, kForward, f.x, f.w, a.m, a.n, a.k, f.plan, f.part, e, s);
+  Product p;
+  p.kind = kForward;
+  p.size = f.size;
+  p.a = f.x; p.b = f.w;
+  p.part = f.part;
+  p.e = e;
+  return launch_products(a.dtype, &p, 1, f.plan, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -175,10 +183,12 @@ struct Backward {
   bool stage_x = false, stage_w = false;
   Source xs, ws;
   Operand dz, x, w;
-  ProductPlan pdx, pdw;
+  ProductSize size[2];  // of the products there are, dW before dx
+  int products = 0;
+  ProductPlan plan;
+  float* part[2] = {nullptr, nullptr};
   float* colsum = nullptr;
   int64_t colsum_blocks = 0;
-  float* part = nullptr;
 };
 Backward plan_backward(const qrbl_linear_backward_args& a, Carve* c) {
   Backward b;
@@ -199,20 +209,25 @@ Backward plan_backward(const qrbl_linear_backward_args& a, Carve* c) {
     b.xs.p = a.x; b.xs.ld = a.ldx; b.xs.rows = a.m; b.xs.cols = a.k;
     b.xs.codes = a.x_codes; b.xs.exps = a.x_exponents;
     b.x = operand_of(a.dtype, b.xs, c, &b.stage_x);
-    b.pdw = plan_product(a.dtype, kGradW, a.n, a.k, a.m);
+    ProductSize& z = b.size[b.products++];
+    z.m = a.n; z.n = a.k; z.k = a.m;
   }
   if (b.dx) {
     b.ws.p = a.w; b.ws.ld = a.ldw; b.ws.rows = a.n; b.ws.cols = a.k;
     b.w = operand_of(a.dtype, b.ws, c, &b.stage_w);
-    b.pdx = plan_product(a.dtype, kGradIn, a.m, a.k, a.n);
+    ProductSize& z = b.size[b.products++];
+    z.m = a.m; z.n = a.k; z.k = a.n;
   }
   if (b.db) {
-    b.colsum_blocks = (a.m + colsum_rows() - 1) / colsum_rows();
+    const int rows = colsum_rows(a.m, a.n);
+    b.colsum_blocks = (a.m + rows - 1) / rows;
     b.colsum = reinterpret_cast<float*>(c->take((size_t)b.colsum_blocks * a.n * sizeof(float)));
   }
-  // the two products run one after the other and share the partial sums
-  const size_t pb = b.pdw.part_bytes > b.pdx.part_bytes ? b.pdw.part_bytes : b.pdx.part_bytes;
-  b.part = reinterpret_cast<float*>(c->take(pb));
+  if (b.products > 0) {
+    b.plan = plan_products(a.dtype, b.size, b.products);
+    for (int i = 0; i < b.products; ++i)
+      b.part[i] = reinterpret_cast<float*>(c->take(b.plan.part_bytes[i]));
+  }
   return b;
 }
 
@@ -258,23 +273,29 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
   auto rows16 = [&](const void* p, int64_t ld, int64_t rows) {
     return aligned16(p) && (rows <= 1 || (ld * es) % 16 == 0);
   };
+  Product p[2];
+  int i = 0;
   if (b.dw) {
     if (b.stage_x && (rc = fill(a.dtype, b.xs, b.x, s)) != QRB_OK) return rc;
-    Epilogue e;
-    e.out = a.dw; e.ldo = a.lddw;
-    e.vec = rows16(a.dw, a.lddw, a.n);
-    rc = launch_product(a.dtype, kGradW, b.dz, b.x, a.n, a.k, a.m, b.pdw, b.part, e, s);
-    if (rc != QRB_OK) return rc;
+    p[i].kind = kGradW;
+    p[i].a = b.dz; p[i].b = b.x;
+    p[i].e.out = a.dw; p[i].e.ldo = a.lddw;
+    p[i].e.vec = rows16(a.dw, a.lddw, a.n);
+    ++i;
   }
   if (b.dx) {
     if (b.stage_w && (rc = fill(a.dtype, b.ws, b.w, s)) != QRB_OK) return rc;
-    Epilogue e;
-    e.out = a.dx; e.ldo = a.lddx;
-    e.vec = rows16(a.dx, a.lddx, a.m);
-    rc = launch_product(a.dtype, kGradIn, b.dz, b.w, a.m, a.k, a.n, b.pdx, b.part, e, s);
-    if (rc != QRB_OK) return rc;
+    p[i].kind = kGradIn;
+    p[i].a = b.dz; p[i].b = b.w;
+    p[i].e.out = a.dx; p[i].e.ldo = a.lddx;
+    p[i].e.vec = rows16(a.dx, a.lddx, a.m);
+    ++i;
   }
-  return QRB_OK;
+  for (int j = 0; j < i; ++j) {
+    p[j].size = b.size[j];
+    p[j].part = b.part[j];
+  }
+  return i == 0 ? QRB_OK : launch_products(a.dtype, p, i, b.plan, s);
 }
 
 int check_packed(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols,

@@ -74,6 +74,55 @@ __device__ __forceinline__ void load_n(const T* p, bool vec, int valid, float (&
   }
 }
 
+// Eight elements as they are in memory, and their values.
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p, bool vec, int valid) {
+  Raw8<T> out;
+  if (vec && valid >= 8) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) out.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    Vec<T, 8> u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u.v[i] = i < valid ? p[i] : from_f<T>(0.f);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) out.w[i] = reinterpret_cast<const uint4*>(&u)[i];
+  }
+  return out;
+}
+template <typename T>
+__device__ __forceinline__ void values2(uint32_t w, float& lo, float& hi) {
+  if constexpr (__is_same(T, bf16)) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void values8(const Raw8<T>& r, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      v[4 * i] = __uint_as_float(r.w[i].x);
+      v[4 * i + 1] = __uint_as_float(r.w[i].y);
+      v[4 * i + 2] = __uint_as_float(r.w[i].z);
+      v[4 * i + 3] = __uint_as_float(r.w[i].w);
+    }
+  } else {
+    values2<T>(r.w[0].x, v[0], v[1]);
+    values2<T>(r.w[0].y, v[2], v[3]);
+    values2<T>(r.w[0].z, v[4], v[5]);
+    values2<T>(r.w[0].w, v[6], v[7]);
+  }
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_n(T* p, bool vec, int valid, const float (&in)[N]) {
   if (vec && valid >= N) {
@@ -185,18 +234,68 @@ __device__ __forceinline__ int block_exponent(float amax, int lo, int hi) {
 __device__ __forceinline__ float pow2f(int e) {  // -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-// x / 2^e rounded to nearest even, at most `most` in magnitude (scale = 2^-e).
-__device__ __forceinline__ int code_of(float x, float scale, float most) {
-  if (!finite_f(x)) return kNanCode;
-  const float q = rintf(x * scale);
-  return (int)fminf(fmaxf(q, -most), most);
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
 }
-__device__ __forceinline__ float value_of(int code, float step) {
-  return code == kNanCode ? __uint_as_float(0x7fc00000u) : (float)code * step;
+// Whether a block whose largest magnitude is amax (by max_abs_nan) and whose
+// exponent is e takes the short path of encode: all values finite, and none
+// rounds above its limit.
+__device__ __forceinline__ bool plain_block(float amax, int e, int hi) {
+  return finite_f(amax) && e < hi;
 }
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-  return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) |
-         ((uint32_t)(d & 255) << 24);
+// Codes of N values of a block, x / 2^e rounded to nearest even. Short path:
+// x * 2^-e (exact) added to 1.5 * 2^23 in one rounding leaves the integer in
+// the sum's low byte. Otherwise Inf and NaN get kNanCode and the rest is held
+// to `most`.
+template <int N>
+__device__ __forceinline__ void encode(const float (&v)[N], int e, bool plain, float most,
+                                       uint32_t (&w)[N / 4]) {
+  const float scale = pow2f(-e);
+  if (plain) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      uint32_t t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = __float_as_uint(fmaf(v[i + j], scale, 12582912.f));
+      w[i / 4] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040),
+                             0x5410);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      uint32_t t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float q = fminf(fmaxf(rintf(v[i + j] * scale), -most), most);
+        t[j] = (uint32_t)(finite_f(v[i + j]) ? (int)q : kNanCode) & 255u;
+      }
+      w[i / 4] = t[0] | (t[1] << 8) | (t[2] << 16) | (t[3] << 24);
+    }
+  }
+}
+// The largest finite magnitude (the short path's amax where all are finite).
+template <int N>
+__device__ __forceinline__ float finite_amax(const float (&v)[N]) {
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) a = fmaxf(a, finite_f(v[i]) ? fabsf(v[i]) : 0.f);
+  return a;
+}
+// Four codes as values. A byte q + 128 put under the exponent of 2^23 is the
+// float 2^23 + 128 + q; kNanCode (byte 0 after the flip) becomes NaN.
+__device__ __forceinline__ void decode4(uint32_t codes, float step, float (&out)[4]) {
+  const uint32_t y = codes ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    out[i] = (__uint_as_float(__byte_perm(y, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+  if ((y - 0x01010101u) & ~y & 0x80808080u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (((y >> (8 * i)) & 255u) == 0) out[i] = __uint_as_float(0x7fc00000u);
+  }
 }
 
 // An FP32 value as three BF16 parts by truncation: a + b + c == x exactly for
@@ -250,18 +349,29 @@ struct Operand {
 //   kGradW    A = dz [k, m] transposed, B = x [k, n]
 enum ProductKind { kForward = 0, kGradIn = 1, kGradW = 2 };
 
-// How a product is cut: tiles of 128 x bn, `splits` parts of k (their FP32
-// sums joined by a second kernel, part_bytes of workspace).
-struct ProductPlan {
-  int bn = 128;
-  int splits = 1;
-  int64_t part_rows = 0, part_ld = 0;
-  size_t part_bytes = 0;
+struct ProductSize {
+  int64_t m = 0, n = 0, k = 0;
 };
-ProductPlan plan_product(int dtype, int kind, int64_t m, int64_t n, int64_t k);
-int launch_product(int dtype, int kind, const Operand& a, const Operand& b, int64_t m, int64_t n,
-                   int64_t k, const ProductPlan& plan, float* part, const Epilogue& e,
-                   cudaStream_t s);
+struct Product {
+  int kind = kForward;
+  ProductSize size;
+  Operand a, b;
+  float* part = nullptr;  // splits > 1: part_bytes of workspace
+  Epilogue e;
+};
+// How the products of one launch are cut: tiles of 128 cg x bn on cg CTAs, each
+// product's reduction in `splits` parts (their FP32 sums joined by a second
+// kernel), the tiles of product `first` first.
+struct ProductPlan {
+  bool ok = false;
+  int cg = 1, bn = 128, first = 0;
+  int splits[2] = {1, 1};
+  int64_t part_rows[2] = {0, 0}, part_ld[2] = {0, 0};
+  size_t part_bytes[2] = {0, 0};
+};
+ProductPlan plan_products(int dtype, const ProductSize* sizes, int count);
+int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
+                    cudaStream_t s);
 // out = epilogue(sum of `splits` partial sums), part[s][row][col] with rows
 // `rows` and row stride ld (splits may be 0).
 int launch_join(int dtype, const float* part, int splits, int64_t rows, int64_t ld, int64_t m,
@@ -277,9 +387,9 @@ int launch_stage(int dtype, const void* src, int64_t lds, const int8_t* codes, c
                  int64_t rows, int64_t cols, void* dst, int64_t ldd, int64_t plane,
                  cudaStream_t s);
 // dz = dy act'(z) as an operand (dst may be null: only the sums), and the
-// column sums of the unrounded dz over each block of colsum_rows() rows into
-// part [blocks][n] (null: none).
-int colsum_rows();
+// column sums of the unrounded dz over each block of colsum_rows(m, n) rows
+// into part [blocks][n] (null: none).
+int colsum_rows(int64_t m, int64_t n);
 struct DzArgs {
   const void* dy = nullptr;
   int64_t lddy = 0;

@@ -2,16 +2,22 @@
 // tensor cores, operands fed by TMA, for the forward product x W^T and the
 // backward products dz W and dz^T x.
 //
-// Tiles of 128 x BN per CTA over a persistent grid of one CTA per SM. Ten
-// warps: 0-7 read the accumulators (warp w: TMEM lanes 32 (w & 3) .. + 31, one
-// half of the columns by w >> 2) and run the epilogue, 8 loads (one lane
-// issues TMA boxes into a ring of stages), 9 issues the MMAs (one lane) and
-// owns the TMEM. A stage holds 64 of the reduction's values for both operands
-// (128-byte swizzle). An operand whose reduction runs along memory rows is
-// K-major; one whose reduction runs across them (w in dz W, both operands of
+// Tiles of 128 x BN per CTA, or 256 x BN per pair of CTAs (CG = 2: one MMA over
+// both SMs, each holding 128 rows of A and half of B's columns, so a CTA loads
+// two thirds of the bytes), over a persistent grid of one CTA per SM. Ten warps:
+// 0-7 read the accumulators (warp w: TMEM lanes 32 (w & 3) .. + 31, one half of
+// the columns by w >> 2) and run the epilogue, 8 loads (one lane issues TMA
+// boxes into a ring of stages), 9 issues the MMAs (one lane, of the pair's first
+// CTA) and owns the TMEM. A stage holds 64 of the reduction's values for both
+// operands (128-byte swizzle). An operand whose reduction runs along memory rows
+// is K-major; one whose reduction runs across them (w in dz W, both operands of
 // dz^T x) is MN-major, so no operand is ever transposed in memory. Two
 // accumulator buffers let the epilogue of one tile run beside the MMAs of the
 // next.
+//
+// One launch takes one product or two independent ones (dx and dW): each CTA
+// or pair runs its share of the longer tiles first, then as many of the shorter
+// ones as level the load (Schedule), so only one launch has a tail.
 //
 // FP32 operands come as three BF16 planes a0 + a1 + a2 (24 bits). A stage
 // holds all three planes of both operands, and the six products a_i b_j with
@@ -26,7 +32,9 @@
 //
 // Every wait is bounded: a timeout sets a block-wide abort flag and the device
 // error flag; the producer then waits (bounded) for its loads in flight, the
-// MMA warp for its MMAs, and the TMEM is freed.
+// MMA warp for its MMAs, and the TMEM is freed. In a pair each CTA's waits for
+// the other are bounded the same way, and both reach the closing cluster
+// barrier before either exits.
 #include <mutex>
 
 #include "qrb_linear.cuh"
@@ -52,10 +60,11 @@ constexpr int B_FULL = 0, B_EMPTY = kMaxStages, B_ACCFULL = 2 * kMaxStages,
 constexpr uint32_t OFF_TMEM = NBAR * 8, OFF_ABORT = OFF_TMEM + 4, CTRL = 1024;
 static_assert(OFF_ABORT + 4 <= CTRL, "control block");
 
-template <int BN, typename T>
+template <int CG, int BN, typename T>
 struct Lay {
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // planes
-  static constexpr uint32_t A = BM * 128, B = BN * 128;
+  static constexpr int BROWS = BN / CG;              // B's columns of one CTA
+  static constexpr uint32_t A = BM * 128, B = BROWS * 128;
   static constexpr uint32_t STAGE = NP * (A + B);
   static constexpr int FIT = (int)((kSmemMost - CTRL - 1024) / STAGE);
   static constexpr int ST = FIT < kMaxStages ? FIT : kMaxStages;
@@ -63,41 +72,76 @@ struct Lay {
   static constexpr int ACC = NP == 3 ? 2 * BN : BN;  // TMEM columns per buffer
   static constexpr int TMEM = 2 * ACC;
   static_assert(ST >= 2 && TMEM <= 512 && TMEM >= 32, "stage ring and TMEM");
+  static_assert(BROWS % 64 == 0, "MN-major atoms");
 };
 
-struct Args {
+struct Problem {
   int m, n;
   int mt, nt;       // tiles
   int kb;           // stages of the whole reduction
   int splits;
   int items;        // mt * nt * splits
   int group;        // tile rows that run together (operand reuse in L2)
+  int amn, bmn;     // operands are MN-major
   float* part;      // splits > 1: partial tiles
   long long part_rows, part_ld;
   Epilogue e;
   int vcodes;       // packed rows are 16-byte aligned
+};
+// Which items a worker (CTA or pair) runs: of problem 0 every workers-th,
+// worker by worker; then of problem 1 its count, x or (with one more of
+// problem 0: worker < r) y <= x. The first (x - y) rounds have only the
+// workers >= r, the later ones all of them.
+struct Schedule {
+  int workers;
+  int q, r;         // problem 0: q items each, one more for the first r workers
+  int x, y;
+};
+struct Args {
+  Problem p[2];
+  Schedule s;
   int* err;
   long long limit;
   int skip_mma;     // test hook: withhold the MMAs, so that the waits run out
 };
 
 struct Item {
+  int prob;         // -1: no more
   int m0, n0, kb0, kb1, split;
 };
-template <int BN>
-__device__ __forceinline__ Item item_of(const Args& a, int item) {
-  const int tiles = a.mt * a.nt;
+template <int CG, int BN>
+__device__ __forceinline__ Item item_of(const Args& a, int worker, int step) {
+  const Schedule& s = a.s;
   Item it;
+  int item;
+  const int own = s.q + (worker < s.r ? 1 : 0);
+  if (step < own) {
+    it.prob = 0;
+    item = step * s.workers + worker;
+  } else {
+    const int j = step - own, lead = s.x - s.y, late = s.workers - s.r;
+    it.prob = j < (worker < s.r ? s.y : s.x) ? 1 : -1;
+    if (worker < s.r)
+      item = lead * late + j * s.workers + worker;
+    else
+      item = j < lead ? j * late + (worker - s.r) : lead * late + (j - lead) * s.workers + worker;
+    if (it.prob < 0 || item >= a.p[1].items) {
+      it.prob = -1;
+      return it;
+    }
+  }
+  const Problem& p = a.p[it.prob];
+  const int tiles = p.mt * p.nt;
   it.split = item / tiles;
   const int t = item - it.split * tiles;
-  const int per = a.group * a.nt;
+  const int per = p.group * p.nt;
   const int g = t / per, r = t - g * per;
-  const int first = g * a.group;
-  const int gm = a.mt - first < a.group ? a.mt - first : a.group;
-  it.m0 = (first + r % gm) * BM;
+  const int first = g * p.group;
+  const int gm = p.mt - first < p.group ? p.mt - first : p.group;
+  it.m0 = (first + r % gm) * (BM * CG);
   it.n0 = (r / gm) * BN;
-  it.kb0 = (int)((long long)a.kb * it.split / a.splits);
-  it.kb1 = (int)((long long)a.kb * (it.split + 1) / a.splits);
+  it.kb0 = (int)((long long)p.kb * it.split / p.splits);
+  it.kb1 = (int)((long long)p.kb * (it.split + 1) / p.splits);
   return it;
 }
 
@@ -109,33 +153,131 @@ __device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo, uint32_t 
 // K-major: rows of 128 bytes, 8-row groups 1024 bytes apart; 16 reduction
 // values are 32 bytes. MN-major: 64-value atoms ATOM apart, 8-row (reduction)
 // groups 1024 bytes apart; 16 reduction rows are 2048 bytes.
-template <bool MN>
-__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
-  return MN ? desc(saddr, ATOM, 1024) : desc(saddr, 16, 1024);
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, bool mn) {
+  return desc(saddr, mn ? ATOM : 16, 1024);
 }
-template <bool MN>
-constexpr uint64_t kStep = MN ? 2048 >> 4 : 32 >> 4;
 
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
                                         uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+}
+// An arrival on the barrier (of both CTAs of a pair) once every MMA issued so
+// far is done.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    tc::mma_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"((unsigned short)3)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t columns) {
+  if constexpr (CG == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns)
+                 : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns)
+                 : "memory");
+}
+// Every thread of the block, or of both blocks of a pair.
+template <int CG>
+__device__ __forceinline__ void sync_all() {
+  if constexpr (CG == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+// The same shared-memory address in the pair's first CTA.
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+template <int CG>
+__device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity) {
+  if constexpr (CG == 1) return tma::mbar_try(bar, parity);
+  uint32_t done;  // the arrivals may come from the other CTA
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(accumulate)
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
       : "memory");
+  return done != 0;
+}
+// Bounded: false on a timeout (which sets *abort) or once *abort is set.
+template <int CG>
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, long long limit,
+                                              volatile int* abort) {
+  if (mbar_done<CG>(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_done<CG>(bar, parity)) {
+    if (*abort != 0) return false;
+    if (clock64() - t0 > limit) {
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
 }
 
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                         int y, int z) {
+  if constexpr (CG == 1)
+    tma::load_3d(dst, map, bar, x, y, z);
+  else  // into this CTA's memory, announced on the first CTA's barrier
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
 // One operand's tile of one stage.
-template <bool MN, int ROWS>
-__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                          int mn0, int kb, int plane) {
-  if constexpr (MN) {
+template <int CG, int ROWS>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, bool mn,
+                                          uint32_t bar, int mn0, int kb, int plane) {
+  if (mn) {
 #pragma unroll
     for (int j = 0; j < ROWS / 64; ++j)
-      tma::load_3d(dst + j * ATOM, map, bar, mn0 + 64 * j, kb * BK, plane);
+      load_box<CG>(dst + j * ATOM, map, bar, mn0 + 64 * j, kb * BK, plane);
   } else {
-    tma::load_3d(dst, map, bar, kb * BK, mn0, plane);
+    load_box<CG>(dst, map, bar, kb * BK, mn0, plane);
   }
 }
 
@@ -147,7 +289,7 @@ __device__ __forceinline__ void act32(float (&v)[32]) {
 
 // The epilogue of 32 consecutive columns of one row (one thread).
 template <typename T, bool FWD>
-__device__ __forceinline__ void finish32(float (&v)[32], int row, int col, const Args& a) {
+__device__ __forceinline__ void finish32(float (&v)[32], int row, int col, const Problem& a) {
   if (row >= a.m || col >= a.n) return;
   const int valid = a.n - col < 32 ? a.n - col : 32;
   const Epilogue& e = a.e;
@@ -161,25 +303,24 @@ __device__ __forceinline__ void finish32(float (&v)[32], int row, int col, const
     if (e.z != nullptr)
       store_n<T, 32>(reinterpret_cast<T*>(e.z) + (int64_t)row * e.ldz + col, e.vec, valid, v);
     if (e.z_codes != nullptr) {
-      float amax = 0.f;
+      constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
+      float amax = 0.f;  // columns beyond n are 0: the operand's rows there read as 0
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        amax = fmaxf(amax, i < valid && finite_f(v[i]) ? fabsf(v[i]) : 0.f);
-      const int ex = block_exponent(amax, ExpRange<T>::lo, ExpRange<T>::hi);
-      const float scale = pow2f(-ex), most = ex == ExpRange<T>::hi ? 63.f : 127.f;
+      for (int i = 0; i < 32; ++i) amax = max_abs_nan(amax, v[i]);
+      const bool fine = finite_f(amax);
+      if (!fine) amax = finite_amax(v);
+      const int ex = block_exponent(amax, lo, hi);
+      const bool plain = fine && ex < hi;
+      uint32_t w[8];
+      encode(v, ex, plain, ex == hi ? 63.f : 127.f, w);
       int8_t* out = e.z_codes + (int64_t)row * a.n + col;
       if (a.vcodes && valid == 32) {
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          w[i] = pack4(code_of(v[4 * i], scale, most), code_of(v[4 * i + 1], scale, most),
-                       code_of(v[4 * i + 2], scale, most), code_of(v[4 * i + 3], scale, most));
         reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
         reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (i < valid) out[i] = (int8_t)code_of(v[i], scale, most);
+          if (i < valid) out[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
       }
       e.z_exps[(int64_t)row * ((a.n + kBlk - 1) / kBlk) + col / kBlk] = (int8_t)ex;
     }
@@ -203,18 +344,19 @@ __device__ __forceinline__ void finish32(float (&v)[32], int row, int col, const
 
 // A split product's partial tile (rows and columns padded to whole tiles).
 __device__ __forceinline__ void partial32(const float (&v)[32], int row, int col, int split,
-                                          const Args& a) {
+                                          const Problem& a) {
   float* p = a.part + ((long long)split * a.part_rows + row) * a.part_ld + col;
 #pragma unroll
   for (int i = 0; i < 32; i += 4)
     *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
 }
 
-template <int BN, bool AMN, bool BMN, typename T, bool FWD>
+template <int CG, int BN, typename T, bool FWD>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+    k_product(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
+              const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
               const __grid_constant__ Args a) {
-  using L = Lay<BN, T>;
+  using L = Lay<CG, BN, T>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = tma::smem_addr(smem_raw);
   const uint32_t pad = (1024 - (raw & 1023)) & 1023;
@@ -224,6 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* s_abort = reinterpret_cast<volatile int*>(sm + OFF_ABORT);
   auto BAR = [&](int i) { return base + 8u * (uint32_t)i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int worker = (int)blockIdx.x / CG, rank = (int)blockIdx.x % CG;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::ST; ++s) {
@@ -232,77 +375,83 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       tma::mbar_init(BAR(B_ACCFULL + b), 1);
-      tma::mbar_init(BAR(B_ACCEMPTY + b), kEpiWarps);
+      tma::mbar_init(BAR(B_ACCEMPTY + b), CG * kEpiWarps);
     }
     tma::mbar_init(BAR(B_FIN), 1);
     tma::mbar_fence_init();
     *s_abort = 0;
   }
-  if (warp == kEpiWarps + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     base + OFF_TMEM),
-                 "n"(L::TMEM)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == kEpiWarps + 1) tmem_alloc<CG>(base + OFF_TMEM, L::TMEM);
   tc::fence_before();
   __syncthreads();
+  if constexpr (CG == 2) sync_all<CG>();
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + OFF_TMEM);
 
   if (warp == kEpiWarps) {  // ---- loads ----
     if (lane == 0) {
-      tma::prefetch_map(&map_a);
-      tma::prefetch_map(&map_b);
+      tma::prefetch_map(&map_a0);
+      tma::prefetch_map(&map_b0);
       int u = 0;  // stages issued
-      for (int item = blockIdx.x; item < a.items && *s_abort == 0; item += gridDim.x) {
-        const Item it = item_of<BN>(a, item);
+      for (int step = 0; *s_abort == 0; ++step) {
+        const Item it = item_of<CG, BN>(a, worker, step);
+        if (it.prob < 0) break;
+        const CUtensorMap* ma = it.prob == 0 ? &map_a0 : &map_a1;
+        const CUtensorMap* mb = it.prob == 0 ? &map_b0 : &map_b1;
+        const bool amn = a.p[it.prob].amn != 0, bmn = a.p[it.prob].bmn != 0;
+        const int am = it.m0 + rank * BM, bn = it.n0 + rank * L::BROWS;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           const int s = u % L::ST;
-          if (u >= L::ST && !tma::mbar_wait_or_abort(BAR(B_EMPTY + s),
-                                                     (uint32_t)((u / L::ST - 1) & 1), a.limit,
-                                                     s_abort))
+          if (u >= L::ST && !wait_or_abort<CG>(BAR(B_EMPTY + s), (uint32_t)((u / L::ST - 1) & 1),
+                                               a.limit, s_abort))
             break;
-          tma::mbar_expect_tx(BAR(B_FULL + s), L::STAGE);
+          if (rank == 0) tma::mbar_expect_tx(BAR(B_FULL + s), CG * L::STAGE);
+          const uint32_t bar = CG == 1 ? BAR(B_FULL + s) : in_first_cta(BAR(B_FULL + s));
           const uint32_t st = ring + s * L::STAGE;
 #pragma unroll
           for (int p = 0; p < L::NP; ++p)
-            load_tile<AMN, BM>(st + p * L::A, &map_a, BAR(B_FULL + s), it.m0, kb, p);
+            load_tile<CG, BM>(st + p * L::A, ma, amn, bar, am, kb, p);
 #pragma unroll
           for (int p = 0; p < L::NP; ++p)
-            load_tile<BMN, BN>(st + L::NP * L::A + p * L::B, &map_b, BAR(B_FULL + s), it.n0, kb,
-                               p);
+            load_tile<CG, L::BROWS>(st + L::NP * L::A + p * L::B, mb, bmn, bar, bn, kb, p);
           ++u;
         }
       }
       if (*s_abort != 0) {  // no load may land after the block has gone
-        for (int v = u > L::ST ? u - L::ST : 0; v < u; ++v)
-          tma::mbar_wait_bounded(BAR(B_FULL + v % L::ST), (uint32_t)((v / L::ST) & 1), a.limit);
+        if constexpr (CG == 1) {
+          for (int v = u > L::ST ? u - L::ST : 0; v < u; ++v)
+            tma::mbar_wait_bounded(BAR(B_FULL + v % L::ST), (uint32_t)((v / L::ST) & 1), a.limit);
+        } else {  // announced on one CTA's barrier: a fixed time, far above any load's
+          const long long t0 = clock64();
+          while (clock64() - t0 < 4000000LL) {
+          }
+        }
       }
     }
   } else if (warp == kEpiWarps + 1) {  // ---- MMAs ----
-    if (lane == 0) {
-      constexpr uint32_t fmt = sizeof(T) == 4 || !__is_same(T, f16) ? 1u : 0u;  // BF16 : F16
-      constexpr uint32_t id = (1u << 4) | (fmt << 7) | (fmt << 10) | ((AMN ? 1u : 0u) << 15) |
-                              ((BMN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
-                              ((uint32_t)(BM >> 4) << 24);
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t fmt = __is_same(T, f16) ? 0u : 1u;  // F16 : BF16
       int u = 0, unit = 0;
-      for (int item = blockIdx.x; item < a.items && *s_abort == 0; item += gridDim.x) {
-        const Item it = item_of<BN>(a, item);
+      for (int step = 0; *s_abort == 0; ++step) {
+        const Item it = item_of<CG, BN>(a, worker, step);
+        if (it.prob < 0) break;
+        const bool amn = a.p[it.prob].amn != 0, bmn = a.p[it.prob].bmn != 0;
+        const uint32_t id = (1u << 4) | (fmt << 7) | (fmt << 10) | ((amn ? 1u : 0u) << 15) |
+                            ((bmn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+                            ((uint32_t)((BM * CG) >> 4) << 24);
+        const uint64_t ka = amn ? 2048 >> 4 : 32 >> 4, kbs = bmn ? 2048 >> 4 : 32 >> 4;
         for (int kb = it.kb0; kb < it.kb1 && *s_abort == 0;) {
           const int end = L::NP == 3 && kb + kChain < it.kb1 ? kb + kChain : it.kb1;
           const int buf = unit & 1;
-          if (unit >= 2 && !tma::mbar_wait_or_abort(BAR(B_ACCEMPTY + buf),
-                                                    (uint32_t)((unit / 2 - 1) & 1), a.limit,
-                                                    s_abort))
+          if (unit >= 2 && !wait_or_abort<CG>(BAR(B_ACCEMPTY + buf),
+                                              (uint32_t)((unit / 2 - 1) & 1), a.limit, s_abort))
             break;
           tc::fence_after();
           const uint32_t d = tmem + buf * L::ACC;
           uint32_t more = 0;
           for (; kb < end; ++kb, ++u) {
             const int s = u % L::ST;
-            if (!tma::mbar_wait_or_abort(BAR(B_FULL + s), (uint32_t)((u / L::ST) & 1), a.limit,
-                                         s_abort))
+            if (!wait_or_abort<CG>(BAR(B_FULL + s), (uint32_t)((u / L::ST) & 1), a.limit, s_abort))
               break;
             tc::fence_after();
             const uint32_t sa = ring + s * L::STAGE, sb = sa + L::NP * L::A;
@@ -311,38 +460,60 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int q = 0; q < (L::NP == 3 ? 6 : 1); ++q) {
                 // (0, 0) into the main accumulator, then the small products
                 constexpr int pi[6] = {0, 0, 1, 1, 0, 2}, pj[6] = {0, 1, 0, 1, 2, 0};
-                const uint64_t da = operand_desc<AMN>(sa + pi[q] * L::A);
-                const uint64_t db = operand_desc<BMN>(sb + pj[q] * L::B);
+                const uint64_t da = operand_desc(sa + pi[q] * L::A, amn);
+                const uint64_t db = operand_desc(sb + pj[q] * L::B, bmn);
                 const uint32_t dq = q == 0 ? d : d + BN;
 #pragma unroll
                 for (int k = 0; k < BK / 16; ++k)
-                  mma_f16(dq, da + k * kStep<AMN>, db + k * kStep<BMN>, id,
-                          more | (q > 1 || k > 0 ? 1u : 0u));
+                  mma_f16<CG>(dq, da + k * ka, db + k * kbs, id,
+                              more | (q > 1 || k > 0 ? 1u : 0u));
               }
               more = 1;
-              tc::mma_commit(BAR(B_EMPTY + s));
+              commit<CG>(BAR(B_EMPTY + s));
             }
           }
           if (*s_abort != 0) break;
-          if (a.skip_mma == 0) tc::mma_commit(BAR(B_ACCFULL + buf));
+          if (a.skip_mma == 0) commit<CG>(BAR(B_ACCFULL + buf));
           ++unit;
         }
       }
-      if (*s_abort != 0) tc::drain_mmas(BAR(B_FIN));
+      if (*s_abort != 0) {  // no MMA may run on into freed TMEM (a pair: fixed time as above)
+        if constexpr (CG == 1) {
+          tc::drain_mmas(BAR(B_FIN));
+        } else {
+          const long long t0 = clock64();
+          while (clock64() - t0 < 4000000LL) {
+          }
+        }
+      }
     }
   } else {  // ---- epilogue ----
     const int quad = warp & 3, half = warp >> 2;
     constexpr int HC = BN / 2;  // columns of this warp
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     int unit = 0;
-    for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
-      const Item it = item_of<BN>(a, item);
-      const int row = it.m0 + quad * 32 + lane, col = it.n0 + half * HC;
+    auto hand_back = [&](int buf) {  // the accumulators are read
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 1)
+          tma::mbar_arrive(BAR(B_ACCEMPTY + buf));
+        else
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                           in_first_cta(BAR(B_ACCEMPTY + buf)))
+                       : "memory");
+      }
+    };
+    for (int step = 0;; ++step) {
+      const Item it = item_of<CG, BN>(a, worker, step);
+      if (it.prob < 0) break;
+      const Problem& p = a.p[FWD ? 0 : it.prob];
+      const int row = it.m0 + rank * BM + quad * 32 + lane, col = it.n0 + half * HC;
       bool ok = true;
       if constexpr (L::NP == 1) {
         const int buf = unit & 1;
-        ok = *s_abort == 0 && tma::mbar_wait_or_abort(BAR(B_ACCFULL + buf),
-                                                      (uint32_t)((unit / 2) & 1), a.limit, s_abort);
+        ok = *s_abort == 0 && wait_or_abort<CG>(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1),
+                                                a.limit, s_abort);
         ok = __all_sync(kFull, ok);
         if (!ok) break;
         tc::fence_after();
@@ -351,15 +522,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < HC; c += 32) {
           float v[32];
           tc::tmem_ld32(t + c, v);
-          if (c + 32 == HC) {  // the accumulators are read: hand the buffer back
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tma::mbar_arrive(BAR(B_ACCEMPTY + buf));
-          }
-          if (a.splits > 1)
-            partial32(v, row, col + c, it.split, a);
+          if (c + 32 == HC) hand_back(buf);
+          if (p.splits > 1)
+            partial32(v, row, col + c, it.split, p);
           else
-            finish32<T, FWD>(v, row, col + c, a);
+            finish32<T, FWD>(v, row, col + c, p);
         }
         ++unit;
       } else {
@@ -370,9 +537,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
         for (int kb = it.kb0; kb < it.kb1; kb += kChain, ++unit) {
           const int buf = unit & 1;
-          ok = *s_abort == 0 &&
-               tma::mbar_wait_or_abort(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit,
-                                       s_abort);
+          ok = *s_abort == 0 && wait_or_abort<CG>(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1),
+                                                  a.limit, s_abort);
           ok = __all_sync(kFull, ok);
           if (!ok) break;
           tc::fence_after();
@@ -385,17 +551,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) sum[c][i] += v[i] + w[i];
           }
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) tma::mbar_arrive(BAR(B_ACCEMPTY + buf));
+          hand_back(buf);
         }
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < HC / 32; ++c) {
-          if (a.splits > 1)
-            partial32(sum[c], row, col + c * 32, it.split, a);
+          if (p.splits > 1)
+            partial32(sum[c], row, col + c * 32, it.split, p);
           else
-            finish32<T, FWD>(sum[c], row, col + c * 32, a);
+            finish32<T, FWD>(sum[c], row, col + c * 32, p);
         }
       }
     }
@@ -404,11 +568,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   tc::fence_before();
   __syncthreads();
+  if constexpr (CG == 2) sync_all<CG>();
   tc::fence_after();
   if (threadIdx.x == 0 && *s_abort != 0) atomicExch(a.err, 1);
-  if (warp == kEpiWarps + 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::TMEM)
-                 : "memory");
+  if (warp == kEpiWarps + 1) tmem_free<CG>(tmem, L::TMEM);
 }
 
 // ---------------------------------------------------------------------------
@@ -449,125 +612,278 @@ const Device* device_info() {
   return info[dev].sms > 0 ? &info[dev] : nullptr;
 }
 
-template <int BN, bool AMN, bool BMN, typename T, bool FWD>
-int launch_t(const Operand& a, const Operand& b, Args& args, const Device& d, cudaStream_t s) {
-  using L = Lay<BN, T>;
+// The kernel for both (or one of the) products, or for a forward product.
+template <int CG, int BN, typename T, bool FWD>
+int launch_t(const Product* const* q, int count, Args& args, const Device& d, cudaStream_t s) {
+  using L = Lay<CG, BN, T>;
   static std::once_flag once[64];
   static bool ready[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QRB_ERR_DEVICE;
   std::call_once(once[dev], [dev] {
-    ready[dev] = cudaFuncSetAttribute(k_product<BN, AMN, BMN, T, FWD>,
+    ready[dev] = cudaFuncSetAttribute(k_product<CG, BN, T, FWD>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)L::SMEM) == cudaSuccess;
   });
   if (!ready[dev]) return QRB_ERR_LAUNCH;
-  CUtensorMap ma, mb;
-  if (!encode16(&ma, a, L::NP, AMN ? BK : BM) || !encode16(&mb, b, L::NP, BMN ? BK : BN))
-    return QRB_ERR_UNSUPPORTED;
-  const int grid = args.items < d.sms ? args.items : d.sms;
-  k_product<BN, AMN, BMN, T, FWD><<<grid, kThreads, L::SMEM, s>>>(ma, mb, args);
+  CUtensorMap ma[2], mb[2];
+  for (int i = 0; i < count; ++i) {
+    if (!encode16(&ma[i], q[i]->a, L::NP, args.p[i].amn ? BK : BM) ||
+        !encode16(&mb[i], q[i]->b, L::NP, args.p[i].bmn ? BK : L::BROWS))
+      return QRB_ERR_UNSUPPORTED;
+  }
+  if (count == 1) {
+    ma[1] = ma[0];
+    mb[1] = mb[0];
+  }
+  if constexpr (CG == 1) {
+    k_product<CG, BN, T, FWD><<<args.s.workers, kThreads, L::SMEM, s>>>(ma[0], mb[0], ma[1], mb[1],
+                                                                        args);
+  } else {
+    cudaLaunchConfig_t lc = {};
+    cudaLaunchAttribute la[1];
+    la[0].id = cudaLaunchAttributeClusterDimension;
+    la[0].val.clusterDim.x = 2;
+    la[0].val.clusterDim.y = 1;
+    la[0].val.clusterDim.z = 1;
+    lc.gridDim = dim3(2 * (unsigned)args.s.workers);
+    lc.blockDim = dim3(kThreads);
+    lc.dynamicSmemBytes = L::SMEM;
+    lc.stream = s;
+    lc.attrs = la;
+    lc.numAttrs = 1;
+    if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD>, ma[0], mb[0], ma[1], mb[1], args) !=
+        cudaSuccess) {
+      (void)cudaGetLastError();
+      return QRB_ERR_LAUNCH;
+    }
+  }
+  (void)d;
   note_launches(1);
   return cudaGetLastError() == cudaSuccess ? QRB_OK : QRB_ERR_LAUNCH;
 }
 
-template <int BN, typename T>
-int launch_kind(int kind, const Operand& a, const Operand& b, Args& args, const Device& d,
-                cudaStream_t s) {
-  switch (kind) {
-    case kForward: return launch_t<BN, false, false, T, true>(a, b, args, d, s);
-    case kGradIn: return launch_t<BN, false, true, T, false>(a, b, args, d, s);
-    case kGradW: return launch_t<BN, true, true, T, false>(a, b, args, d, s);
-  }
-  return QRB_ERR_INVALID_ARG;
+template <int CG, int BN, typename T>
+int launch_dir(bool fwd, const Product* const* q, int count, Args& args, const Device& d,
+               cudaStream_t s) {
+  return fwd ? launch_t<CG, BN, T, true>(q, count, args, d, s)
+             : launch_t<CG, BN, T, false>(q, count, args, d, s);
 }
 
-template <int BN>
-int launch_bn(int dtype, int kind, const Operand& a, const Operand& b, Args& args, const Device& d,
-              cudaStream_t s) {
-  switch (dtype) {
-    case QRBL_F32:
-      if constexpr (BN <= 128) return launch_kind<BN, float>(kind, a, b, args, d, s);
-      return QRB_ERR_INVALID_ARG;
-    case QRBL_F16: return launch_kind<BN, f16>(kind, a, b, args, d, s);
-    case QRBL_BF16: return launch_kind<BN, bf16>(kind, a, b, args, d, s);
+template <typename T>
+int launch_type(int cg, int bn, bool fwd, const Product* const* q, int count, Args& args,
+                const Device& d, cudaStream_t s) {
+  if (cg == 1 && bn == 64) return launch_dir<1, 64, T>(fwd, q, count, args, d, s);
+  if (cg == 1 && bn == 128) return launch_dir<1, 128, T>(fwd, q, count, args, d, s);
+  if (cg == 2 && bn == 128) return launch_dir<2, 128, T>(fwd, q, count, args, d, s);
+  if constexpr (sizeof(T) == 2) {
+    if (cg == 2 && bn == 256) return launch_dir<2, 256, T>(fwd, q, count, args, d, s);
   }
   return QRB_ERR_INVALID_ARG;
 }
 
 int64_t tiles_of(int64_t v, int64_t t) { return (v + t - 1) / t; }
 
+// The cuts of the kernel: CTAs per tile and tile width.
+struct Cut {
+  int cg, bn;
+};
+constexpr Cut kCuts16[] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
+constexpr Cut kCuts32[] = {{2, 128}, {1, 128}, {1, 64}};
+
+// Estimated SM clocks of one stage of one CTA: the larger of its MMAs (2 BN
+// clocks, shared by a pair; six times as many in FP32) and its loads (64 bytes
+// a clock; rows beyond a short m are not read).
+double stage_clocks(bool f32, Cut c, int64_t m) {
+  const double rows = m < BM ? (double)m : BM;
+  const double mma = 2.0 * c.bn * (f32 ? 6 : 1);
+  const double load = 2.0 * (rows + c.bn / c.cg) * (f32 ? 3 : 1);
+  return mma > load ? mma : load;
+}
+double item_clocks(bool f32, Cut c, int64_t m, int64_t kb) {
+  return (double)kb * stage_clocks(f32, c, m) + 500.0;
+}
+
+// The schedule of `items[0]` longer and `items[1]` shorter items over `most`
+// workers, and its length in the items' clocks.
+double make_schedule(const int64_t* items, const double* clocks, int64_t most, Schedule* out) {
+  const int64_t all = items[0] + items[1];
+  const int64_t g = all < most ? all : most;
+  Schedule s = {};
+  s.workers = (int)g;
+  s.q = (int)(items[0] / g);
+  s.r = (int)(items[0] % g);
+  double length = (s.q + (s.r > 0 ? 1 : 0)) * clocks[0];
+  if (items[1] > 0) {
+    // the least x whose level holds every short item; y by what the one more
+    // long item leaves of it
+    const double ratio = clocks[0] / clocks[1];
+    int64_t x = (items[1] - 1) / g;
+    for (;; ++x) {
+      int64_t y = x - (int64_t)(ratio + 0.5);
+      if (y < 0) y = 0;
+      if (s.r == 0) y = x;
+      if (x * (g - s.r) + y * s.r >= items[1]) {
+        s.x = (int)x;
+        s.y = (int)y;
+        break;
+      }
+    }
+    const double late = s.q * clocks[0] + s.x * clocks[1];
+    const double early = s.r > 0 ? (s.q + 1) * clocks[0] + s.y * clocks[1] : 0;
+    length = late > early ? late : early;
+  }
+  *out = s;
+  return length;
+}
+
+Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, Cut c, int splits) {
+  Problem p = {};
+  p.m = (int)m;
+  p.n = (int)n;
+  p.mt = (int)tiles_of(m, BM * c.cg);
+  p.nt = (int)tiles_of(n, c.bn);
+  p.kb = (int)tiles_of(k, BK);
+  p.splits = splits;
+  p.items = p.mt * p.nt * splits;
+  p.group = c.cg == 2 ? 8 : 16;
+  p.amn = kind == kGradW;
+  p.bmn = kind != kForward;
+  return p;
+}
+
 }  // namespace
 
-// The cut with the least estimated time, in SM clocks: a stage takes the larger
-// of its MMAs (2 BN clocks, six times as many in FP32) and its loads (64 bytes
-// a clock); a tile adds a start and an end; a split adds writing and reading
-// the partial tiles and the second launch.
-ProductPlan plan_product(int dtype, int kind, int64_t m, int64_t n, int64_t k) {
-  (void)kind;
+// The cut with the least estimated time, in SM clocks: the schedule's length, a
+// start, and for each split product the writing and reading of its partial
+// tiles and its second launch.
+static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
   ProductPlan best;
   const Device* d = device_info();
   const int64_t sms = d != nullptr ? d->sms : 148;
   const bool f32 = dtype == QRBL_F32;
-  const int64_t kb = tiles_of(k, BK), mt = tiles_of(m, BM);
-  double least = 0;
-  const int rows = m < BM ? (int)m : BM;
-  for (int bn = f32 ? 128 : 256; bn >= 64; bn /= 2) {
-    const int64_t tiles = mt * tiles_of(n, bn);
-    const double mma = 2.0 * bn * (f32 ? 6 : 1), load = 2.0 * (rows + bn) * (f32 ? 3 : 1);
-    const double stage = mma > load ? mma : load;
-    for (int s = 1; s <= 16 && s <= kb; ++s) {
-      if (s > 1 && tiles * (s - 1) >= sms) break;
-      const double waves = (double)tiles_of(tiles * s, sms);
-      double t = waves * ((double)tiles_of(kb, s) * stage + 4.0 * bn) + 3000.0;
-      if (s > 1) t += 6000.0 + 2.0 * s * (double)m * (double)n * 4.0 / 2500.0;
-      if (least == 0 || t < least) {
-        least = t;
-        best.bn = bn;
-        best.splits = s;
+  double least = -1;
+  const Cut* cuts = f32 ? kCuts32 : kCuts16;
+  const int ncuts = f32 ? 3 : 4;
+  for (int ci = 0; ci < ncuts; ++ci) {
+    const Cut c = cuts[ci];
+    const int64_t workers = sms / c.cg;
+    int64_t tiles[2] = {0, 0}, kb[2] = {1, 1};
+    for (int i = 0; i < count; ++i) {
+      tiles[i] = tiles_of(sizes[i].m, BM * c.cg) * tiles_of(sizes[i].n, c.bn);
+      kb[i] = tiles_of(sizes[i].k, BK);
+      if (tiles[i] > (1 << 26)) return best;  // (refused: 26 bits of tiles)
+    }
+    for (int s0 = 1; s0 <= 16 && s0 <= kb[0]; ++s0) {
+      if (s0 > 1 && tiles[0] * (s0 - 1) >= workers) break;
+      for (int s1 = 1; s1 <= (count > 1 ? 16 : 1) && s1 <= kb[1]; ++s1) {
+        if (s1 > 1 && tiles[1] * (s1 - 1) >= workers) break;
+        const int sp[2] = {s0, s1};
+        double len[2] = {0, 0}, t = 3000.0;
+        int64_t items[2] = {0, 0};
+        for (int i = 0; i < count; ++i) {
+          items[i] = tiles[i] * sp[i];
+          len[i] = item_clocks(f32, c, sizes[i].m, tiles_of(kb[i], sp[i]));
+          if (sp[i] > 1)
+            t += 6000.0 + 2.0 * sp[i] * (double)sizes[i].m * (double)sizes[i].n * 4.0 / 2500.0;
+        }
+        const bool swap = count > 1 && len[1] > len[0];
+        const int64_t it[2] = {items[swap ? 1 : 0], count > 1 ? items[swap ? 0 : 1] : 0};
+        const double cl[2] = {len[swap ? 1 : 0], count > 1 ? len[swap ? 0 : 1] : 1.0};
+        Schedule sc;
+        t += make_schedule(it, cl, workers, &sc);
+        if (least < 0 || t < least) {
+          least = t;
+          best.cg = c.cg;
+          best.bn = c.bn;
+          best.first = swap ? 1 : 0;
+          best.splits[0] = s0;
+          best.splits[1] = s1;
+        }
       }
     }
   }
-  if (best.splits > 1) {
-    best.part_rows = mt * BM;
-    best.part_ld = tiles_of(n, best.bn) * best.bn;
-    best.part_bytes = (size_t)best.splits * best.part_rows * best.part_ld * sizeof(float);
+  for (int i = 0; i < count; ++i) {
+    if (best.splits[i] <= 1) continue;
+    best.part_rows[i] = tiles_of(sizes[i].m, BM * best.cg) * BM * best.cg;
+    best.part_ld[i] = tiles_of(sizes[i].n, best.bn) * best.bn;
+    best.part_bytes[i] =
+        (size_t)best.splits[i] * best.part_rows[i] * best.part_ld[i] * sizeof(float);
   }
+  best.ok = least >= 0;
   return best;
 }
 
-int launch_product(int dtype, int kind, const Operand& a, const Operand& b, int64_t m, int64_t n,
-                   int64_t k, const ProductPlan& plan, float* part, const Epilogue& e,
-                   cudaStream_t s) {
+// A pure function of its arguments and the device's SM count; the last few
+// results are kept per thread, since a call asks twice (its workspace, its
+// launch) and a model's layers repeat.
+ProductPlan plan_products(int dtype, const ProductSize* sizes, int count) {
+  struct Entry {
+    int dtype = -1, count = 0, sms = 0;
+    ProductSize z[2];
+    ProductPlan plan;
+  };
+  static thread_local Entry kept[64];
+  const Device* d = device_info();
+  const int sms = d != nullptr ? d->sms : 0;
+  uint64_t h = (uint64_t)dtype * 3 + (uint64_t)count;
+  for (int i = 0; i < count; ++i)
+    h = (h * 1000003u + (uint64_t)sizes[i].m) * 1000003u + (uint64_t)sizes[i].n * 8191u +
+        (uint64_t)sizes[i].k;
+  Entry& e = kept[(h ^ (h >> 17) ^ (h >> 31)) % 64];
+  bool same = e.dtype == dtype && e.count == count && e.sms == sms;
+  for (int i = 0; i < count && same; ++i)
+    same = e.z[i].m == sizes[i].m && e.z[i].n == sizes[i].n && e.z[i].k == sizes[i].k;
+  if (!same) {
+    e.dtype = dtype;
+    e.count = count;
+    e.sms = sms;
+    for (int i = 0; i < count; ++i) e.z[i] = sizes[i];
+    e.plan = search_plan(dtype, sizes, count);
+  }
+  return e.plan;
+}
+
+int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
+                    cudaStream_t s) {
   const Device* d = device_info();
   if (d == nullptr) return QRB_ERR_DEVICE;
+  if (!plan.ok) return QRB_ERR_UNSUPPORTED;
+  const Cut c = {plan.cg, plan.bn};
+  const bool f32 = dtype == QRBL_F32;
   Args args = {};
-  args.m = (int)m;
-  args.n = (int)n;
-  const int64_t mt = tiles_of(m, BM), nt = tiles_of(n, plan.bn);
-  if (mt * nt * plan.splits > 0x7fffffffLL) return QRB_ERR_UNSUPPORTED;
-  args.mt = (int)mt;
-  args.nt = (int)nt;
-  args.kb = (int)tiles_of(k, BK);
-  args.splits = plan.splits;
-  args.items = (int)(mt * nt * plan.splits);
-  args.group = 8;
-  args.part = plan.splits > 1 ? part : nullptr;
-  args.part_rows = plan.part_rows;
-  args.part_ld = plan.part_ld;
-  args.e = e;
-  args.vcodes = aligned16(e.z_codes) && n % 16 == 0;
+  const Product* q[2] = {nullptr, nullptr};
+  int64_t items[2] = {0, 0};
+  double clocks[2] = {1.0, 1.0};
+  for (int j = 0; j < count; ++j) {
+    const int i = count > 1 ? (j == 0 ? plan.first : 1 - plan.first) : 0;  // longer items first
+    q[j] = &products[i];
+    const ProductSize& z = products[i].size;
+    args.p[j] = problem_of(products[i].kind, z.m, z.n, z.k, c, plan.splits[i]);
+    args.p[j].part = plan.splits[i] > 1 ? products[i].part : nullptr;
+    args.p[j].part_rows = plan.part_rows[i];
+    args.p[j].part_ld = plan.part_ld[i];
+    args.p[j].e = products[i].e;
+    args.p[j].vcodes = aligned16(products[i].e.z_codes) && z.n % 16 == 0;
+    items[j] = args.p[j].items;
+    clocks[j] = item_clocks(f32, c, z.m, tiles_of(args.p[j].kb, plan.splits[i]));
+  }
+  make_schedule(items, clocks, d->sms / c.cg, &args.s);
   args.err = d->err;
   args.limit = device_wait_limit();
   args.skip_mma = test_skip_mma() ? 1 : 0;
+  const bool fwd = products[0].kind == kForward;
   int rc = QRB_ERR_INVALID_ARG;
-  switch (plan.bn) {
-    case 64: rc = launch_bn<64>(dtype, kind, a, b, args, *d, s); break;
-    case 128: rc = launch_bn<128>(dtype, kind, a, b, args, *d, s); break;
-    case 256: rc = launch_bn<256>(dtype, kind, a, b, args, *d, s); break;
+  switch (dtype) {
+    case QRBL_F32: rc = launch_type<float>(c.cg, c.bn, fwd, q, count, args, *d, s); break;
+    case QRBL_F16: rc = launch_type<f16>(c.cg, c.bn, fwd, q, count, args, *d, s); break;
+    case QRBL_BF16: rc = launch_type<bf16>(c.cg, c.bn, fwd, q, count, args, *d, s); break;
   }
-  if (rc != QRB_OK || plan.splits <= 1) return rc;
-  return launch_join(dtype, part, plan.splits, plan.part_rows, plan.part_ld, m, n, e, s);
+  for (int i = 0; i < count && rc == QRB_OK; ++i)
+    if (plan.splits[i] > 1)
+      rc = launch_join(dtype, products[i].part, plan.splits[i], plan.part_rows[i],
+                       plan.part_ld[i], products[i].size.m, products[i].size.n, products[i].e, s);
+  return rc;
 }
 
 }  // namespace lin
