@@ -9,37 +9,39 @@ namespace lin {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kVals = 8;     // values per thread and row
 
-// Threads tx over the columns (8 each), 256 / tx over the rows.
-struct Grid2 {
-  int tx;
-  dim3 grid, block;
+bool rows_aligned(const void* p, int64_t ld, int elem, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (ld * elem) % bytes == 0;
+}
+
+// Threads tx over the columns (V values each), 256 / tx over the rows, `per`
+// rows each: blocks over the columns fastest.
+struct Cover {
+  int tx;            // a power of two, at least one packed block's threads
+  int64_t nx;        // blocks along the columns
+  int64_t blocks;
 };
-Grid2 grid2(int64_t rows, int64_t cols, int rows_per_thread, bool* ok) {
-  Grid2 g;
-  int64_t want = (cols + kVals - 1) / kVals;
-  g.tx = 4;  // a 32-value block stays within one warp
-  while (g.tx < want && g.tx < kThreads) g.tx *= 2;
-  const int64_t per = (int64_t)(kThreads / g.tx) * rows_per_thread;
-  const int64_t gx = (rows + per - 1) / per;
-  const int64_t gy = (want + g.tx - 1) / g.tx;
-  *ok = gx <= 0x7fffffffLL && gy <= 65535;
-  g.grid = dim3((unsigned)gx, (unsigned)gy);
-  g.block = dim3((unsigned)g.tx, (unsigned)(kThreads / g.tx));
-  return g;
+Cover cover(int64_t rows, int64_t cols, int v, int per) {
+  Cover c;
+  const int64_t want = (cols + v - 1) / v;
+  c.tx = 4;
+  while (c.tx < want && c.tx < kThreads) c.tx *= 2;
+  c.nx = (want + c.tx - 1) / c.tx;
+  const int64_t high = (int64_t)(kThreads / c.tx) * per;
+  c.blocks = c.nx * ((rows + high - 1) / high);
+  return c;
 }
 
 // Eight codes: one access where they are all there and aligned.
 __device__ __forceinline__ uint2 load_codes(const int8_t* p, bool vec, int valid) {
-  if (vec && valid >= kVals) return *reinterpret_cast<const uint2*>(p);
+  if (vec && valid >= 8) return *reinterpret_cast<const uint2*>(p);
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < kVals; ++i)
+  for (int i = 0; i < 8; ++i)
     if (i < valid) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void decode8(uint2 q, float step, float (&out)[kVals]) {
+__device__ __forceinline__ void decode8(uint2 q, float step, float (&out)[8]) {
   float lo[4], hi[4];
   decode4(q.x, step, lo);
   decode4(q.y, step, hi);
@@ -49,223 +51,385 @@ __device__ __forceinline__ void decode8(uint2 q, float step, float (&out)[kVals]
     out[4 + i] = hi[i];
   }
 }
+__device__ __forceinline__ int clip(int64_t left, int most) {
+  return left >= most ? most : (left > 0 ? (int)left : 0);
+}
 
-// ---------------------------------------------------------------------------
-// pack / unpack
-// ---------------------------------------------------------------------------
-// Four neighbouring threads hold one block of 32 values; its largest magnitude
-// comes from two shuffles. ROWS rows per thread keep that many loads in flight.
-template <typename T, int ROWS>
-__global__ void __launch_bounds__(kThreads)
-    k_pack(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols, int64_t nblk,
-           int8_t* __restrict__ codes, int8_t* __restrict__ exps, int vin, int vout) {
-  const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * kVals;
-  const int64_t r0 = (int64_t)blockIdx.x * blockDim.y * ROWS + threadIdx.y;
-  constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
-  float v[ROWS][kVals];
-  const int valid = (int)(cols - c < kVals ? (cols > c ? cols - c : 0) : kVals);
-#pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    const int64_t r = r0 + (int64_t)j * blockDim.y;
-    load_n<T, kVals>(x + r * ld + c, vin, r < rows ? valid : 0, v[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    const int64_t r = r0 + (int64_t)j * blockDim.y;
-    float a = fabsf(v[j][0]);
-#pragma unroll
-    for (int i = 1; i < kVals; ++i) a = max_abs_nan(a, v[j][i]);
-    a = max_abs_nan(a, __shfl_xor_sync(kFull, a, 1));
-    a = max_abs_nan(a, __shfl_xor_sync(kFull, a, 2));
-    if (__any_sync(kFull, !finite_f(a))) {
-      const bool fine = finite_f(a);
-      float f = finite_amax(v[j]);
-      f = fmaxf(f, __shfl_xor_sync(kFull, f, 1));
-      f = fmaxf(f, __shfl_xor_sync(kFull, f, 2));
-      if (!fine) {  // Inf or NaN in this block: its exponent from the rest
-        const int e = block_exponent(f, lo, hi);
-        uint32_t w[2];
-        encode(v[j], e, false, e == hi ? 63.f : 127.f, w);
-        if (r < rows && valid > 0) {
-          int8_t* out = codes + r * cols + c;
-#pragma unroll
-          for (int i = 0; i < kVals; ++i)
-            if (i < valid) out[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
-          if ((threadIdx.x & 3) == 0) exps[r * nblk + c / kBlk] = (int8_t)e;
-        }
-        continue;
-      }
-    }
-    const int e = block_exponent(a, lo, hi);
-    uint32_t w[2];
-    encode(v[j], e, plain_block(a, e, hi), 63.f, w);
-    if (r >= rows || valid == 0) continue;
-    int8_t* out = codes + r * cols + c;
-    if (vout && valid >= kVals) {
-      *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVals; ++i)
-        if (i < valid) out[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
-    }
-    if ((threadIdx.x & 3) == 0) exps[r * nblk + c / kBlk] = (int8_t)e;
+// 32 bytes at a 32-byte aligned address in one access.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+  if constexpr (__is_same(T, bf16)) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
 
-// A matrix as a product's operand or as itself. PACKED: from codes and
-// exponents. PLANES: three BF16 planes of FP32 values; else type T.
-template <typename T, bool PACKED, bool PLANES, int ROWS>
+// ---------------------------------------------------------------------------
+// pack
+// ---------------------------------------------------------------------------
+// Two neighbouring threads hold one block of 32 values; its largest magnitude
+// comes from one shuffle. ROWS rows per thread keep that many loads in flight.
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(kThreads)
-    k_stage(const T* __restrict__ x, int64_t ld, const int8_t* __restrict__ codes,
-            const int8_t* __restrict__ exps, int64_t rows, int64_t cols, int64_t nblk,
-            void* __restrict__ dst, int64_t ldd, int64_t plane, int vin, int vout) {
-  const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * kVals;
-  const int64_t r0 = (int64_t)blockIdx.x * blockDim.y * ROWS + threadIdx.y;
-  if (c >= cols) return;
-  const int valid = (int)(cols - c < kVals ? cols - c : kVals);
-  float v[ROWS][kVals];
+    k_pack(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols, int64_t nblk,
+           int8_t* __restrict__ codes, int8_t* __restrict__ exps, int tx, int64_t nx, int vin,
+           int vout) {
+  constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi, V = 16;
+  const int64_t by = blockIdx.x / nx, bx = blockIdx.x - by * nx;
+  const int ty = kThreads / tx, x0 = threadIdx.x & (tx - 1), y0 = threadIdx.x / tx;
+  const int64_t c = (bx * tx + x0) * V;
+  const int64_t r0 = by * ty * ROWS + y0;
+  const int valid = clip(cols - c, V);
+  Raw8<T> raw[ROWS][2];
 #pragma unroll
   for (int j = 0; j < ROWS; ++j) {
-    const int64_t r = r0 + (int64_t)j * blockDim.y;
+    const int64_t r = r0 + (int64_t)j * ty;
+    const int have = r < rows ? valid : 0;
+    const T* p = x + r * ld + c;
+    raw[j][0] = load_raw8<T>(p, vin, have);
+    raw[j][1] = load_raw8<T>(p + 8, vin, have - 8);
+  }
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const int64_t r = r0 + (int64_t)j * ty;
+    float v[V];
+    values8<T>(raw[j][0], *reinterpret_cast<float(*)[8]>(v));
+    values8<T>(raw[j][1], *reinterpret_cast<float(*)[8]>(v + 8));
+    float a = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < V; ++i) a = max_abs_nan(a, v[i]);
+    a = max_abs_nan(a, __shfl_xor_sync(kFull, a, 1));
+    const bool fine = finite_f(a);
+    if (__any_sync(kFull, !fine)) {  // Inf or NaN somewhere: exponents from the rest
+      float f = finite_amax(v);
+      f = fmaxf(f, __shfl_xor_sync(kFull, f, 1));
+      a = f;
+    }
+    const int e = block_exponent(a, lo, hi);
+    uint32_t w[V / 4];
+    encode(v, e, fine && e < hi, e == hi ? 63.f : 127.f, w);
+    if (r >= rows || valid == 0) continue;
+    int8_t* out = codes + r * cols + c;
+    if (vout && valid == V) {
+      *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < valid) out[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+    if ((threadIdx.x & 1) == 0) exps[r * nblk + c / kBlk] = (int8_t)e;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// stage / unpack
+// ---------------------------------------------------------------------------
+struct StageJob {
+  StageArgs a;
+  int tx = 4;
+  int64_t nx = 1, blocks = 0, nblk = 0;
+  int vin = 0, vout = 0;
+};
+constexpr int stage_rows(int elem) { return elem == 4 ? 2 : 4; }
+constexpr int kStageVals = 16;
+
+// A matrix as a product's operand or as itself. PACKED: from codes and
+// exponents. PLANES: three BF16 planes of FP32 values; else type T. 16 values of
+// each of four rows (FP32: two) per thread, the loads of all in flight together.
+template <typename T, bool PACKED, bool PLANES>
+__device__ __forceinline__ void stage_block(const StageJob& j, int64_t block) {
+  constexpr int V = kStageVals, ROWS = sizeof(T) == 4 ? 2 : 4;
+  const StageArgs& a = j.a;
+  const int64_t by = block / j.nx, bx = block - by * j.nx;
+  const int ty = kThreads / j.tx, x0 = threadIdx.x & (j.tx - 1), y0 = threadIdx.x / j.tx;
+  const int64_t c = (bx * j.tx + x0) * V;
+  const int64_t r0 = by * ty * ROWS + y0;
+  const int valid = clip(a.cols - c, V);
+  if (!j.vin) {  // rows not 16-byte aligned: neighbouring threads, neighbouring values
+    const int64_t c0 = bx * j.tx * V + x0;
+#pragma unroll 1
+    for (int i = 0; i < ROWS; ++i) {
+      const int64_t r = r0 + (int64_t)i * ty;
+      if (r >= a.rows) return;
+      float v[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int64_t cc = c0 + (int64_t)k * j.tx;
+        if (cc >= a.cols)
+          v[k] = 0.f;
+        else if constexpr (PACKED)
+          v[k] = value_of(a.codes[r * a.cols + cc], pow2f(a.exps[r * j.nblk + cc / kBlk]));
+        else
+          v[k] = to_f<T>(reinterpret_cast<const T*>(a.src)[r * a.lds + cc]);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int64_t cc = c0 + (int64_t)k * j.tx;
+        if (cc >= a.cols) continue;
+        if constexpr (PLANES) {
+          bf16* d = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + cc;
+          split3(v[k], d[0], d[a.plane], d[2 * a.plane]);
+        } else {
+          reinterpret_cast<T*>(a.dst)[r * a.ldd + cc] = from_f<T>(v[k]);
+        }
+      }
+    }
+    return;
+  }
+  if (valid == 0) return;
+  Raw8<T> raw[ROWS][2];
+  uint4 q[ROWS];
+  int e[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int64_t r = r0 + (int64_t)i * ty;
+    const int have = r < a.rows ? valid : 0;
     if constexpr (PACKED) {
-      const uint2 q = load_codes(codes + r * cols + c, vin, r < rows ? valid : 0);
-      decode8(q, r < rows ? pow2f(exps[r * nblk + c / kBlk]) : 0.f, v[j]);
+      const int8_t* p = a.codes + r * a.cols + c;
+      if (j.vin && have == V) {
+        q[i] = *reinterpret_cast<const uint4*>(p);
+      } else {
+        const uint2 lo = load_codes(p, false, have), hi = load_codes(p + 8, false, have - 8);
+        q[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+      e[i] = have > 0 ? a.exps[r * j.nblk + c / kBlk] : 0;
     } else {
-      load_n<T, kVals>(x + r * ld + c, vin, r < rows ? valid : 0, v[j]);
+      const T* p = reinterpret_cast<const T*>(a.src) + r * a.lds + c;
+      raw[i][0] = load_raw8<T>(p, j.vin, have);
+      raw[i][1] = load_raw8<T>(p + 8, j.vin, have - 8);
     }
   }
 #pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    const int64_t r = r0 + (int64_t)j * blockDim.y;
-    if (r >= rows) continue;
-    if constexpr (PLANES) {
-      bf16* d = reinterpret_cast<bf16*>(dst) + r * ldd + c;
-      Vec<bf16, kVals> p[3];
+  for (int i = 0; i < ROWS; ++i) {
+    const int64_t r = r0 + (int64_t)i * ty;
+    if (r >= a.rows) return;
+    if constexpr (PACKED && sizeof(T) == 2) {
+      if (j.vout == 2 && valid == V) {
+        uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < kVals; ++i) split3(v[j][i], p[0].v[i], p[1].v[i], p[2].v[i]);
+        for (int h = 0; h < 2; ++h) {
+          float v[8];
+          decode8(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]),
+                  v);
 #pragma unroll
-      for (int k = 0; k < 3; ++k)  // ldd % 8 == 0: the padding may be written
-        *reinterpret_cast<Vec<bf16, kVals>*>(d + k * plane) = p[k];
-    } else {
-      store_n<T, kVals>(reinterpret_cast<T*>(dst) + r * ldd + c, vout, valid, v[j]);
+          for (int k = 0; k < 4; ++k) w[4 * h + k] = pair_of<T>(v[2 * k], v[2 * k + 1]);
+        }
+        store32(reinterpret_cast<T*>(a.dst) + r * a.ldd + c, w);
+        continue;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (valid <= 8 * h) continue;
+      float v[8];
+      if constexpr (PACKED)
+        decode8(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]), v);
+      else
+        values8<T>(raw[i][h], v);
+      if constexpr (PLANES) {
+        bf16* d = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + c + 8 * h;
+        Vec<bf16, 8> p[3];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) split3(v[k], p[0].v[k], p[1].v[k], p[2].v[k]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)  // ldd % 8 == 0: the padding may be written
+          *reinterpret_cast<Vec<bf16, 8>*>(d + k * a.plane) = p[k];
+      } else {
+        store_n<T, 8>(reinterpret_cast<T*>(a.dst) + r * a.ldd + c + 8 * h, j.vout, valid - 8 * h,
+                      v);
+      }
     }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_unpack(StageJob j) {
+  stage_block<T, true, false>(j, blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------
 // dz = dy act'(z), and its column sums
 // ---------------------------------------------------------------------------
 // Warps of 256 columns (8 per lane), 8 warps over the rows; a block takes `rows`
-// rows of them, 2 per warp at a time so that their loads are in flight
-// together. Each thread sums its rows in order, then the block's warps are
-// added in order: the same bits every time. part[blockIdx.x][col].
-constexpr int kDzRows = 2;
-template <bool EXACT, int ACT>
-__device__ __forceinline__ void dz8(float (&d)[kVals], const float (&z)[kVals]) {
-#pragma unroll
-  for (int i = 0; i < kVals; ++i) d[i] *= act_grad_fn<EXACT>(z[i], ACT);
-}
+// rows of them, 2 per warp at a time, the next 2 already being loaded. Each thread sums its rows in order, then the block's warps are
+// added in order: the same bits every time. part[row block][col].
+struct DzJob {
+  DzArgs a;
+  int64_t nx = 1, blocks = 0, nblk = 0;
+  int rows = 32, vdy = 0, vz = 0, vdst = 0;
+};
+// Rows that are not all aligned: one value at a time, lane + 32 i of the
+// block's 256 columns, neighbouring lanes at neighbouring values.
 template <typename T, bool PACKED, bool PLANES>
-__global__ void __launch_bounds__(kThreads, 3)
-    k_dz(DzArgs a, int64_t nblk, int rows, int vdy, int vz, int vdst) {
-  __shared__ float sums[8][32 * kVals];
-  constexpr bool EXACT = sizeof(T) == 4;
-  const int lane = threadIdx.x, warp = threadIdx.y;
-  const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * kVals;
-  const int64_t rb = (int64_t)blockIdx.x * rows;
-  const int64_t rend = rb + rows < a.m ? rb + rows : a.m;
-  const int valid = (int)(a.n - c < kVals ? (a.n > c ? a.n - c : 0) : kVals);
-  float acc[kVals];
+__device__ __forceinline__ void dz_rows_any(const DzJob& j, int64_t c0, int64_t rb, int64_t rend,
+                                            float (&acc)[8]) {
+  const DzArgs& a = j.a;
+  for (int64_t r = rb + (threadIdx.x >> 5); r < rend; r += 8) {
+    float d[8], f[8];
 #pragma unroll
-  for (int i = 0; i < kVals; ++i) acc[i] = 0.f;
-  if (valid > 0) {
-    for (int64_t r0 = rb + warp; r0 < rend; r0 += 8 * kDzRows) {
-      Raw8<T> g[kDzRows], z[kDzRows];
-      uint2 q[kDzRows];
-      int e[kDzRows];
-#pragma unroll
-      for (int j = 0; j < kDzRows; ++j) {
-        const int64_t r = r0 + 8 * j;
-        const int have = r < rend ? valid : 0;
-        g[j] = load_raw8<T>(reinterpret_cast<const T*>(a.dy) + r * a.lddy + c, vdy, have);
-        if (a.act != QRBL_ACT_NONE) {
-          if constexpr (PACKED) {
-            q[j] = load_codes(a.z_codes + r * a.n + c, vz, have);
-            e[j] = have > 0 ? a.z_exps[r * nblk + c / kBlk] : 0;
-          } else {
-            z[j] = load_raw8<T>(reinterpret_cast<const T*>(a.z) + r * a.ldz + c, vz, have);
-          }
-        }
+    for (int i = 0; i < 8; ++i) {
+      const int64_t c = c0 + (threadIdx.x & 31) + 32 * i;
+      const bool in = c < a.n;
+      d[i] = in ? to_f<T>(reinterpret_cast<const T*>(a.dy)[r * a.lddy + c]) : 0.f;
+      f[i] = 0.f;
+      if (a.act != QRBL_ACT_NONE && in) {
+        if constexpr (PACKED)
+          f[i] = value_of(a.z_codes[r * a.n + c], pow2f(a.z_exps[r * j.nblk + c / kBlk]));
+        else
+          f[i] = to_f<T>(reinterpret_cast<const T*>(a.z)[r * a.ldz + c]);
       }
+    }
+    act_grad_by(d, f, a.act);
 #pragma unroll
-      for (int j = 0; j < kDzRows; ++j) {
-        const int64_t r = r0 + 8 * j;
+    for (int i = 0; i < 8; ++i) {
+      const int64_t c = c0 + (threadIdx.x & 31) + 32 * i;
+      acc[i] += d[i];
+      if (a.dst == nullptr || c >= a.n) continue;
+      if constexpr (PLANES) {
+        bf16* out = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + c;
+        split3(d[i], out[0], out[a.plane], out[2 * a.plane]);
+      } else {
+        reinterpret_cast<T*>(a.dst)[r * a.ldd + c] = from_f<T>(d[i]);
+      }
+    }
+  }
+}
+
+template <typename T, bool PACKED>
+struct DzIn {  // one row's eight values of dy and z
+  Raw8<T> g, z;
+  uint2 q;
+  int e;
+};
+template <typename T, bool PACKED>
+__device__ __forceinline__ DzIn<T, PACKED> dz_load(const DzJob& j, int64_t r, int64_t c,
+                                                   int have) {
+  const DzArgs& a = j.a;
+  DzIn<T, PACKED> in;
+  in.g = load_raw8<T>(reinterpret_cast<const T*>(a.dy) + r * a.lddy + c, j.vdy, have);
+  if (a.act != QRBL_ACT_NONE) {
+    if constexpr (PACKED) {
+      in.q = load_codes(a.z_codes + r * a.n + c, j.vz, have);
+      in.e = have > 0 ? a.z_exps[r * j.nblk + c / kBlk] : 0;
+    } else {
+      in.z = load_raw8<T>(reinterpret_cast<const T*>(a.z) + r * a.ldz + c, j.vz, have);
+    }
+  }
+  return in;
+}
+
+template <typename T, bool PACKED, bool PLANES>
+__device__ __forceinline__ void dz_block(const DzJob& j, int64_t block, float (*sums)[256]) {
+  constexpr int V = 8, D = sizeof(T) == 4 ? 1 : 2;  // rows loaded together
+  const DzArgs& a = j.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t by = block / j.nx, bx = block - by * j.nx;
+  const int64_t c = (bx * 32 + lane) * V;
+  const int64_t rb = by * j.rows;
+  const int64_t rend = rb + j.rows < a.m ? rb + j.rows : a.m;
+  const int valid = clip(a.n - c, V);
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  const bool any = !(j.vdy && (j.vz || a.act == QRBL_ACT_NONE) && (j.vdst || a.dst == nullptr));
+  if (any) {
+    dz_rows_any<T, PACKED, PLANES>(j, bx * 256, rb, rend, acc);
+  } else if (valid > 0) {
+    DzIn<T, PACKED> cur[D], nxt[D];
+    auto load = [&](DzIn<T, PACKED>(&to)[D], int64_t r0) {
+#pragma unroll
+      for (int k = 0; k < D; ++k)
+        to[k] = dz_load<T, PACKED>(j, r0 + 8 * k, c, r0 + 8 * k < rend ? valid : 0);
+    };
+    load(cur, rb + warp);
+    for (int64_t r0 = rb + warp; r0 < rend; r0 += 8 * D) {
+      load(nxt, r0 + 8 * D);
+#pragma unroll
+      for (int k = 0; k < D; ++k) {
+        const int64_t r = r0 + 8 * k;
         if (r >= rend) break;
-        float d[kVals];
-        values8<T>(g[j], d);
+        float d[V];
+        values8<T>(cur[k].g, d);
         if (a.act != QRBL_ACT_NONE) {
-          float f[kVals];
-          if constexpr (PACKED) {
-            decode8(q[j], pow2f(e[j]), f);
-          } else {
-            values8<T>(z[j], f);
-          }
-          switch (a.act) {
-            case QRBL_ACT_RELU: dz8<EXACT, QRBL_ACT_RELU>(d, f); break;
-            case QRBL_ACT_GELU: dz8<EXACT, QRBL_ACT_GELU>(d, f); break;
-            case QRBL_ACT_GELU_TANH: dz8<EXACT, QRBL_ACT_GELU_TANH>(d, f); break;
-            case QRBL_ACT_SILU: dz8<EXACT, QRBL_ACT_SILU>(d, f); break;
-          }
+          float f[V];
+          if constexpr (PACKED)
+            decode8(cur[k].q, pow2f(cur[k].e), f);
+          else
+            values8<T>(cur[k].z, f);
+          act_grad_by(d, f, a.act);
         }
 #pragma unroll
-        for (int i = 0; i < kVals; ++i) acc[i] += d[i];
+        for (int i = 0; i < V; ++i) acc[i] += d[i];
         if (a.dst == nullptr) continue;
         if constexpr (PLANES) {
           bf16* out = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + c;
-          Vec<bf16, kVals> p[3];
+          Vec<bf16, V> p[3];
 #pragma unroll
-          for (int i = 0; i < kVals; ++i) split3(d[i], p[0].v[i], p[1].v[i], p[2].v[i]);
+          for (int i = 0; i < V; ++i) split3(d[i], p[0].v[i], p[1].v[i], p[2].v[i]);
 #pragma unroll
-          for (int k = 0; k < 3; ++k)
-            *reinterpret_cast<Vec<bf16, kVals>*>(out + k * a.plane) = p[k];
+          for (int i = 0; i < 3; ++i)
+            *reinterpret_cast<Vec<bf16, V>*>(out + i * a.plane) = p[i];
         } else {
-          store_n<T, kVals>(reinterpret_cast<T*>(a.dst) + r * a.ldd + c, vdst, valid, d);
+          store_n<T, V>(reinterpret_cast<T*>(a.dst) + r * a.ldd + c, j.vdst, valid, d);
         }
       }
+#pragma unroll
+      for (int k = 0; k < D; ++k) cur[k] = nxt[k];
     }
   }
   if (a.part == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < kVals; ++i) sums[warp][lane + 32 * i] = acc[i];
+  for (int i = 0; i < V; ++i) sums[warp][lane + 32 * i] = acc[i];
   __syncthreads();
-  const int t = warp * 32 + lane;  // one column each: lane t / 8, value t % 8
+  const int t = threadIdx.x;  // one column each: lane t / 8, value t % 8 (any: lane t % 32)
+  const int at = any ? t : t / V + 32 * (t % V);
   float s = 0.f;
 #pragma unroll
-  for (int y = 0; y < 8; ++y) s += sums[y][t / kVals + 32 * (t % kVals)];
-  const int64_t col = (int64_t)blockIdx.y * 256 + t;
-  if (col < a.n) a.part[(int64_t)blockIdx.x * a.n + col] = s;
+  for (int y = 0; y < 8; ++y) s += sums[y][at];
+  const int64_t col = bx * 256 + t;
+  if (col < a.n) a.part[by * a.n + col] = s;
 }
 
-// out[col] = sum over the blocks of part[block][col]: 32 columns and 8 groups
-// of blocks per CTA, the groups added in order.
+// One launch for all that comes before a product: the first blocks are dz's,
+// then the first and the second staged operand's.
+struct PrepArgs {
+  DzJob dz;
+  StageJob st[2];
+};
 template <typename T>
-__global__ void __launch_bounds__(256)
-    k_colsum(const float* __restrict__ part, int64_t blocks, int64_t n, T* __restrict__ out) {
-  __shared__ float sums[8][33];
-  const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  float s = 0.f;
-  if (col < n) {
-#pragma unroll 8
-    for (int64_t b = threadIdx.y; b < blocks; b += 8) s += part[b * n + col];
+__global__ void __launch_bounds__(kThreads, 3) k_prepare(const __grid_constant__ PrepArgs p) {
+  constexpr bool PLANES = sizeof(T) == 4;
+  __shared__ float sums[8][256];
+  int64_t b = blockIdx.x;
+  if (b < p.dz.blocks) {
+    if (p.dz.a.z_codes != nullptr)
+      dz_block<T, true, PLANES>(p.dz, b, sums);
+    else
+      dz_block<T, false, PLANES>(p.dz, b, sums);
+    return;
   }
-  sums[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y == 0 && col < n) {
-    float t = 0.f;
-#pragma unroll
-    for (int y = 0; y < 8; ++y) t += sums[y][threadIdx.x];
-    out[col] = from_f<T>(t);
-  }
+  b -= p.dz.blocks;
+  const bool second = b >= p.st[0].blocks;
+  const StageJob& j = p.st[second ? 1 : 0];
+  if (second) b -= p.st[0].blocks;
+  if (j.a.codes != nullptr)
+    stage_block<T, true, PLANES>(j, b);
+  else
+    stage_block<T, false, PLANES>(j, b);
+}
+
+// out[col] = sum over the blocks of part[block][col].
+template <typename T>
+__global__ void __launch_bounds__(128) k_colsum(ColSum c) {
+  column_sum<T>(c, (int64_t)blockIdx.x * 128 + threadIdx.x, (int64_t)gridDim.x * 128);
 }
 
 // ---------------------------------------------------------------------------
@@ -276,7 +440,6 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_join(const float* __restrict__ part, int splits, int64_t rows, int64_t ld, int64_t m,
            int64_t n, Epilogue e) {
-  constexpr bool EXACT = sizeof(T) == 4;
   const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * 4;
   const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int valid = r < m && c < n ? (int)(n - c < 4 ? n - c : 4) : 0;
@@ -318,8 +481,7 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   if (valid == 0) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = act_fn<EXACT>(v[i], e.act);
+  act_by(v, e.act);
   if (e.residual != nullptr) {
     float q[4];
     load_n<T, 4>(reinterpret_cast<const T*>(e.residual) + r * e.ldr + c, e.vec, valid, q);
@@ -334,57 +496,72 @@ int launched() {
   return cudaGetLastError() == cudaSuccess ? QRB_OK : QRB_ERR_LAUNCH;
 }
 
-bool rows_aligned(const void* p, int64_t ld, int elem, int bytes) {
-  return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (ld * elem) % bytes == 0;
-}
-
 template <typename T>
 int pack_t(const void* x, int64_t ld, int64_t rows, int64_t cols, int8_t* codes, int8_t* exps,
            cudaStream_t s) {
-  constexpr int ROWS = 4;
-  bool ok;
-  const Grid2 g = grid2(rows, cols, ROWS, &ok);
-  if (!ok) return QRB_ERR_UNSUPPORTED;
-  k_pack<T, ROWS><<<g.grid, g.block, 0, s>>>(
-      reinterpret_cast<const T*>(x), ld, rows, cols, blocks_of(cols), codes, exps,
-      rows_aligned(x, ld, sizeof(T), 16), rows_aligned(codes, cols, 1, 8));
+  constexpr int ROWS = sizeof(T) == 4 ? 2 : 4;
+  const Cover g = cover(rows, cols, 16, ROWS);
+  if (g.blocks > 0x7fffffffLL) return QRB_ERR_UNSUPPORTED;
+  k_pack<T, ROWS><<<(unsigned)g.blocks, kThreads, 0, s>>>(
+      reinterpret_cast<const T*>(x), ld, rows, cols, blocks_of(cols), codes, exps, g.tx, g.nx,
+      rows_aligned(x, ld, sizeof(T), 16), rows_aligned(codes, cols, 1, 16));
   return launched();
 }
 
-template <typename T, bool PLANES>
-int stage_t(const void* src, int64_t lds, const int8_t* codes, const int8_t* exps, int64_t rows,
-            int64_t cols, void* dst, int64_t ldd, int64_t plane, cudaStream_t s) {
-  constexpr int ROWS = 4;
-  bool ok;
-  const Grid2 g = grid2(rows, cols, ROWS, &ok);
-  if (!ok) return QRB_ERR_UNSUPPORTED;
-  const int vout = rows_aligned(dst, ldd, sizeof(T), 16);
-  if (codes != nullptr)
-    k_stage<T, true, PLANES, ROWS><<<g.grid, g.block, 0, s>>>(
-        nullptr, 0, codes, exps, rows, cols, blocks_of(cols), dst, ldd, plane,
-        rows_aligned(codes, cols, 1, 8), vout);
-  else
-    k_stage<T, false, PLANES, ROWS><<<g.grid, g.block, 0, s>>>(
-        reinterpret_cast<const T*>(src), lds, nullptr, nullptr, rows, cols, blocks_of(cols), dst,
-        ldd, plane, rows_aligned(src, lds, sizeof(T), 16), vout);
+StageJob stage_job(int elem, const StageArgs& a) {
+  StageJob j;
+  j.a = a;
+  const Cover g = cover(a.rows, a.cols, kStageVals, stage_rows(elem));
+  j.tx = g.tx;
+  j.nx = g.nx;
+  j.blocks = g.blocks;
+  j.nblk = blocks_of(a.cols);
+  j.vin = a.codes != nullptr ? rows_aligned(a.codes, a.cols, 1, 16)
+                             : rows_aligned(a.src, a.lds, elem, 16);
+  j.vout = rows_aligned(a.dst, a.ldd, elem, 32) ? 2 : rows_aligned(a.dst, a.ldd, elem, 16);
+  return j;
+}
+
+template <typename T>
+int unpack_t(const int8_t* codes, const int8_t* exps, int64_t rows, int64_t cols, void* x,
+             int64_t ld, cudaStream_t s) {
+  StageArgs a;
+  a.codes = codes;
+  a.exps = exps;
+  a.rows = rows;
+  a.cols = cols;
+  a.dst = x;
+  a.ldd = ld;
+  const StageJob j = stage_job(sizeof(T), a);
+  if (j.blocks > 0x7fffffffLL) return QRB_ERR_UNSUPPORTED;
+  k_unpack<T><<<(unsigned)j.blocks, kThreads, 0, s>>>(j);
   return launched();
 }
 
 template <typename T>
-int dz_t(const DzArgs& a, cudaStream_t s) {
-  constexpr bool PLANES = sizeof(T) == 4;
-  const int rows = colsum_rows(a.m, a.n);
-  const int64_t gx = (a.m + rows - 1) / rows, gy = (a.n + 255) / 256;
-  if (gx > 0x7fffffffLL || gy > 65535) return QRB_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)gx, (unsigned)gy), block(32, 8);
-  const int vdy = rows_aligned(a.dy, a.lddy, sizeof(T), 16);
-  const int vdst = rows_aligned(a.dst, a.ldd, sizeof(T), 16);
-  if (a.z_codes != nullptr)
-    k_dz<T, true, PLANES><<<grid, block, 0, s>>>(a, blocks_of(a.n), rows, vdy,
-                                                 rows_aligned(a.z_codes, a.n, 1, 8), vdst);
-  else
-    k_dz<T, false, PLANES><<<grid, block, 0, s>>>(
-        a, blocks_of(a.n), rows, vdy, rows_aligned(a.z, a.ldz, sizeof(T), 16), vdst);
+int prepare_t(const Prepare& p, cudaStream_t s) {
+  PrepArgs a;
+  int64_t blocks = 0;
+  if (p.has_dz) {
+    const DzArgs& d = p.dz;
+    a.dz.a = d;
+    a.dz.rows = colsum_rows(d.m, d.n);
+    a.dz.nx = (d.n + 255) / 256;
+    a.dz.blocks = a.dz.nx * ((d.m + a.dz.rows - 1) / a.dz.rows);
+    a.dz.nblk = blocks_of(d.n);
+    a.dz.vdy = rows_aligned(d.dy, d.lddy, sizeof(T), 16);
+    a.dz.vdst = rows_aligned(d.dst, d.ldd, sizeof(T), 16);
+    a.dz.vz = d.z_codes != nullptr ? rows_aligned(d.z_codes, d.n, 1, 8)
+                                   : rows_aligned(d.z, d.ldz, sizeof(T), 16);
+    blocks += a.dz.blocks;
+  }
+  for (int i = 0; i < p.stages; ++i) {
+    a.st[i] = stage_job(sizeof(T), p.stage[i]);
+    blocks += a.st[i].blocks;
+  }
+  if (blocks == 0) return QRB_OK;
+  if (blocks > 0x7fffffffLL) return QRB_ERR_UNSUPPORTED;
+  k_prepare<T><<<(unsigned)blocks, kThreads, 0, s>>>(a);
   return launched();
 }
 
@@ -418,14 +595,11 @@ int launch_pack(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols
 
 int launch_unpack(int dtype, const int8_t* codes, const int8_t* exps, int64_t rows, int64_t cols,
                   void* x, int64_t ld, cudaStream_t s) {
-  QRBL_BY_TYPE(dtype, return (stage_t<T, false>(nullptr, 0, codes, exps, rows, cols, x, ld, 0, s)));
+  QRBL_BY_TYPE(dtype, return unpack_t<T>(codes, exps, rows, cols, x, ld, s));
 }
 
-int launch_stage(int dtype, const void* src, int64_t lds, const int8_t* codes, const int8_t* exps,
-                 int64_t rows, int64_t cols, void* dst, int64_t ldd, int64_t plane,
-                 cudaStream_t s) {
-  QRBL_BY_TYPE(dtype, return (stage_t<T, sizeof(T) == 4>(src, lds, codes, exps, rows, cols, dst,
-                                                         ldd, plane, s)));
+int launch_prepare(int dtype, const Prepare& p, cudaStream_t s) {
+  QRBL_BY_TYPE(dtype, return prepare_t<T>(p, s));
 }
 
 // 128 rows where that leaves four blocks or more per SM (fewer partial sums to
@@ -434,15 +608,11 @@ int colsum_rows(int64_t m, int64_t n) {
   return ((m + 127) / 128) * ((n + 255) / 256) >= 592 ? 128 : 32;
 }
 
-int launch_dz(int dtype, const DzArgs& a, cudaStream_t s) {
-  QRBL_BY_TYPE(dtype, return dz_t<T>(a, s));
-}
-
-int launch_colsum(int dtype, const float* part, int64_t blocks, int64_t n, void* out,
-                  cudaStream_t s) {
-  const int64_t gx = (n + 31) / 32;
+int launch_colsum(int dtype, const ColSum& c, cudaStream_t s) {
+  const int64_t gx = (c.n + 127) / 128;
+  const unsigned grid = (unsigned)(gx < 65535 ? gx : 65535);
   QRBL_BY_TYPE(dtype, {
-    k_colsum<T><<<(unsigned)gx, dim3(32, 8), 0, s>>>(part, blocks, n, reinterpret_cast<T*>(out));
+    k_colsum<T><<<grid, 128, 0, s>>>(c);
     return launched();
   });
 }

@@ -66,9 +66,17 @@ Operand operand_of(int dtype, const Source& s, Carve* c, bool* stage) {
   o.ld = s.rows <= 1 ? up8(s.cols) : s.ld;  // one row: any legal stride
   return o;
 }
-int fill(int dtype, const Source& s, const Operand& o, cudaStream_t st) {
-  return launch_stage(dtype, s.p, s.ld, s.codes, s.exps, s.rows, s.cols, const_cast<void*>(o.p),
-                      o.ld, o.plane, st);
+void add_stage(Prepare* p, const Source& s, const Operand& o) {
+  StageArgs& a = p->stage[p->stages++];
+  a.src = s.p;
+  a.lds = s.ld;
+  a.codes = s.codes;
+  a.exps = s.exps;
+  a.rows = s.rows;
+  a.cols = s.cols;
+  a.dst = const_cast<void*>(o.p);
+  a.ldd = o.ld;
+  a.plane = o.plane;
 }
 
 // ---------------------------------------------------------------------------
@@ -92,6 +100,7 @@ int check(const qrbl_linear_args& a) {
 }
 
 struct Forward {
+  bool rows = false;  // few rows: their own kernel
   Source xs, ws;
   Operand x, w;
   bool stage_x = false, stage_w = false;
@@ -101,6 +110,12 @@ struct Forward {
 };
 Forward plan_forward(const qrbl_linear_args& a, Carve* c) {
   Forward f;
+  f.rows = a.m <= rows_most(a.dtype);
+  if (f.rows) {
+    f.x.p = a.x; f.x.ld = a.ldx;
+    f.w.p = a.w; f.w.ld = a.ldw;
+    return f;
+  }
   f.xs.p = a.x; f.xs.ld = a.ldx; f.xs.rows = a.m; f.xs.cols = a.k;
   f.ws.p = a.w; f.ws.ld = a.ldw; f.ws.rows = a.n; f.ws.cols = a.k;
   f.x = operand_of(a.dtype, f.xs, c, &f.stage_x);
@@ -133,15 +148,18 @@ int forward(const qrbl_linear_args& a, void* workspace, size_t bytes, cudaStream
   const Forward f = plan_forward(a, &c);
   if (c.used > 0 && (workspace == nullptr || bytes < c.used)) return QRB_ERR_WORKSPACE;
   if (c.used > 0 && !aligned16(workspace)) return QRB_ERR_INVALID_ARG;
-  if (f.stage_x && (rc = fill(a.dtype, f.xs, f.x, s)) != QRB_OK) return rc;
-  if (f.stage_w && (rc = fill(a.dtype, f.ws, f.w, s)) != QRB_OK) return rc;
+  if (f.rows) return launch_rows(a.dtype, f.x, f.w, a.m, a.n, a.k, e, s);
+  Prepare before;
+  if (f.stage_x) add_stage(&before, f.xs, f.x);
+  if (f.stage_w) add_stage(&before, f.ws, f.w);
+  if (before.stages > 0 && (rc = launch_prepare(a.dtype, before, s)) != QRB_OK) return rc;
   Product p;
   p.kind = kForward;
   p.size = f.size;
   p.a = f.x; p.b = f.w;
   p.part = f.part;
   p.e = e;
-  return launch_products(a.dtype, &p, 1, f.plan, s);
+  return launch_products(a.dtype, &p, 1, f.plan, nullptr, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -178,7 +196,7 @@ int check(const qrbl_linear_backward_args& a) {
 
 struct Backward {
   bool dx = false, dw = false, db = false;
-  bool dz_kernel = false;  // dz (or its sums) need the elementwise kernel
+  bool dz_kernel = false;  // dz (or its sums) are computed first
   bool dz_stored = false;
   bool stage_x = false, stage_w = false;
   Source xs, ws;
@@ -253,8 +271,10 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
     if (b.db && (rc = zero_rows(a.dbias, a.n, 1, a.n, es, s)) != QRB_OK) return rc;
     return QRB_OK;
   }
+  Prepare before;
   if (b.dz_kernel) {
-    DzArgs d;
+    DzArgs& d = before.dz;
+    before.has_dz = true;
     d.dy = a.dy; d.lddy = a.lddy;
     d.z = a.z; d.ldz = a.ldz;
     d.z_codes = a.z_codes; d.z_exps = a.z_exponents;
@@ -266,17 +286,23 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
       d.plane = b.dz.plane;
     }
     d.part = b.colsum;
-    if ((rc = launch_dz(a.dtype, d, s)) != QRB_OK) return rc;
-    if (b.db && (rc = launch_colsum(a.dtype, b.colsum, b.colsum_blocks, a.n, a.dbias, s)) != QRB_OK)
-      return rc;
   }
+  if (b.stage_x) add_stage(&before, b.xs, b.x);
+  if (b.stage_w) add_stage(&before, b.ws, b.w);
+  if ((before.has_dz || before.stages > 0) &&
+      (rc = launch_prepare(a.dtype, before, s)) != QRB_OK)
+    return rc;
+  ColSum sum;
+  sum.part = b.colsum;
+  sum.blocks = b.colsum_blocks;
+  sum.n = a.n;
+  sum.out = a.dbias;
   auto rows16 = [&](const void* p, int64_t ld, int64_t rows) {
     return aligned16(p) && (rows <= 1 || (ld * es) % 16 == 0);
   };
   Product p[2];
   int i = 0;
   if (b.dw) {
-    if (b.stage_x && (rc = fill(a.dtype, b.xs, b.x, s)) != QRB_OK) return rc;
     p[i].kind = kGradW;
     p[i].a = b.dz; p[i].b = b.x;
     p[i].e.out = a.dw; p[i].e.ldo = a.lddw;
@@ -284,7 +310,6 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
     ++i;
   }
   if (b.dx) {
-    if (b.stage_w && (rc = fill(a.dtype, b.ws, b.w, s)) != QRB_OK) return rc;
     p[i].kind = kGradIn;
     p[i].a = b.dz; p[i].b = b.w;
     p[i].e.out = a.dx; p[i].e.ldo = a.lddx;
@@ -295,7 +320,8 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
     p[j].size = b.size[j];
     p[j].part = b.part[j];
   }
-  return i == 0 ? QRB_OK : launch_products(a.dtype, p, i, b.plan, s);
+  if (i > 0) return launch_products(a.dtype, p, i, b.plan, b.db ? &sum : nullptr, s);
+  return b.db ? launch_colsum(a.dtype, sum, s) : QRB_OK;
 }
 
 int check_packed(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols,

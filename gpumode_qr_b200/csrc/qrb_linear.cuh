@@ -123,6 +123,29 @@ __device__ __forceinline__ void values8(const Raw8<T>& r, float (&v)[8]) {
   }
 }
 
+// 32 consecutive elements, 16-byte aligned, as they are in memory.
+template <typename T>
+struct Raw32 {
+  Raw8<T> r[4];
+};
+template <typename T>
+__device__ __forceinline__ Raw32<T> load_raw32(const T* p) {
+  Raw32<T> out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out.r[i] = load_raw8<T>(p + 8 * i, true, 8);
+  return out;
+}
+template <typename T>
+__device__ __forceinline__ void add_raw32(float (&v)[32], const Raw32<T>& r) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[8];
+    values8<T>(r.r[i], f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[8 * i + j] += f[j];
+  }
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_n(T* p, bool vec, int valid, const float (&in)[N]) {
   if (vec && valid >= N) {
@@ -144,75 +167,158 @@ __device__ __forceinline__ void store_n(T* p, bool vec, int valid, const float (
 // ---------------------------------------------------------------------------
 // activations
 // ---------------------------------------------------------------------------
-// EXACT (FP32 layers): the library functions. Otherwise (results rounded to 8
-// or 11 bits): the hardware exponential and reciprocal (relative error below
-// 2^-20), and Phi from Abramowitz and Stegun 7.1.26 (absolute error of erf
-// below 1.5e-7).
-template <bool EXACT>
-__device__ __forceinline__ float sigmoid(float v) {
-  if constexpr (EXACT) return 1.0f / (1.0f + expf(-v));
-  return __fdividef(1.0f, 1.0f + __expf(-v));  // exp overflow: 1 / inf = 0
-}
-
-// Phi(z), and exp(-z^2 / 2) for its derivative.
-template <bool EXACT>
-__device__ __forceinline__ float normal_cdf(float z, float* gauss) {
-  const float h = z * 0.70710678118654752f;
-  if constexpr (EXACT) {
-    *gauss = expf(-h * h);
-    return 0.5f * erfcf(-h);
-  }
-  const float x = fabsf(h);
-  const float e = __expf(-x * x);
-  const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float q = 0.5f * p * t * e;  // erfc(x) / 2
-  *gauss = e;
-  return z >= 0.f ? 1.0f - q : (z < 0.f ? q : z);  // NaN stays NaN
-}
-
+// Two values at a time in packed FP32, with the hardware exponential and
+// reciprocal (relative error below 2^-21). Every activation is z / (1 + 2^t)
+// with t a polynomial in z: t = -log2(e) z for SILU,
+// -log2(e) 2 sqrt(2 / pi) (z + 0.044715 z^3) for GELU_TANH, and for GELU a
+// degree-13 odd polynomial fitted here to -log2(e) logit(Phi(z)) so that Phi is
+// within 6e-8 (weighted minimax over |z| <= 7; beyond, t keeps its sign and
+// grows, so Phi saturates): as close as z / 2 (1 + erf) in FP32. The library's
+// expf, erfcf and division keep more of the far tails' relative accuracy but
+// cost four times the instructions, and unrolled over a row they no longer fit
+// the instruction cache (an FP32 128 x 128 tile's epilogue took 17,000 clocks).
 constexpr float kTanhC = 1.5957691216057308f;  // 2 sqrt(2 / pi): tanh(u) = 2 sigmoid(2 u) - 1
 
-template <bool EXACT>
-__device__ __forceinline__ float act_fn(float z, int act) {
-  switch (act) {
-    case QRBL_ACT_RELU: return z > 0.f ? z : (z <= 0.f ? 0.f : z);
-    case QRBL_ACT_GELU: {
-      float g;
-      return z * normal_cdf<EXACT>(z, &g);
-    }
-    case QRBL_ACT_GELU_TANH: return z * sigmoid<EXACT>(kTanhC * fmaf(0.044715f * z * z, z, z));
-    case QRBL_ACT_SILU: return z * sigmoid<EXACT>(z);
-    default: return z;
-  }
+// Two FP32 values in one 64-bit register.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 f2_of(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f2 f2_of(float a) { return f2_of(a, a); }
+__device__ __forceinline__ void f2_to(f2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ f2 ex2_2(f2 x) {
+  float a, b;
+  f2_to(x, a, b);
+  return f2_of(ex2(a), ex2(b));
+}
+__device__ __forceinline__ f2 rcp_2(f2 x) {
+  float a, b, r, q;
+  f2_to(x, a, b);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(b));
+  return f2_of(r, q);
 }
 
-template <bool EXACT>
-__device__ __forceinline__ float act_grad_fn(float z, int act) {
+constexpr float kLog2e = 1.4426950408889634f;
+// 1 / (1 + 2^t(z)); zz = z^2
+template <int ACT>
+__device__ __forceinline__ f2 gate2(f2 z, f2 zz) {
+  f2 t;
+  if constexpr (ACT == QRBL_ACT_SILU) {
+    t = mul2(z, f2_of(-kLog2e));
+  } else if constexpr (ACT == QRBL_ACT_GELU_TANH) {
+    t = mul2(z, fma2(zz, f2_of(-kLog2e * kTanhC * 0.044715f), f2_of(-kLog2e * kTanhC)));
+  } else {
+    f2 q = f2_of(-kLog2e * 3.51234251e-09f);
+    q = fma2(q, zz, f2_of(-kLog2e * -2.64526714e-07f));
+    q = fma2(q, zz, f2_of(-kLog2e * 7.92948924e-06f));
+    q = fma2(q, zz, f2_of(-kLog2e * -1.10612389e-04f));
+    q = fma2(q, zz, f2_of(-kLog2e * -6.51899468e-05f));
+    q = fma2(q, zz, f2_of(-kLog2e * 7.26661691e-02f));
+    q = fma2(q, zz, f2_of(-kLog2e * 1.59576988f));
+    t = mul2(z, q);
+  }
+  return rcp_2(add2(ex2_2(t), f2_of(1.f)));
+}
+template <int ACT>
+__device__ __forceinline__ f2 act2(f2 z) {
+  return mul2(z, gate2<ACT>(z, mul2(z, z)));
+}
+template <int ACT>
+__device__ __forceinline__ f2 act_grad2(f2 z) {
+  const f2 zz = mul2(z, z);
+  if constexpr (ACT == QRBL_ACT_GELU) {
+    // Phi(z) + z g / sqrt(2 pi) with g = exp(-z^2 / 2), which also gives Phi:
+    // by Abramowitz and Stegun 7.1.26, with x = |z| / sqrt(2) and
+    // t = 1 / (1 + 0.3275911 x), erfc(x) = g (a1 t + .. + a5 t^5) within
+    // 1.5e-7. (One exponential and one reciprocal; the polynomial above would
+    // need a second exponential for g.)
+    const f2 sign = 0x8000000080000000ull;
+    const f2 g = ex2_2(mul2(zz, f2_of(-0.5f * kLog2e)));
+    const f2 t = rcp_2(fma2(z & ~sign, f2_of(0.3275911f * 0.70710678118654752f), f2_of(1.f)));
+    f2 q = fma2(t, f2_of(-0.5f * 1.061405429f), f2_of(0.5f * 1.453152027f));
+    q = fma2(q, t, f2_of(-0.5f * 1.421413741f));
+    q = fma2(q, t, f2_of(0.5f * 0.284496736f));
+    q = fma2(q, t, f2_of(-0.5f * 0.254829592f));
+    const f2 half = fma2(mul2(q, t), g, f2_of(0.5f));  // 1 / 2 - erfc(x) / 2 >= 0
+    const f2 phi = add2(half | (z & sign), f2_of(0.5f));
+    return fma2(mul2(z, f2_of(0.3989422804014327f)), g, phi);
+  }
+  const f2 s = gate2<ACT>(z, zz);
+  const f2 d = fma2(mul2(s, f2_of(-1.f)), s, s);  // s (1 - s)
+  if constexpr (ACT == QRBL_ACT_GELU_TANH) {
+    float a, b;
+    f2_to(zz, a, b);  // capped: the factor stays finite where s (1 - s) is 0
+    const f2 cap = f2_of(fminf(a, 1e6f), fminf(b, 1e6f));
+    return fma2(mul2(z, d), fma2(cap, f2_of(0.134145f * kTanhC), f2_of(kTanhC)), s);
+  }
+  return fma2(z, d, s);
+}
+
+// v <- act(v), and d <- d act'(z).
+template <int ACT, int N>
+__device__ __forceinline__ void act_n(float (&v)[N]) {
+  if constexpr (ACT == QRBL_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i];  // NaN stays NaN
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) f2_to(act2<ACT>(f2_of(v[i], v[i + 1])), v[i], v[i + 1]);
+  }
+}
+template <int ACT, int N>
+__device__ __forceinline__ void act_grad_n(float (&d)[N], const float (&z)[N]) {
+  if constexpr (ACT == QRBL_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] *= z[i] > 0.f ? 1.f : (z[i] <= 0.f ? 0.f : z[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      f2_to(mul2(f2_of(d[i], d[i + 1]), act_grad2<ACT>(f2_of(z[i], z[i + 1]))), d[i], d[i + 1]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void act_by(float (&v)[N], int act) {
   switch (act) {
-    case QRBL_ACT_RELU: return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
-    case QRBL_ACT_GELU: {
-      float g;
-      const float p = normal_cdf<EXACT>(z, &g);
-      return fmaf(0.3989422804014327f * z, g, p);
-    }
-    case QRBL_ACT_GELU_TANH: {
-      const float z2 = z * z;
-      const float s = sigmoid<EXACT>(kTanhC * fmaf(0.044715f * z2, z, z));
-      // z s (1 - s) u' with u' = kTanhC (1 + 3 * 0.044715 z^2); s (1 - s) is 0
-      // where the sigmoid has saturated, also where u' overflows
-      const float d = s * (1.0f - s);
-      return d > 0.f ? fmaf(z * d, kTanhC * fmaf(0.134145f, z2, 1.0f), s) : s;
-    }
-    case QRBL_ACT_SILU: {
-      const float s = sigmoid<EXACT>(z);
-      const float d = s * (1.0f - s);
-      return d > 0.f ? fmaf(z, d, s) : s;
-    }
-    default: return 1.f;
+    case QRBL_ACT_RELU: act_n<QRBL_ACT_RELU>(v); break;
+    case QRBL_ACT_GELU: act_n<QRBL_ACT_GELU>(v); break;
+    case QRBL_ACT_GELU_TANH: act_n<QRBL_ACT_GELU_TANH>(v); break;
+    case QRBL_ACT_SILU: act_n<QRBL_ACT_SILU>(v); break;
+    default: break;
+  }
+}
+template <int N>
+__device__ __forceinline__ void act_grad_by(float (&d)[N], const float (&z)[N], int act) {
+  switch (act) {
+    case QRBL_ACT_RELU: act_grad_n<QRBL_ACT_RELU>(d, z); break;
+    case QRBL_ACT_GELU: act_grad_n<QRBL_ACT_GELU>(d, z); break;
+    case QRBL_ACT_GELU_TANH: act_grad_n<QRBL_ACT_GELU_TANH>(d, z); break;
+    case QRBL_ACT_SILU: act_grad_n<QRBL_ACT_SILU>(d, z); break;
+    default: break;
   }
 }
 
@@ -284,13 +390,20 @@ __device__ __forceinline__ float finite_amax(const float (&v)[N]) {
   for (int i = 0; i < N; ++i) a = fmaxf(a, finite_f(v[i]) ? fabsf(v[i]) : 0.f);
   return a;
 }
+// One code as a value.
+__device__ __forceinline__ float value_of(int code, float step) {
+  return code == kNanCode ? __uint_as_float(0x7fc00000u) : (float)code * step;
+}
 // Four codes as values. A byte q + 128 put under the exponent of 2^23 is the
 // float 2^23 + 128 + q; kNanCode (byte 0 after the flip) becomes NaN.
 __device__ __forceinline__ void decode4(uint32_t codes, float step, float (&out)[4]) {
   const uint32_t y = codes ^ 0x80808080u;
+  const f2 off = f2_of(-8388736.f), st = f2_of(step);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    out[i] = (__uint_as_float(__byte_perm(y, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+  for (int i = 0; i < 4; i += 2)
+    f2_to(mul2(add2(f2_of(__uint_as_float(__byte_perm(y, 0x4b000000u, 0x7540 + i)),
+                          __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7541 + i))),
+                    off), st), out[i], out[i + 1]);
   if ((y - 0x01010101u) & ~y & 0x80808080u) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -369,9 +482,16 @@ struct ProductPlan {
   int64_t part_rows[2] = {0, 0}, part_ld[2] = {0, 0};
   size_t part_bytes[2] = {0, 0};
 };
+struct ColSum;
 ProductPlan plan_products(int dtype, const ProductSize* sizes, int count);
+// sum (may be null): column sums finished in the same launch.
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
-                    cudaStream_t s);
+                    const ColSum* sum, cudaStream_t s);
+// The forward product of m <= rows_most(dtype) rows, x and w read in place at
+// any alignment.
+int64_t rows_most(int dtype);
+int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
+                const Epilogue& e, cudaStream_t s);
 // out = epilogue(sum of `splits` partial sums), part[s][row][col] with rows
 // `rows` and row stride ld (splits may be 0).
 int launch_join(int dtype, const float* part, int splits, int64_t rows, int64_t ld, int64_t m,
@@ -381,14 +501,22 @@ int launch_pack(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols
                 int8_t* exps, cudaStream_t s);
 int launch_unpack(int dtype, const int8_t* codes, const int8_t* exps, int64_t rows, int64_t cols,
                   void* x, int64_t ld, cudaStream_t s);
+// What has to be done before a product, in one launch: up to two operands
+// staged, and dz = dy act'(z).
 // A plain (src) or packed (codes, exps) matrix as a product's operand: copied
 // to dst with row stride ldd, FP32 split into three planes `plane` apart.
-int launch_stage(int dtype, const void* src, int64_t lds, const int8_t* codes, const int8_t* exps,
-                 int64_t rows, int64_t cols, void* dst, int64_t ldd, int64_t plane,
-                 cudaStream_t s);
-// dz = dy act'(z) as an operand (dst may be null: only the sums), and the
-// column sums of the unrounded dz over each block of colsum_rows(m, n) rows
-// into part [blocks][n] (null: none).
+struct StageArgs {
+  const void* src = nullptr;
+  int64_t lds = 0;
+  const int8_t* codes = nullptr;
+  const int8_t* exps = nullptr;
+  int64_t rows = 0, cols = 0;
+  void* dst = nullptr;
+  int64_t ldd = 0, plane = 0;
+};
+// dz as an operand (dst may be null: only the sums), and the column sums of the
+// unrounded dz over each block of colsum_rows(m, n) rows into part [blocks][n]
+// (null: none).
 int colsum_rows(int64_t m, int64_t n);
 struct DzArgs {
   const void* dy = nullptr;
@@ -403,9 +531,30 @@ struct DzArgs {
   int64_t ldd = 0, plane = 0;
   float* part = nullptr;
 };
-int launch_dz(int dtype, const DzArgs& a, cudaStream_t s);
-int launch_colsum(int dtype, const float* part, int64_t blocks, int64_t n, void* out,
-                  cudaStream_t s);
+struct Prepare {
+  StageArgs stage[2];
+  int stages = 0;
+  DzArgs dz;
+  bool has_dz = false;
+};
+int launch_prepare(int dtype, const Prepare& p, cudaStream_t s);
+// out[col] = sum of part[block][col]; a product's launch can do it as well
+// (ColSum), while its first tiles accumulate.
+struct ColSum {
+  const float* part = nullptr;
+  int64_t blocks = 0, n = 0;
+  void* out = nullptr;
+};
+template <typename T>
+__device__ __forceinline__ void column_sum(const ColSum& c, int64_t first, int64_t step) {
+  for (int64_t col = first; col < c.n; col += step) {
+    float s = 0.f;
+#pragma unroll 16
+    for (int64_t b = 0; b < c.blocks; ++b) s += __ldg(c.part + b * c.n + col);
+    reinterpret_cast<T*>(c.out)[col] = from_f<T>(s);
+  }
+}
+int launch_colsum(int dtype, const ColSum& c, cudaStream_t s);
 
 }  // namespace lin
 }  // namespace qrb

@@ -52,6 +52,7 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kSmemMost = 232448;  // 227 KB
+constexpr int kPitch = 33;              // words of a row in a warp's turning buffer
 constexpr uint32_t ATOM = 64 * 128;     // MN-major box: 64 reduction rows of 128 bytes
 
 // control block at the start of shared memory
@@ -66,9 +67,12 @@ struct Lay {
   static constexpr int BROWS = BN / CG;              // B's columns of one CTA
   static constexpr uint32_t A = BM * 128, B = BROWS * 128;
   static constexpr uint32_t STAGE = NP * (A + B);
-  static constexpr int FIT = (int)((kSmemMost - CTRL - 1024) / STAGE);
+  // rows that a warp turns at a time (FP32: few, which leaves room for a stage)
+  static constexpr int TROWS = NP == 3 ? 8 : 32;
+  static constexpr uint32_t TURN = kEpiWarps * TROWS * kPitch * 4;
+  static constexpr int FIT = (int)((kSmemMost - CTRL - 1024 - TURN) / STAGE);
   static constexpr int ST = FIT < kMaxStages ? FIT : kMaxStages;
-  static constexpr uint32_t SMEM = 1024 + CTRL + ST * STAGE;  // 1024: base alignment
+  static constexpr uint32_t SMEM = 1024 + CTRL + ST * STAGE + TURN;  // 1024: base alignment
   static constexpr int ACC = NP == 3 ? 2 * BN : BN;  // TMEM columns per buffer
   static constexpr int TMEM = 2 * ACC;
   static_assert(ST >= 2 && TMEM <= 512 && TMEM >= 32, "stage ring and TMEM");
@@ -86,7 +90,6 @@ struct Problem {
   float* part;      // splits > 1: partial tiles
   long long part_rows, part_ld;
   Epilogue e;
-  int vcodes;       // packed rows are 16-byte aligned
 };
 // Which items a worker (CTA or pair) runs: of problem 0 every workers-th,
 // worker by worker; then of problem 1 its count, x or (with one more of
@@ -100,6 +103,7 @@ struct Schedule {
 struct Args {
   Problem p[2];
   Schedule s;
+  ColSum sum;       // column sums to finish beside the products (out null: none)
   int* err;
   long long limit;
   int skip_mma;     // test hook: withhold the MMAs, so that the waits run out
@@ -227,26 +231,27 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
-template <int CG>
-__device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity) {
-  if constexpr (CG == 1) return tma::mbar_try(bar, parity);
-  uint32_t done;  // the arrivals may come from the other CTA
+// Bounded: false on a timeout (which sets *abort) or once *abort is set.
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
+      : "=r"(pred));
+  return pred != 0;
 }
-// Bounded: false on a timeout (which sets *abort) or once *abort is set.
-template <int CG>
+// Block-scope acquire, also for what the other CTA of a pair announces: all that
+// passes between them is TMA and TMEM traffic, ordered by the barriers
+// themselves; a cluster-scope release or acquire would wait for this CTA's
+// global stores and drop its L1 (measured: 25,000 clocks per 128 x 256 tile
+// with GELU and packing, against 9,000 without).
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, long long limit,
                                               volatile int* abort) {
-  if (mbar_done<CG>(bar, parity)) return true;
+  if (tma::mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!mbar_done<CG>(bar, parity)) {
+  while (!tma::mbar_try(bar, parity)) {
     if (*abort != 0) return false;
     if (clock64() - t0 > limit) {
       *abort = 1;
@@ -254,6 +259,12 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, lon
     }
   }
   return true;
+}
+
+// The same for a whole warp: every lane gets the same answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, long long limit,
+                                          volatile int* abort) {
+  return __all_sync(kFull, wait_or_abort(bar, parity, limit, abort));
 }
 
 template <int CG>
@@ -281,65 +292,137 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
   }
 }
 
-template <typename T, int ACT>
-__device__ __forceinline__ void act32(float (&v)[32]) {
+// A warp's block of 32 columns of up to eight rows, packed (lane = column).
+template <typename T>
+__device__ __forceinline__ void pack_rows(const float (&p)[8], int64_t row, int left, bool live,
+                                          int col, const Problem& a) {
+  constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
+  const int lane = threadIdx.x & 31;
+  const Epilogue& e = a.e;
+  float amax[8];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = act_fn<sizeof(T) == 4>(v[i], ACT);
+  for (int k = 0; k < 8; ++k) amax[k] = live && finite_f(p[k]) ? fabsf(p[k]) : 0.f;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2)
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      amax[k] = fmaxf(amax[k], __shfl_xor_sync(kFull, amax[k], o));
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int ex = block_exponent(amax[k], lo, hi);
+    const float one[4] = {p[k], 0.f, 0.f, 0.f};
+    uint32_t w[1];
+    encode(one, ex, finite_f(p[k]) && ex < hi, ex == hi ? 63.f : 127.f, w);
+    if (live && k < left) {
+      e.z_codes[(row + k) * a.n + col + lane] = (int8_t)(w[0] & 255u);
+      if (lane == 0)
+        e.z_exps[(row + k) * ((a.n + kBlk - 1) / kBlk) + col / kBlk] = (int8_t)ex;
+    }
+  }
 }
 
-// The epilogue of 32 consecutive columns of one row (one thread).
+// The epilogue of a warp's 32 x 32 block, rows from row0, columns from col, as
+// lane = column: the block (v: lane = row) is turned through shared memory, TROWS
+// rows at a time, so that every access is consecutive elements of one row,
+// whatever their alignment: blocks that are cut by the matrix's edge or whose
+// rows are not 16-byte aligned.
+template <typename T, bool FWD, int TROWS>
+__device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, int col,
+                                              const Problem& a, float* turn) {
+  if (row0 >= a.m || col >= a.n) return;
+  const int lane = threadIdx.x & 31;
+  const int rows = a.m - row0 < 32 ? a.m - row0 : 32;
+  const bool live = col + lane < a.n;
+  const Epilogue& e = a.e;
+  float bias = 0.f;
+  if constexpr (FWD) {
+    if (e.bias != nullptr && live) bias = to_f<T>(reinterpret_cast<const T*>(e.bias)[col + lane]);
+  }
+#pragma unroll 1
+  for (int base = 0; base < rows; base += TROWS) {
+    __syncwarp();
+    if (lane >= base && lane < base + TROWS) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) turn[(lane - base) * kPitch + i] = v[i];
+    }
+    __syncwarp();
+    const int most = rows - base < TROWS ? rows - base : TROWS;
+#pragma unroll 1
+    for (int r0 = 0; r0 < most; r0 += 8) {
+      const int64_t row0g = row0 + base + r0;
+      const int left = most - r0;
+      // eight rows' values and residuals together, then eight rows' results
+      float p[8], q[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        p[k] = k < left ? turn[(r0 + k) * kPitch + lane] : 0.f;
+        q[k] = 0.f;
+      }
+      if constexpr (FWD) {
+        if (e.residual != nullptr) {
+          const T* s = reinterpret_cast<const T*>(e.residual) + row0g * e.ldr + col + lane;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (live && k < left) q[k] = to_f<T>(s[k * e.ldr]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] += bias;
+        if (e.z != nullptr && live) {
+          T* z = reinterpret_cast<T*>(e.z) + row0g * e.ldz + col + lane;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < left) z[k * e.ldz] = from_f<T>(p[k]);
+        }
+        if (e.z_codes != nullptr) pack_rows<T>(p, row0g, left, live, col, a);
+        act_by(p, e.act);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] += q[k];
+      }
+      if (live) {
+        T* out = reinterpret_cast<T*>(e.out) + row0g * e.ldo + col + lane;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < left) out[k * e.ldo] = from_f<T>(p[k]);
+      }
+    }
+  }
+}
+
+// The same for a whole block of 16-byte aligned rows, as lane = row: each lane's
+// 32 columns are whole sectors. 16-bit types: the bias and residual were loaded
+// before the accumulators were ready.
 template <typename T, bool FWD>
-__device__ __forceinline__ void finish32(float (&v)[32], int row, int col, const Problem& a) {
-  if (row >= a.m || col >= a.n) return;
-  const int valid = a.n - col < 32 ? a.n - col : 32;
+__device__ __forceinline__ void finish32(float (&v)[32], int row, int col, const Problem& a,
+                                         const Raw32<T>& bias, const Raw32<T>& res) {
   const Epilogue& e = a.e;
   if constexpr (FWD) {
-    if (e.bias != nullptr) {
-      float b[32];
-      load_n<T, 32>(reinterpret_cast<const T*>(e.bias) + col, e.vec, valid, b);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] += b[i];
+    if (e.bias != nullptr) add_raw32<T>(v, bias);
+    Raw32<T> late;  // (FP32: no registers to hold it earlier)
+    if constexpr (sizeof(T) == 4) {
+      if (e.residual != nullptr)
+        late = load_raw32<T>(reinterpret_cast<const T*>(e.residual) + (int64_t)row * e.ldr + col);
     }
     if (e.z != nullptr)
-      store_n<T, 32>(reinterpret_cast<T*>(e.z) + (int64_t)row * e.ldz + col, e.vec, valid, v);
+      store_n<T, 32>(reinterpret_cast<T*>(e.z) + (int64_t)row * e.ldz + col, true, 32, v);
     if (e.z_codes != nullptr) {
       constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
-      float amax = 0.f;  // columns beyond n are 0: the operand's rows there read as 0
+      float amax = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; ++i) amax = max_abs_nan(amax, v[i]);
       const bool fine = finite_f(amax);
       if (!fine) amax = finite_amax(v);
       const int ex = block_exponent(amax, lo, hi);
-      const bool plain = fine && ex < hi;
       uint32_t w[8];
-      encode(v, ex, plain, ex == hi ? 63.f : 127.f, w);
-      int8_t* out = e.z_codes + (int64_t)row * a.n + col;
-      if (a.vcodes && valid == 32) {
-        reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < valid) out[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
-      }
+      encode(v, ex, fine && ex < hi, ex == hi ? 63.f : 127.f, w);
+      uint4* out = reinterpret_cast<uint4*>(e.z_codes + (int64_t)row * a.n + col);
+      out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      out[1] = make_uint4(w[4], w[5], w[6], w[7]);
       e.z_exps[(int64_t)row * ((a.n + kBlk - 1) / kBlk) + col / kBlk] = (int8_t)ex;
     }
-    switch (e.act) {
-      case QRBL_ACT_RELU: act32<T, QRBL_ACT_RELU>(v); break;
-      case QRBL_ACT_GELU: act32<T, QRBL_ACT_GELU>(v); break;
-      case QRBL_ACT_GELU_TANH: act32<T, QRBL_ACT_GELU_TANH>(v); break;
-      case QRBL_ACT_SILU: act32<T, QRBL_ACT_SILU>(v); break;
-      default: break;
-    }
-    if (e.residual != nullptr) {
-      float r[32];
-      load_n<T, 32>(reinterpret_cast<const T*>(e.residual) + (int64_t)row * e.ldr + col, e.vec,
-                    valid, r);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] += r[i];
-    }
+    act_by(v, e.act);
+    if (e.residual != nullptr) add_raw32<T>(v, sizeof(T) == 4 ? late : res);
   }
-  store_n<T, 32>(reinterpret_cast<T*>(e.out) + (int64_t)row * e.ldo + col, e.vec, valid, v);
+  store_n<T, 32>(reinterpret_cast<T*>(e.out) + (int64_t)row * e.ldo + col, true, 32, v);
 }
 
 // A split product's partial tile (rows and columns padded to whole tiles).
@@ -365,9 +448,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t ring = base + CTRL;
   volatile int* s_abort = reinterpret_cast<volatile int*>(sm + OFF_ABORT);
   auto BAR = [&](int i) { return base + 8u * (uint32_t)i; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (the shuffle tells the compiler that a warp's lanes agree: the loading and
+  // the issuing warp run whole, in uniform registers, and one elected lane
+  // issues; with a lane's own registers each tcgen05.mma took 120 clocks)
+  const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int worker = (int)blockIdx.x / CG, rank = (int)blockIdx.x % CG;
 
+  if (warp == kEpiWarps && lane == 0) {
+    tma::prefetch_map(&map_a0);
+    tma::prefetch_map(&map_b0);
+    if (a.p[1].items > 0) {
+      tma::prefetch_map(&map_a1);
+      tma::prefetch_map(&map_b1);
+    }
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::ST; ++s) {
       tma::mbar_init(BAR(B_FULL + s), 1);
@@ -389,50 +483,51 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + OFF_TMEM);
 
   if (warp == kEpiWarps) {  // ---- loads ----
-    if (lane == 0) {
-      tma::prefetch_map(&map_a0);
-      tma::prefetch_map(&map_b0);
-      int u = 0;  // stages issued
-      for (int step = 0; *s_abort == 0; ++step) {
-        const Item it = item_of<CG, BN>(a, worker, step);
-        if (it.prob < 0) break;
-        const CUtensorMap* ma = it.prob == 0 ? &map_a0 : &map_a1;
-        const CUtensorMap* mb = it.prob == 0 ? &map_b0 : &map_b1;
-        const bool amn = a.p[it.prob].amn != 0, bmn = a.p[it.prob].bmn != 0;
-        const int am = it.m0 + rank * BM, bn = it.n0 + rank * L::BROWS;
-        for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          const int s = u % L::ST;
-          if (u >= L::ST && !wait_or_abort<CG>(BAR(B_EMPTY + s), (uint32_t)((u / L::ST - 1) & 1),
-                                               a.limit, s_abort))
-            break;
+    int u = 0;  // stages issued
+    bool live = true;
+    for (int step = 0; live; ++step) {
+      const Item it = item_of<CG, BN>(a, worker, step);
+      if (it.prob < 0) break;
+      const CUtensorMap* ma = it.prob == 0 ? &map_a0 : &map_a1;
+      const CUtensorMap* mb = it.prob == 0 ? &map_b0 : &map_b1;
+      const bool amn = a.p[it.prob].amn != 0, bmn = a.p[it.prob].bmn != 0;
+      const int am = it.m0 + rank * BM, bn = it.n0 + rank * L::BROWS;
+      for (int kb = it.kb0; kb < it.kb1; ++kb) {
+        const int s = u % L::ST;
+        if (u >= L::ST)
+          live = warp_wait(BAR(B_EMPTY + s), (uint32_t)((u / L::ST - 1) & 1), a.limit, s_abort);
+        if (!live) break;
+        const uint32_t bar = CG == 1 ? BAR(B_FULL + s) : in_first_cta(BAR(B_FULL + s));
+        const uint32_t st = ring + s * L::STAGE;
+        if (elect_one()) {
           if (rank == 0) tma::mbar_expect_tx(BAR(B_FULL + s), CG * L::STAGE);
-          const uint32_t bar = CG == 1 ? BAR(B_FULL + s) : in_first_cta(BAR(B_FULL + s));
-          const uint32_t st = ring + s * L::STAGE;
 #pragma unroll
           for (int p = 0; p < L::NP; ++p)
             load_tile<CG, BM>(st + p * L::A, ma, amn, bar, am, kb, p);
 #pragma unroll
           for (int p = 0; p < L::NP; ++p)
             load_tile<CG, L::BROWS>(st + L::NP * L::A + p * L::B, mb, bmn, bar, bn, kb, p);
-          ++u;
         }
+        __syncwarp();
+        ++u;
       }
-      if (*s_abort != 0) {  // no load may land after the block has gone
-        if constexpr (CG == 1) {
-          for (int v = u > L::ST ? u - L::ST : 0; v < u; ++v)
-            tma::mbar_wait_bounded(BAR(B_FULL + v % L::ST), (uint32_t)((v / L::ST) & 1), a.limit);
-        } else {  // announced on one CTA's barrier: a fixed time, far above any load's
-          const long long t0 = clock64();
-          while (clock64() - t0 < 4000000LL) {
-          }
+    }
+    if (__any_sync(kFull, *s_abort != 0)) {  // no load may land after the block has gone
+      if constexpr (CG == 1) {
+        for (int v = u > L::ST ? u - L::ST : 0; v < u; ++v)
+          tma::mbar_wait_bounded(BAR(B_FULL + v % L::ST), (uint32_t)((v / L::ST) & 1), a.limit);
+      } else {  // announced on one CTA's barrier: a fixed time, far above any load's
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000LL) {
         }
       }
     }
   } else if (warp == kEpiWarps + 1) {  // ---- MMAs ----
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t fmt = __is_same(T, f16) ? 0u : 1u;  // F16 : BF16
       int u = 0, unit = 0;
-      for (int step = 0; *s_abort == 0; ++step) {
+      bool live = true;
+      for (int step = 0; live; ++step) {
         const Item it = item_of<CG, BN>(a, worker, step);
         if (it.prob < 0) break;
         const bool amn = a.p[it.prob].amn != 0, bmn = a.p[it.prob].bmn != 0;
@@ -440,46 +535,50 @@ __global__ void __launch_bounds__(kThreads, 1)
                             ((bmn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
                             ((uint32_t)((BM * CG) >> 4) << 24);
         const uint64_t ka = amn ? 2048 >> 4 : 32 >> 4, kbs = bmn ? 2048 >> 4 : 32 >> 4;
-        for (int kb = it.kb0; kb < it.kb1 && *s_abort == 0;) {
+        const uint64_t da0 = operand_desc(ring, amn);
+        const uint64_t db0 = operand_desc(ring + L::NP * L::A, bmn);
+        for (int kb = it.kb0; live && kb < it.kb1;) {
           const int end = L::NP == 3 && kb + kChain < it.kb1 ? kb + kChain : it.kb1;
           const int buf = unit & 1;
-          if (unit >= 2 && !wait_or_abort<CG>(BAR(B_ACCEMPTY + buf),
-                                              (uint32_t)((unit / 2 - 1) & 1), a.limit, s_abort))
-            break;
+          if (unit >= 2)
+            live = warp_wait(BAR(B_ACCEMPTY + buf), (uint32_t)((unit / 2 - 1) & 1), a.limit,
+                             s_abort);
           tc::fence_after();
           const uint32_t d = tmem + buf * L::ACC;
           uint32_t more = 0;
-          for (; kb < end; ++kb, ++u) {
+          for (; live && kb < end; ++kb, ++u) {
             const int s = u % L::ST;
-            if (!wait_or_abort<CG>(BAR(B_FULL + s), (uint32_t)((u / L::ST) & 1), a.limit, s_abort))
-              break;
+            live = warp_wait(BAR(B_FULL + s), (uint32_t)((u / L::ST) & 1), a.limit, s_abort);
+            if (!live) break;
             tc::fence_after();
-            const uint32_t sa = ring + s * L::STAGE, sb = sa + L::NP * L::A;
-            if (a.skip_mma == 0) {
+            const uint64_t at = (uint64_t)(s * (int)(L::STAGE >> 4));
+            if (a.skip_mma == 0 && elect_one()) {
 #pragma unroll
               for (int q = 0; q < (L::NP == 3 ? 6 : 1); ++q) {
                 // (0, 0) into the main accumulator, then the small products
                 constexpr int pi[6] = {0, 0, 1, 1, 0, 2}, pj[6] = {0, 1, 0, 1, 2, 0};
-                const uint64_t da = operand_desc(sa + pi[q] * L::A, amn);
-                const uint64_t db = operand_desc(sb + pj[q] * L::B, bmn);
+                const uint64_t da = da0 + at + (uint64_t)(pi[q] * (L::A >> 4));
+                const uint64_t db = db0 + at + (uint64_t)(pj[q] * (L::B >> 4));
                 const uint32_t dq = q == 0 ? d : d + BN;
 #pragma unroll
                 for (int k = 0; k < BK / 16; ++k)
                   mma_f16<CG>(dq, da + k * ka, db + k * kbs, id,
                               more | (q > 1 || k > 0 ? 1u : 0u));
               }
-              more = 1;
               commit<CG>(BAR(B_EMPTY + s));
             }
+            __syncwarp();
+            more = 1;
           }
-          if (*s_abort != 0) break;
-          if (a.skip_mma == 0) commit<CG>(BAR(B_ACCFULL + buf));
+          if (!live) break;
+          if (a.skip_mma == 0 && elect_one()) commit<CG>(BAR(B_ACCFULL + buf));
+          __syncwarp();
           ++unit;
         }
       }
-      if (*s_abort != 0) {  // no MMA may run on into freed TMEM (a pair: fixed time as above)
+      if (__any_sync(kFull, *s_abort != 0)) {  // no MMA may run on into freed TMEM (a pair: fixed time as above)
         if constexpr (CG == 1) {
-          tc::drain_mmas(BAR(B_FIN));
+          if (elect_one()) tc::drain_mmas(BAR(B_FIN));
         } else {
           const long long t0 = clock64();
           while (clock64() - t0 < 4000000LL) {
@@ -491,6 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quad = warp & 3, half = warp >> 2;
     constexpr int HC = BN / 2;  // columns of this warp
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    float* turn = reinterpret_cast<float*>(sm + CTRL + L::ST * L::STAGE) + warp * L::TROWS * kPitch;
     int unit = 0;
     auto hand_back = [&](int buf) {  // the accumulators are read
       tc::fence_before();
@@ -499,22 +599,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (CG == 1)
           tma::mbar_arrive(BAR(B_ACCEMPTY + buf));
         else
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+          asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
                            in_first_cta(BAR(B_ACCEMPTY + buf)))
                        : "memory");
       }
     };
+    if constexpr (!FWD) {
+      if (a.sum.out != nullptr)
+        column_sum<T>(a.sum, (int64_t)blockIdx.x * (kEpiWarps * 32) + threadIdx.x,
+                      (int64_t)gridDim.x * (kEpiWarps * 32));
+    }
     for (int step = 0;; ++step) {
       const Item it = item_of<CG, BN>(a, worker, step);
       if (it.prob < 0) break;
       const Problem& p = a.p[FWD ? 0 : it.prob];
-      const int row = it.m0 + rank * BM + quad * 32 + lane, col = it.n0 + half * HC;
+      const int row0 = it.m0 + rank * BM + quad * 32, col = it.n0 + half * HC;
       bool ok = true;
       if constexpr (L::NP == 1) {
+        // the bias and residual of a block are loaded while the accumulators
+        // (first block) or the block before are worked on
+        Raw32<T> bias, res;
+        const Epilogue& e = p.e;
+        const int row = row0 + lane;
+        // whole aligned blocks; all lanes agree except on rows beyond m
+        auto whole = [&](int c) { return e.vec != 0 && c + 32 <= p.n; };
+        auto ahead = [&](int c) { return FWD && p.splits == 1 && whole(c) && row < p.m; };
+        auto load_bias = [&](int c) {
+          if (e.bias != nullptr) bias = load_raw32<T>(reinterpret_cast<const T*>(e.bias) + c);
+        };
+        auto load_res = [&](int c) {
+          if (e.residual != nullptr)
+            res = load_raw32<T>(reinterpret_cast<const T*>(e.residual) +
+                                (int64_t)row * e.ldr + c);
+        };
+        if (ahead(col)) {
+          load_bias(col);
+          load_res(col);
+        }
         const int buf = unit & 1;
-        ok = *s_abort == 0 && wait_or_abort<CG>(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1),
-                                                a.limit, s_abort);
-        ok = __all_sync(kFull, ok);
+        ok = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
         if (!ok) break;
         tc::fence_after();
         const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
@@ -523,10 +646,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           float v[32];
           tc::tmem_ld32(t + c, v);
           if (c + 32 == HC) hand_back(buf);
-          if (p.splits > 1)
+          if (p.splits > 1) {
             partial32(v, row, col + c, it.split, p);
-          else
-            finish32<T, FWD>(v, row, col + c, p);
+          } else if (whole(col + c)) {
+            if (row < p.m) finish32<T, FWD>(v, row, col + c, p, bias, res);
+          } else {
+            finish_turned<T, FWD, L::TROWS>(v, row0, col + c, p, turn);
+          }
+          if (c + 32 < HC && ahead(col + c + 32)) {
+            load_bias(col + c + 32);
+            load_res(col + c + 32);
+          }
         }
         ++unit;
       } else {
@@ -537,9 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
         for (int kb = it.kb0; kb < it.kb1; kb += kChain, ++unit) {
           const int buf = unit & 1;
-          ok = *s_abort == 0 && wait_or_abort<CG>(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1),
-                                                  a.limit, s_abort);
-          ok = __all_sync(kFull, ok);
+          ok = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
           if (!ok) break;
           tc::fence_after();
           const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
@@ -554,12 +682,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           hand_back(buf);
         }
         if (!ok) break;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < HC / 32; ++c) {
-          if (p.splits > 1)
-            partial32(sum[c], row, col + c * 32, it.split, p);
-          else
-            finish32<T, FWD>(sum[c], row, col + c * 32, p);
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = HC == 32 || c == 0 ? sum[0][i] : sum[HC / 32 - 1][i];
+          const int at = col + c * 32;
+          if (p.splits > 1) {
+            partial32(v, row0 + lane, at, it.split, p);
+          } else if (p.e.vec != 0 && at + 32 <= p.n) {
+            if (row0 + lane < p.m) {
+              Raw32<T> bias;
+              if (FWD && p.e.bias != nullptr)
+                bias = load_raw32<T>(reinterpret_cast<const T*>(p.e.bias) + at);
+              finish32<T, FWD>(v, row0 + lane, at, p, bias, bias);
+            }
+          } else {
+            finish_turned<T, FWD, L::TROWS>(v, row0, at, p, turn);
+          }
         }
       }
     }
@@ -845,7 +985,7 @@ ProductPlan plan_products(int dtype, const ProductSize* sizes, int count) {
 }
 
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
-                    cudaStream_t s) {
+                    const ColSum* sum, cudaStream_t s) {
   const Device* d = device_info();
   if (d == nullptr) return QRB_ERR_DEVICE;
   if (!plan.ok) return QRB_ERR_UNSUPPORTED;
@@ -864,11 +1004,13 @@ int launch_products(int dtype, const Product* products, int count, const Product
     args.p[j].part_rows = plan.part_rows[i];
     args.p[j].part_ld = plan.part_ld[i];
     args.p[j].e = products[i].e;
-    args.p[j].vcodes = aligned16(products[i].e.z_codes) && z.n % 16 == 0;
+    if (products[i].e.z_codes != nullptr)  // packed rows 16-byte aligned too
+      args.p[j].e.vec &= aligned16(products[i].e.z_codes) && z.n % 16 == 0;
     items[j] = args.p[j].items;
     clocks[j] = item_clocks(f32, c, z.m, tiles_of(args.p[j].kb, plan.splits[i]));
   }
   make_schedule(items, clocks, d->sms / c.cg, &args.s);
+  if (sum != nullptr) args.sum = *sum;
   args.err = d->err;
   args.limit = device_wait_limit();
   args.skip_mma = test_skip_mma() ? 1 : 0;

@@ -22,7 +22,7 @@ or from an ``autograd.Function``).
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -34,24 +34,16 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 #: Values of a row that share one exponent in the packed form.
 PACK_BLOCK = 32
 
-_I64, _P = ctypes.c_int64, ctypes.c_void_p
-
-
-class _LinearArgs(ctypes.Structure):
-    _fields_ = [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
-                ("m", _I64), ("n", _I64), ("k", _I64),
-                ("x", _P), ("ldx", _I64), ("w", _P), ("ldw", _I64), ("bias", _P),
-                ("residual", _P), ("ldr", _I64), ("y", _P), ("ldy", _I64), ("z", _P),
-                ("ldz", _I64), ("z_codes", _P), ("z_exponents", _P)]
-
-
-class _BackwardArgs(ctypes.Structure):
-    _fields_ = [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
-                ("m", _I64), ("n", _I64), ("k", _I64),
-                ("dy", _P), ("lddy", _I64), ("x", _P), ("ldx", _I64), ("x_codes", _P),
-                ("x_exponents", _P), ("w", _P), ("ldw", _I64), ("z", _P), ("ldz", _I64),
-                ("z_codes", _P), ("z_exponents", _P), ("dx", _P), ("lddx", _I64), ("dw", _P),
-                ("lddw", _I64), ("dbias", _P)]
+# The C ABI's argument structs (qrbl_linear_args, qrbl_linear_backward_args) as
+# bytes, field by field in the header's order: two int32, then 8 bytes each
+# (sizes and strides signed, pointers unsigned, 0 for none).
+_LINEAR_FIELDS = ("dtype", "activation", "m", "n", "k", "x", "ldx", "w", "ldw", "bias", "residual",
+                  "ldr", "y", "ldy", "z", "ldz", "z_codes", "z_exponents")
+_linear_args = struct.Struct("@ii qqq Pq Pq P Pq Pq Pq PP").pack
+_BACKWARD_FIELDS = ("dtype", "activation", "m", "n", "k", "dy", "lddy", "x", "ldx", "x_codes",
+                    "x_exponents", "w", "ldw", "z", "ldz", "z_codes", "z_exponents", "dx", "lddx",
+                    "dw", "lddw", "dbias")
+_backward_args = struct.Struct("@ii qqq Pq Pq PP Pq Pq PP Pq Pq P").pack
 
 
 class PackedActivation(NamedTuple):
@@ -100,8 +92,8 @@ def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     (copying only if needed)."""
     if t.dim() != 2:
         t = t.reshape(-1, cols) if cols else t.new_empty((t.shape[:-1].numel(), 0))
-    s = t.stride()
-    if (s[1] != 1 and cols > 1) or (s[0] < cols and t.shape[0] > 1):
+    row, col = t.stride()
+    if (col != 1 and cols > 1) or (row < cols and t.shape[0] > 1):
         t = t.contiguous()
     return t
 
@@ -113,15 +105,29 @@ def _activation(name: str) -> int:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {name!r}") from None
 
 
-def _run(size, call, args, dev: torch.device) -> None:
-    ref = ctypes.byref(args)
+def _raw_stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object
+
+    def _raw_stream(dev: torch.device) -> int:  # noqa: F811
+        return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _run(call, size, args: bytes, dev: torch.device) -> None:
+    """``call`` on ``dev``'s current stream, with the workspace it asks for."""
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _run(size, call, args, dev)
-    need = size(ref)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _lib.check(call(ref, ws.data_ptr() if need else None, need,
-                    torch.cuda.current_stream(dev).cuda_stream))
+            return _run(call, size, args, dev)
+    stream = _raw_stream(dev)
+    rc = call(args, None, 0, stream)
+    if rc == 3:  # QRB_ERR_WORKSPACE: nothing was enqueued
+        need = size(args)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = call(args, ws.data_ptr(), need, stream)
+    if rc:
+        _lib.check(rc)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -142,41 +148,45 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     """
     _check("x", x)
     _check("weight", weight, x)
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x must be [..., k] and weight [n, k], got {tuple(x.shape)} and "
-                         f"{tuple(weight.shape)}")
-    act = _activation(activation)
-    n, k = weight.shape
-    shape = (*x.shape[:-1], n)
+    xs, ws = x.shape, weight.shape
+    if len(ws) != 2 or not xs or xs[-1] != ws[1]:
+        raise ValueError(f"x must be [..., k] and weight [n, k], got {tuple(xs)} and {tuple(ws)}")
+    act = ACTIVATIONS[activation] if activation in ACTIVATIONS else _activation(activation)
+    n, k = ws
+    shape = (*xs[:-1], n)
     x2, w2 = _rows(x, k), _rows(weight, k)
     m = x2.shape[0]
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    a = _LinearArgs(_DTYPES[x.dtype], act, m, n, k, x2.data_ptr(), x2.stride(0), w2.data_ptr(),
-                    w2.stride(0), None, None, 0, y.data_ptr(), n)
+    bp = rp = ldr = zp = ldz = qp = ep = 0
     if bias is not None:
         _check("bias", bias, x)
-        if tuple(bias.shape) != (n,):
+        if bias.shape != (n,):
             raise ValueError(f"bias must be ({n},), got {tuple(bias.shape)}")
-        bias = bias.contiguous()
-        a.bias = bias.data_ptr()
+        if bias.stride(0) != 1:
+            bias = bias.contiguous()
+        bp = bias.data_ptr()
     if residual is not None:
         _check("residual", residual, x)
-        if tuple(residual.shape) != shape:
+        if residual.shape != shape:
             raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
         residual = _rows(residual, n)
-        a.residual, a.ldr = residual.data_ptr(), residual.stride(0)
+        rp, ldr = residual.data_ptr(), residual.stride(0)
     z = None
-    if keep == "plain":
-        z = torch.empty(shape, dtype=x.dtype, device=x.device)
-        a.z, a.ldz = z.data_ptr(), n
-    elif keep == "packed":
-        z = _empty_packed(shape, x)
-        a.z_codes, a.z_exponents = z.codes.data_ptr(), z.exponents.data_ptr()
-    elif keep is not None:
-        raise ValueError(f"keep must be None, 'plain' or 'packed', got {keep!r}")
+    if keep is not None:
+        if keep == "plain":
+            z = x.new_empty(shape)
+            zp, ldz = z.data_ptr(), n
+        elif keep == "packed":
+            z = _empty_packed(shape, x)
+            qp, ep = z.codes.data_ptr(), z.exponents.data_ptr()
+        else:
+            raise ValueError(f"keep must be None, 'plain' or 'packed', got {keep!r}")
+    y = x.new_empty(shape)
     if m and n:
         L = _lib.lib()
-        _run(L.qrbl_linear_workspace_bytes, L.qrbl_linear, a, x.device)
+        _run(L.qrbl_linear, L.qrbl_linear_workspace_bytes,
+             _linear_args(_DTYPES[x.dtype], act, m, n, k, x2.data_ptr(), x2.stride(0),
+                          w2.data_ptr(), w2.stride(0), bp, rp, ldr, y.data_ptr(), n, zp, ldz, qp,
+                          ep), x.device)
     return y if keep is None else (y, z)
 
 
@@ -196,81 +206,77 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     """
     _check("dy", dy)
     _check("weight", weight, dy)
-    if weight.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != weight.shape[0]:
-        raise ValueError(f"dy must be [..., n] and weight [n, k], got {tuple(dy.shape)} and "
-                         f"{tuple(weight.shape)}")
-    act = _activation(activation)
+    ds, ws = dy.shape, weight.shape
+    if len(ws) != 2 or not ds or ds[-1] != ws[0]:
+        raise ValueError(f"dy must be [..., n] and weight [n, k], got {tuple(ds)} and {tuple(ws)}")
+    act = ACTIVATIONS[activation] if activation in ACTIVATIONS else _activation(activation)
     if isinstance(need, str) or not set(need) <= {"x", "weight", "bias"}:
         raise ValueError(f"need must name some of 'x', 'weight' and 'bias', got {need!r}")
-    n, k = weight.shape
-    lead = tuple(dy.shape[:-1])
+    n, k = ws
+    lead = tuple(ds[:-1])
     dy2, w2 = _rows(dy, n), _rows(weight, k)
     m = dy2.shape[0]
-    a = _BackwardArgs(_DTYPES[dy.dtype], act, m, n, k, dy2.data_ptr(), dy2.stride(0))
-    a.w, a.ldw = w2.data_ptr(), w2.stride(0)
-    held = []  # views and copies the call reads
+    xp = ldx = xq = xe = zp = ldz = zq = ze = dxp = dwp = dbp = 0
+    dx = dw = db = None
     if "weight" in need:
         if isinstance(x, PackedActivation):
             _check_packed("x", x, dy, (*lead, k))
-            codes, exps = x.codes.contiguous(), x.exponents.contiguous()
-            held += [codes, exps]
+            xcodes, xexps = x.codes.contiguous(), x.exponents.contiguous()
             if k:
-                a.x_codes, a.x_exponents = codes.data_ptr(), exps.data_ptr()
+                xq, xe = xcodes.data_ptr(), xexps.data_ptr()
         else:
             if x is None:
                 raise ValueError("x is needed for the weight's gradient")
             _check("x", x, dy)
-            if tuple(x.shape) != (*lead, k):
+            if x.shape != (*lead, k):
                 raise ValueError(f"x must be {(*lead, k)}, got {tuple(x.shape)}")
             x2 = _rows(x, k)
-            held.append(x2)
-            a.x, a.ldx = x2.data_ptr(), x2.stride(0)
+            xp, ldx = x2.data_ptr(), x2.stride(0)
+        dw = dy.new_empty((n, k))
+        dwp = dw.data_ptr()
     if act:
         if isinstance(z, PackedActivation):
             if activation == "relu":
                 raise ValueError("relu's gradient needs z as a tensor: packed, small values lose "
                                  "their sign")
             _check_packed("z", z, dy, (*lead, n))
-            codes, exps = z.codes.contiguous(), z.exponents.contiguous()
-            held += [codes, exps]
-            a.z_codes, a.z_exponents = codes.data_ptr(), exps.data_ptr()
+            zcodes, zexps = z.codes.contiguous(), z.exponents.contiguous()
+            zq, ze = zcodes.data_ptr(), zexps.data_ptr()
         else:
             if z is None:
                 raise ValueError(f"z is needed for the gradient of {activation!r}")
             _check("z", z, dy)
-            if tuple(z.shape) != (*lead, n):
+            if z.shape != (*lead, n):
                 raise ValueError(f"z must be {(*lead, n)}, got {tuple(z.shape)}")
             z2 = _rows(z, n)
-            held.append(z2)
-            a.z, a.ldz = z2.data_ptr(), z2.stride(0)
-    dx = dw = db = None
+            zp, ldz = z2.data_ptr(), z2.stride(0)
     if "x" in need:
-        dx = torch.empty((*lead, k), dtype=dy.dtype, device=dy.device)
-        a.dx, a.lddx = dx.data_ptr(), k
-    if "weight" in need:
-        dw = torch.empty((n, k), dtype=dy.dtype, device=dy.device)
-        a.dw, a.lddw = dw.data_ptr(), k
+        dx = dy.new_empty((*lead, k))
+        dxp = dx.data_ptr()
     if "bias" in need:
-        db = torch.empty((n,), dtype=dy.dtype, device=dy.device)
-        a.dbias = db.data_ptr()
+        db = dy.new_empty((n,))
+        dbp = db.data_ptr()
     L = _lib.lib()
-    _run(L.qrbl_linear_backward_workspace_bytes, L.qrbl_linear_backward, a, dy.device)
+    _run(L.qrbl_linear_backward, L.qrbl_linear_backward_workspace_bytes,
+         _backward_args(_DTYPES[dy.dtype], act, m, n, k, dy2.data_ptr(), dy2.stride(0), xp, ldx,
+                        xq, xe, w2.data_ptr(), w2.stride(0), zp, ldz, zq, ze, dxp, k, dwp, k,
+                        dbp), dy.device)
     return dx, dw, db
 
 
 def _empty_packed(shape: tuple, like: torch.Tensor) -> PackedActivation:
     return PackedActivation(
-        torch.empty(shape, dtype=torch.int8, device=like.device),
-        torch.empty((*shape[:-1], -(-shape[-1] // PACK_BLOCK)), dtype=torch.int8,
-                    device=like.device),
-        like.dtype)
+        like.new_empty(shape, dtype=torch.int8),
+        like.new_empty((*shape[:-1], -(-shape[-1] // PACK_BLOCK)), dtype=torch.int8), like.dtype)
 
 
 def _on(dev: torch.device, call, *args) -> None:
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _on(dev, call, *args)
-    _lib.check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+    rc = call(*args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc)
 
 
 def pack_activation(x: torch.Tensor) -> PackedActivation:

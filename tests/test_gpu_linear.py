@@ -17,7 +17,6 @@ Tolerances, elementwise, from arithmetic (u = half a step of the output type):
 
 from __future__ import annotations
 
-import ctypes
 import itertools
 import math
 import threading
@@ -209,9 +208,9 @@ def test_linear_in_place_residual():
     r = rnd((100, 72), 24, BF)
     want = api.linear(x, w, None, r, "gelu")
     out = r.clone()
-    a = layers._LinearArgs(2, 2, 100, 72, 64, x.data_ptr(), 64, w.data_ptr(), 64, None,
-                           out.data_ptr(), 72, out.data_ptr(), 72)
-    assert _lib.lib().qrbl_linear(ctypes.byref(a), None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    a = layers._linear_args(2, 2, 100, 72, 64, x.data_ptr(), 64, w.data_ptr(), 64, 0,
+                            out.data_ptr(), 72, out.data_ptr(), 72, 0, 0, 0, 0)
+    assert _lib.lib().qrbl_linear(a, None, 0, torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out, want)
 
 
@@ -224,11 +223,11 @@ def test_rows_and_columns_outside_stay_as_they_were(m, n, k, dt):
     want = api.linear(x, w)
     for ldy in (n, n + 8, n + 3):
         y = torch.full((m + 200, ldy), 7.0, device=DEV, dtype=dt)
-        a = layers._LinearArgs(layers._DTYPES[dt], 0, m, n, k, x.data_ptr(), k, w.data_ptr(), k,
-                               None, None, 0, y.data_ptr(), ldy)
-        need = L.qrbl_linear_workspace_bytes(ctypes.byref(a))
+        a = layers._linear_args(layers._DTYPES[dt], 0, m, n, k, x.data_ptr(), k, w.data_ptr(), k,
+                                0, 0, 0, y.data_ptr(), ldy, 0, 0, 0, 0)
+        need = L.qrbl_linear_workspace_bytes(a)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
-        assert L.qrbl_linear(ctypes.byref(a), ws.data_ptr(), need, s) == 0
+        assert L.qrbl_linear(a, ws.data_ptr(), need, s) == 0
         assert torch.equal(y[:m, :n], want)
         assert (y[m:] == 7).all() and (y[:, n:] == 7).all()
 

@@ -3,7 +3,6 @@
 
 from __future__ import annotations
 
-import ctypes
 import re
 import subprocess
 
@@ -32,15 +31,30 @@ def test_entry_points_are_public():
         assert name in pkg.__all__ and getattr(pkg, name) is getattr(api, name)
 
 
-def test_struct_layouts_match_the_header():
+def _fields(struct: str) -> list[tuple[str, str]]:
+    """(name, kind) of a header struct's fields: "i" int32, "q" int64, "P" pointer."""
     text = HEADER.read_text()
-    for struct, cls in (("qrbl_linear_args", layers._LinearArgs),
-                        ("qrbl_linear_backward_args", layers._BackwardArgs)):
-        body = text[:text.index("} " + struct + ";")].rsplit("typedef struct {", 1)[1]
-        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
-        names = [n.strip(" *") for line in body.split(";") if line.strip()
-                 for n in line.strip().split(None, 1 if "const" not in line else 2)[-1].split(",")]
-        assert names == [f[0] for f in cls._fields_]
+    body = text[:text.index("} " + struct + ";")].rsplit("typedef struct {", 1)[1]
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    out = []
+    for decl in body.split(";"):
+        if decl.strip():
+            kind = "P" if "*" in decl else {"int32_t": "i", "int64_t": "q"}[decl.split()[0]]
+            names = decl.replace("const", "").split(None, 1)[1]
+            out += [(n.strip(" *"), kind) for n in names.split(",")]
+    return out
+
+
+def test_struct_layouts_match_the_header():
+    import struct
+
+    for name, fields, pack in (("qrbl_linear_args", layers._LINEAR_FIELDS, layers._linear_args),
+                               ("qrbl_linear_backward_args", layers._BACKWARD_FIELDS,
+                                layers._backward_args)):
+        decl = _fields(name)
+        assert tuple(n for n, _ in decl) == fields
+        values = list(range(1, len(fields) + 1))
+        assert pack(*values) == struct.pack("@" + "".join(k for _, k in decl), *values)
 
 
 def test_cpu_tensors_and_types_are_refused():
@@ -68,41 +82,38 @@ def test_cpu_tensors_and_types_are_refused():
 
 
 def _fwd(**kw):
-    a = layers._LinearArgs(2, 0, 4, 16, 32, P, 32, P, 32, None, None, 0, P, 16, None, 0, None, None)
-    for k, v in kw.items():
-        setattr(a, k, v)
-    return a
+    a = dict(zip(layers._LINEAR_FIELDS,
+                 (2, 0, 4, 16, 32, P, 32, P, 32, 0, 0, 0, P, 16, 0, 0, 0, 0)))
+    return layers._linear_args(*{**a, **kw}.values())
 
 
 def _bwd(**kw):
-    a = layers._BackwardArgs(2, 4, 4, 16, 32, P, 16, P, 32, None, None, P, 32, P, 16, None, None,
-                             P, 32, P, 32, P)
-    for k, v in kw.items():
-        setattr(a, k, v)
-    return a
+    a = dict(zip(layers._BACKWARD_FIELDS,
+                 (2, 4, 4, 16, 32, P, 16, P, 32, 0, 0, P, 32, P, 16, 0, 0, P, 32, P, 32, P)))
+    return layers._backward_args(*{**a, **kw}.values())
 
 
 @pytest.mark.parametrize("bad", [
     {"dtype": 3}, {"dtype": -1}, {"activation": 5}, {"activation": -1}, {"m": -1}, {"n": -1},
-    {"k": -1}, {"x": None}, {"w": None}, {"y": None}, {"ldx": 31}, {"ldw": 31}, {"ldy": 15},
+    {"k": -1}, {"x": 0}, {"w": 0}, {"y": 0}, {"ldx": 31}, {"ldw": 31}, {"ldy": 15},
     {"residual": P, "ldr": 15}, {"z": P, "ldz": 15}, {"z_codes": P}, {"z_exponents": P},
     {"x": P + 1}, {"w": P + 1}, {"y": P + 1}, {"bias": P + 1}, {"dtype": 0, "x": P + 2},
     {"ldx": -1, "m": 1}])
 def test_forward_validation(bad):
     a = _fwd(**bad)
-    assert _lib.lib().qrbl_linear(ctypes.byref(a), None, 0, None) == 1
-    assert _lib.lib().qrbl_linear_workspace_bytes(ctypes.byref(a)) == 0
+    assert _lib.lib().qrbl_linear(a, None, 0, None) == 1
+    assert _lib.lib().qrbl_linear_workspace_bytes(a) == 0
 
 
 @pytest.mark.parametrize("bad", [
-    {"dtype": 7}, {"activation": 9}, {"m": -1}, {"dy": None}, {"x": None}, {"w": None}, {"z": None},
+    {"dtype": 7}, {"activation": 9}, {"m": -1}, {"dy": 0}, {"x": 0}, {"w": 0}, {"z": 0},
     {"lddy": 15}, {"ldx": 31}, {"ldw": 31}, {"ldz": 15}, {"lddx": 31}, {"lddw": 31},
     {"x_codes": P}, {"z_codes": P}, {"x_codes": P, "x_exponents": P},
     {"z_codes": P, "z_exponents": P}, {"dbias": P + 1}, {"dx": P + 1}, {"dw": P + 1},
-    {"z": None, "z_codes": P, "z_exponents": P, "activation": 1}])
+    {"z": 0, "z_codes": P, "z_exponents": P, "activation": 1}])
 def test_backward_validation(bad):
     a = _bwd(**bad)
-    assert _lib.lib().qrbl_linear_backward(ctypes.byref(a), None, 0, None) == 1
+    assert _lib.lib().qrbl_linear_backward(a, None, 0, None) == 1
 
 
 def test_sizes_workspaces_and_empty_calls():
@@ -110,29 +121,29 @@ def test_sizes_workspaces_and_empty_calls():
     assert L.qrbl_linear(None, None, 0, None) == 1
     assert L.qrbl_linear_backward(None, None, 0, None) == 1
     # no rows or no columns: nothing to do, and nothing is touched
-    assert L.qrbl_linear(ctypes.byref(_fwd(m=0, x=None, y=None)), None, 0, None) == 0
-    assert L.qrbl_linear(ctypes.byref(_fwd(n=0, w=None, y=None)), None, 0, None) == 0
-    none = {"dx": None, "dw": None, "dbias": None}
-    assert L.qrbl_linear_backward(ctypes.byref(_bwd(dy=None, **none)), None, 0, None) == 0
+    assert L.qrbl_linear(_fwd(m=0, x=0, y=0), None, 0, None) == 0
+    assert L.qrbl_linear(_fwd(n=0, w=0, y=0), None, 0, None) == 0
+    none = {"dx": 0, "dw": 0, "dbias": 0}
+    assert L.qrbl_linear_backward(_bwd(dy=0, **none), None, 0, None) == 0
     assert L.qrbl_pack(2, None, 0, 0, 64, None, None, None) == 0
     assert L.qrbl_unpack(2, None, None, 5, 0, None, 0, None) == 0
     # beyond 32-bit coordinates
     big = (1 << 30) + 1
-    assert L.qrbl_linear(ctypes.byref(_fwd(k=big, ldx=big, ldw=big)), None, 0, None) == 2
-    assert L.qrbl_linear_backward(ctypes.byref(_bwd(m=big)), None, 0, None) == 2
+    assert L.qrbl_linear(_fwd(k=big, ldx=big, ldw=big), None, 0, None) == 2
+    assert L.qrbl_linear_backward(_bwd(m=big), None, 0, None) == 2
     # an operand that is not 16-byte aligned, or FP32, is staged: a workspace is required
-    for a in (_fwd(x=P + 2), _fwd(ldx=33), _fwd(dtype=0)):
-        need = L.qrbl_linear_workspace_bytes(ctypes.byref(a))
+    for a in (_fwd(m=64, x=P + 2), _fwd(m=64, ldx=33), _fwd(m=64, dtype=0)):
+        need = L.qrbl_linear_workspace_bytes(a)
         assert need > 0
-        assert L.qrbl_linear(ctypes.byref(a), None, need, None) == 3
-        assert L.qrbl_linear(ctypes.byref(a), P, need - 1, None) == 3
-        assert L.qrbl_linear(ctypes.byref(a), P + 4, need, None) == 1
+        assert L.qrbl_linear(a, None, need, None) == 3
+        assert L.qrbl_linear(a, P, need - 1, None) == 3
+        assert L.qrbl_linear(a, P + 4, need, None) == 1
     b = _bwd()
-    need = L.qrbl_linear_backward_workspace_bytes(ctypes.byref(b))
+    need = L.qrbl_linear_backward_workspace_bytes(b)
     assert need > 0
-    assert L.qrbl_linear_backward(ctypes.byref(b), None, need, None) == 3
-    assert L.qrbl_linear_backward(ctypes.byref(b), P, need - 1, None) == 3
-    assert L.qrbl_linear_backward(ctypes.byref(b), P + 8, need, None) == 1
+    assert L.qrbl_linear_backward(b, None, need, None) == 3
+    assert L.qrbl_linear_backward(b, P, need - 1, None) == 3
+    assert L.qrbl_linear_backward(b, P + 8, need, None) == 1
 
 
 @pytest.mark.parametrize("args", [
@@ -149,7 +160,7 @@ def test_injected_failure_enqueues_nothing():
     _lib.set_config("fail_next", 1)
     assert _lib.lib().qrbl_pack(2, P, 64, 2, 64, P, P, None) == 6
     _lib.set_config("fail_next", 1)
-    assert _lib.lib().qrbl_linear(ctypes.byref(_fwd()), None, 0, None) == 6
+    assert _lib.lib().qrbl_linear(_fwd(), None, 0, None) == 6
     _lib.set_config("fail_next", 1)
-    assert _lib.lib().qrbl_linear_backward(ctypes.byref(_bwd()), None, 0, None) == 6
+    assert _lib.lib().qrbl_linear_backward(_bwd(), None, 0, None) == 6
     assert _lib.get_config("fail_next") == 0
