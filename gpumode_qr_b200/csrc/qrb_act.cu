@@ -151,39 +151,36 @@ __device__ __forceinline__ void stage_block(const StageJob& j, int64_t block) {
   const int64_t by = block / j.nx, bx = block - by * j.nx;
   const int ty = kThreads / j.tx, x0 = threadIdx.x & (j.tx - 1), y0 = threadIdx.x / j.tx;
   const int64_t c = (bx * j.tx + x0) * V;
-  const int64_t r0 = by * ty * ROWS + y0;
-  const int valid = clip(a.cols - c, V);
-  if (!j.vin) {  // rows not 16-byte aligned: neighbouring threads, neighbouring values
+  if (!j.vin) {  // rows not 16-byte aligned: one row, neighbouring threads at neighbouring values
     const int64_t c0 = bx * j.tx * V + x0;
-#pragma unroll 1
-    for (int i = 0; i < ROWS; ++i) {
-      const int64_t r = r0 + (int64_t)i * ty;
-      if (r >= a.rows) return;
-      float v[V];
+    const int64_t r = by * ty + y0;
+    if (r >= a.rows) return;
+    float v[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int64_t cc = c0 + (int64_t)k * j.tx;
-        if (cc >= a.cols)
-          v[k] = 0.f;
-        else if constexpr (PACKED)
-          v[k] = value_of(a.codes[r * a.cols + cc], pow2f(a.exps[r * j.nblk + cc / kBlk]));
-        else
-          v[k] = to_f<T>(reinterpret_cast<const T*>(a.src)[r * a.lds + cc]);
-      }
+    for (int k = 0; k < V; ++k) {
+      const int64_t cc = c0 + (int64_t)k * j.tx;
+      if (cc >= a.cols)
+        v[k] = 0.f;
+      else if constexpr (PACKED)
+        v[k] = value_of(a.codes[r * a.cols + cc], pow2f(a.exps[r * j.nblk + cc / kBlk]));
+      else
+        v[k] = to_f<T>(reinterpret_cast<const T*>(a.src)[r * a.lds + cc]);
+    }
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int64_t cc = c0 + (int64_t)k * j.tx;
-        if (cc >= a.cols) continue;
-        if constexpr (PLANES) {
-          bf16* d = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + cc;
-          split3(v[k], d[0], d[a.plane], d[2 * a.plane]);
-        } else {
-          reinterpret_cast<T*>(a.dst)[r * a.ldd + cc] = from_f<T>(v[k]);
-        }
+    for (int k = 0; k < V; ++k) {
+      const int64_t cc = c0 + (int64_t)k * j.tx;
+      if (cc >= a.cols) continue;
+      if constexpr (PLANES) {
+        bf16* d = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + cc;
+        split3(v[k], d[0], d[a.plane], d[2 * a.plane]);
+      } else {
+        reinterpret_cast<T*>(a.dst)[r * a.ldd + cc] = from_f<T>(v[k]);
       }
     }
     return;
   }
+  const int64_t r0 = by * ty * ROWS + y0;
+  const int valid = clip(a.cols - c, V);
   if (valid == 0) return;
   Raw8<T> raw[ROWS][2];
   uint4 q[ROWS];
@@ -511,13 +508,13 @@ int pack_t(const void* x, int64_t ld, int64_t rows, int64_t cols, int8_t* codes,
 StageJob stage_job(int elem, const StageArgs& a) {
   StageJob j;
   j.a = a;
-  const Cover g = cover(a.rows, a.cols, kStageVals, stage_rows(elem));
+  j.vin = a.codes != nullptr ? rows_aligned(a.codes, a.cols, 1, 16)
+                             : rows_aligned(a.src, a.lds, elem, 16);
+  const Cover g = cover(a.rows, a.cols, kStageVals, j.vin ? stage_rows(elem) : 1);
   j.tx = g.tx;
   j.nx = g.nx;
   j.blocks = g.blocks;
   j.nblk = blocks_of(a.cols);
-  j.vin = a.codes != nullptr ? rows_aligned(a.codes, a.cols, 1, 16)
-                             : rows_aligned(a.src, a.lds, elem, 16);
   j.vout = rows_aligned(a.dst, a.ldd, elem, 32) ? 2 : rows_aligned(a.dst, a.ldd, elem, 16);
   return j;
 }
@@ -603,9 +600,11 @@ int launch_prepare(int dtype, const Prepare& p, cudaStream_t s) {
 }
 
 // 128 rows where that leaves four blocks or more per SM (fewer partial sums to
-// write and add), else 32.
+// write and add), 32 where that leaves one, else 8: a row per warp.
 int colsum_rows(int64_t m, int64_t n) {
-  return ((m + 127) / 128) * ((n + 255) / 256) >= 592 ? 128 : 32;
+  const int64_t across = (n + 255) / 256;
+  if ((m + 127) / 128 * across >= 592) return 128;
+  return (m + 31) / 32 * across >= 148 ? 32 : 8;
 }
 
 int launch_colsum(int dtype, const ColSum& c, cudaStream_t s) {

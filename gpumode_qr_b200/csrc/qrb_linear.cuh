@@ -123,29 +123,6 @@ __device__ __forceinline__ void values8(const Raw8<T>& r, float (&v)[8]) {
   }
 }
 
-// 32 consecutive elements, 16-byte aligned, as they are in memory.
-template <typename T>
-struct Raw32 {
-  Raw8<T> r[4];
-};
-template <typename T>
-__device__ __forceinline__ Raw32<T> load_raw32(const T* p) {
-  Raw32<T> out;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out.r[i] = load_raw8<T>(p + 8 * i, true, 8);
-  return out;
-}
-template <typename T>
-__device__ __forceinline__ void add_raw32(float (&v)[32], const Raw32<T>& r) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float f[8];
-    values8<T>(r.r[i], f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[8 * i + j] += f[j];
-  }
-}
-
 template <typename T, int N>
 __device__ __forceinline__ void store_n(T* p, bool vec, int valid, const float (&in)[N]) {
   if (vec && valid >= N) {

@@ -46,33 +46,46 @@ namespace lin {
 namespace {
 
 constexpr int BM = 128;       // rows per CTA
-constexpr int BK = 64;        // reduction values per stage: 128 bytes
-constexpr int kChain = 4;     // FP32: stages per accumulator chain
+constexpr int kChainValues = 256;  // FP32: reduction values per accumulator chain
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kSmemMost = 232448;  // 227 KB
-constexpr int kPitch = 33;              // words of a row in a warp's turning buffer
-constexpr uint32_t ATOM = 64 * 128;     // MN-major box: 64 reduction rows of 128 bytes
+constexpr int kPitch = 33;              // words of a row in a warp's turned block
 
 // control block at the start of shared memory
 constexpr int B_FULL = 0, B_EMPTY = kMaxStages, B_ACCFULL = 2 * kMaxStages,
-              B_ACCEMPTY = B_ACCFULL + 2, B_FIN = B_ACCEMPTY + 2, NBAR = B_FIN + 1;
+              B_ACCEMPTY = B_ACCFULL + 2, B_FIN = B_ACCEMPTY + 2, B_RES = B_FIN + 1,
+              NBAR = B_RES + 2 * kEpiWarps;
 constexpr uint32_t OFF_TMEM = NBAR * 8, OFF_ABORT = OFF_TMEM + 4, CTRL = 1024;
 static_assert(OFF_ABORT + 4 <= CTRL, "control block");
 
 template <int CG, int BN, typename T>
 struct Lay {
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // planes
+  static constexpr int BK = NP == 3 ? 32 : 64;       // reduction values per stage
+  static constexpr uint32_t KROW = BK * 2;           // bytes of a K-major row
+  static constexpr uint32_t ATOM = BK * 128;         // MN-major box: BK rows of 128 bytes
+  static constexpr int CHAIN = kChainValues / BK;    // FP32: stages per accumulator chain
   static constexpr int BROWS = BN / CG;              // B's columns of one CTA
-  static constexpr uint32_t A = BM * 128, B = BROWS * 128;
+  static constexpr uint32_t A = BM * KROW, B = BROWS * KROW;
   static constexpr uint32_t STAGE = NP * (A + B);
-  // rows that a warp turns at a time (FP32: few, which leaves room for a stage)
-  static constexpr int TROWS = NP == 3 ? 8 : 32;
-  static constexpr uint32_t TURN = kEpiWarps * TROWS * kPitch * 4;
+  // The epilogue's staging: each warp has HALVES buffers of 32 rows of up to 128
+  // bytes, from which TMA stores the results (and into which it loads the
+  // residual); unaligned matrices use the same memory to turn blocks, TROWS rows
+  // at a time.
+  static constexpr int HC = BN / 2;                  // columns of one epilogue warp
+  static constexpr int HALVES = NP == 3 ? 1 : 2;
+  static constexpr uint32_t WBUF = HALVES * 4096;
+  static constexpr int TROWS = NP == 3 ? 16 : 32;
+  static constexpr uint32_t ROWB = HC * sizeof(T) < 128 ? HC * sizeof(T) : 128;
+  static constexpr int GW = ROWB / sizeof(T);        // columns of one staged block
+  static constexpr uint32_t TURN = kEpiWarps * WBUF;
   static constexpr int FIT = (int)((kSmemMost - CTRL - 1024 - TURN) / STAGE);
   static constexpr int ST = FIT < kMaxStages ? FIT : kMaxStages;
   static constexpr uint32_t SMEM = 1024 + CTRL + ST * STAGE + TURN;  // 1024: base alignment
+  static_assert(TROWS * kPitch * 4 <= (int)WBUF && (ROWB == 64 || ROWB == 128), "staging");
+  static_assert(A % 1024 == 0 && B % 1024 == 0, "swizzle atoms");
   static constexpr int ACC = NP == 3 ? 2 * BN : BN;  // TMEM columns per buffer
   static constexpr int TMEM = 2 * ACC;
   static_assert(ST >= 2 && TMEM <= 512 && TMEM >= 32, "stage ring and TMEM");
@@ -149,16 +162,20 @@ __device__ __forceinline__ Item item_of(const Args& a, int worker, int step) {
   return it;
 }
 
-constexpr uint64_t kSw128 = 2;
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+constexpr uint64_t kSw128 = 2, kSw64 = 4;
+__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo, uint32_t sbo,
+                                         uint64_t layout) {
   return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) | (1ull << 46) | (kSw128 << 61);
+         ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) | (1ull << 46) | (layout << 61);
 }
-// K-major: rows of 128 bytes, 8-row groups 1024 bytes apart; 16 reduction
-// values are 32 bytes. MN-major: 64-value atoms ATOM apart, 8-row (reduction)
-// groups 1024 bytes apart; 16 reduction rows are 2048 bytes.
+// K-major: rows of KROW bytes (128 or 64, swizzled over that width), 8-row
+// groups 8 KROW apart; 16 reduction values are 32 bytes. MN-major: 64-value
+// atoms (128-byte rows) ATOM apart, 8-row (reduction) groups 1024 bytes apart;
+// 16 reduction rows are 2048 bytes.
+template <typename L>
 __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, bool mn) {
-  return desc(saddr, mn ? ATOM : 16, 1024);
+  return mn ? desc(saddr, L::ATOM, 1024, kSw128)
+            : desc(saddr, 16, 8 * L::KROW, L::KROW == 128 ? kSw128 : kSw64);
 }
 
 template <int CG>
@@ -280,16 +297,97 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, u
         : "memory");
 }
 // One operand's tile of one stage.
-template <int CG, int ROWS>
+template <int CG, typename L, int ROWS>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, bool mn,
                                           uint32_t bar, int mn0, int kb, int plane) {
   if (mn) {
 #pragma unroll
     for (int j = 0; j < ROWS / 64; ++j)
-      load_box<CG>(dst + j * ATOM, map, bar, mn0 + 64 * j, kb * BK, plane);
+      load_box<CG>(dst + j * L::ATOM, map, bar, mn0 + 64 * j, kb * L::BK, plane);
   } else {
-    load_box<CG>(dst, map, bar, kb * BK, mn0, plane);
+    load_box<CG>(dst, map, bar, kb * L::BK, mn0, plane);
   }
+}
+
+// Staged blocks: 32 rows (lane = row) of ROWB bytes with TMA's 128- or 64-byte
+// swizzle, which also spreads a warp's 16-byte accesses over the banks.
+template <uint32_t ROWB>
+__device__ __forceinline__ uint32_t staged_at(uint32_t buf, int row, int unit) {
+  const int x = ROWB == 128 ? unit ^ (row & 7) : unit ^ ((row >> 1) & 3);
+  return buf + row * ROWB + x * 16;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+  if constexpr (__is_same(T, bf16)) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+// 32 values of the lane's row from column `first` of the block.
+template <typename E, uint32_t ROWB>
+__device__ __forceinline__ void stage_write(uint32_t buf, int first, const float (&v)[32]) {
+  const int row = threadIdx.x & 31;
+  constexpr int PER = 16 / sizeof(E);  // values of 16 bytes
+#pragma unroll
+  for (int j = 0; j < 32 / PER; ++j) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(E) == 4)
+        w[k] = __float_as_uint(v[PER * j + k]);
+      else
+        w[k] = pair_of<E>(v[PER * j + 2 * k], v[PER * j + 2 * k + 1]);
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
+                     staged_at<ROWB>(buf, row, first / PER + j)),
+                 "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                 : "memory");
+  }
+}
+template <typename T, uint32_t ROWB>
+__device__ __forceinline__ void stage_add(uint32_t buf, int first, float (&v)[32]) {
+  const int row = threadIdx.x & 31;
+  constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < 32 / PER; ++j) {
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(staged_at<ROWB>(buf, row, first / PER + j))
+                 : "memory");
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        v[PER * j + k] += __uint_as_float(w[k]);
+      } else {
+        float lo, hi;
+        values2<T>(w[k], lo, hi);
+        v[PER * j + 2 * k] += lo;
+        v[PER * j + 2 * k + 1] += hi;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::
+                   "l"(reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void load_box2(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                          int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+// At most one of this thread's stores still reads shared memory.
+__device__ __forceinline__ void bulk_wait_read_one() {
+  asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
 }
 
 // A warp's block of 32 columns of up to eight rows, packed (lane = column).
@@ -338,8 +436,18 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
   if constexpr (FWD) {
     if (e.bias != nullptr && live) bias = to_f<T>(reinterpret_cast<const T*>(e.bias)[col + lane]);
   }
-#pragma unroll 1
-  for (int base = 0; base < rows; base += TROWS) {
+  // all rows' residuals in flight together
+  T res[32];
+  if constexpr (FWD) {
+    if (e.residual != nullptr) {
+      const T* s = reinterpret_cast<const T*>(e.residual) + (int64_t)row0 * e.ldr + col + lane;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) res[k] = live && k < rows ? s[k * e.ldr] : from_f<T>(0.f);
+    }
+  }
+#pragma unroll
+  for (int base = 0; base < 32; base += TROWS) {
+    if (base >= rows) break;
     __syncwarp();
     if (lane >= base && lane < base + TROWS) {
 #pragma unroll
@@ -347,8 +455,9 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
     }
     __syncwarp();
     const int most = rows - base < TROWS ? rows - base : TROWS;
-#pragma unroll 1
-    for (int r0 = 0; r0 < most; r0 += 8) {
+#pragma unroll
+    for (int r0 = 0; r0 < TROWS; r0 += 8) {
+      if (r0 >= most) break;
       const int64_t row0g = row0 + base + r0;
       const int left = most - r0;
       // eight rows' values and residuals together, then eight rows' results
@@ -360,10 +469,8 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
       }
       if constexpr (FWD) {
         if (e.residual != nullptr) {
-          const T* s = reinterpret_cast<const T*>(e.residual) + row0g * e.ldr + col + lane;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (live && k < left) q[k] = to_f<T>(s[k * e.ldr]);
+          for (int k = 0; k < 8; ++k) q[k] = to_f<T>(res[base + r0 + k]);
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) p[k] += bias;
@@ -388,56 +495,44 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
   }
 }
 
-// The same for a whole block of 16-byte aligned rows, as lane = row: each lane's
-// 32 columns are whole sectors. 16-bit types: the bias and residual were loaded
-// before the accumulators were ready.
-template <typename T, bool FWD>
-__device__ __forceinline__ void finish32(float (&v)[32], int row, int col, const Problem& a,
-                                         const Raw32<T>& bias, const Raw32<T>& res) {
+// The packed form of 32 columns of one row (lane = row).
+template <typename T>
+__device__ __forceinline__ void pack32(const float (&v)[32], int row, int col, const Problem& a) {
+  constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
   const Epilogue& e = a.e;
-  if constexpr (FWD) {
-    if (e.bias != nullptr) add_raw32<T>(v, bias);
-    Raw32<T> late;  // (FP32: no registers to hold it earlier)
-    if constexpr (sizeof(T) == 4) {
-      if (e.residual != nullptr)
-        late = load_raw32<T>(reinterpret_cast<const T*>(e.residual) + (int64_t)row * e.ldr + col);
-    }
-    if (e.z != nullptr)
-      store_n<T, 32>(reinterpret_cast<T*>(e.z) + (int64_t)row * e.ldz + col, true, 32, v);
-    if (e.z_codes != nullptr) {
-      constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
-      float amax = 0.f;
+  float amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) amax = max_abs_nan(amax, v[i]);
-      const bool fine = finite_f(amax);
-      if (!fine) amax = finite_amax(v);
-      const int ex = block_exponent(amax, lo, hi);
-      uint32_t w[8];
-      encode(v, ex, fine && ex < hi, ex == hi ? 63.f : 127.f, w);
-      uint4* out = reinterpret_cast<uint4*>(e.z_codes + (int64_t)row * a.n + col);
-      out[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      out[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      e.z_exps[(int64_t)row * ((a.n + kBlk - 1) / kBlk) + col / kBlk] = (int8_t)ex;
-    }
-    act_by(v, e.act);
-    if (e.residual != nullptr) add_raw32<T>(v, sizeof(T) == 4 ? late : res);
-  }
-  store_n<T, 32>(reinterpret_cast<T*>(e.out) + (int64_t)row * e.ldo + col, true, 32, v);
+  for (int i = 0; i < 32; ++i) amax = max_abs_nan(amax, v[i]);
+  const bool fine = finite_f(amax);
+  if (!fine) amax = finite_amax(v);
+  const int ex = block_exponent(amax, lo, hi);
+  uint32_t w[8];
+  encode(v, ex, fine && ex < hi, ex == hi ? 63.f : 127.f, w);
+  if (row >= a.m || col >= a.n) return;
+  int8_t* out = e.z_codes + (int64_t)row * a.n + col;  // n % 16 == 0, 16-byte aligned
+  reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (col + 16 < a.n) reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  e.z_exps[(int64_t)row * ((a.n + kBlk - 1) / kBlk) + col / kBlk] = (int8_t)ex;
 }
 
-// A split product's partial tile (rows and columns padded to whole tiles).
-__device__ __forceinline__ void partial32(const float (&v)[32], int row, int col, int split,
-                                          const Problem& a) {
-  float* p = a.part + ((long long)split * a.part_rows + row) * a.part_ld + col;
+// 32 values at p (of them `valid` within the row), 16-byte aligned, added.
+template <typename T>
+__device__ __forceinline__ void add_bias(float (&v)[32], const T* p, int valid) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 4)
-    *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  for (int j = 0; j < 4; ++j) {
+    float f[8];
+    values8<T>(load_raw8<T>(p + 8 * j, true, valid - 8 * j), f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 * j + i] += f[i];
+  }
 }
 
 template <int CG, int BN, typename T, bool FWD>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
               const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
+              const __grid_constant__ CUtensorMap map_o0, const __grid_constant__ CUtensorMap map_o1,
+              const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_z,
               const __grid_constant__ Args a) {
   using L = Lay<CG, BN, T>;
   extern __shared__ uint8_t smem_raw[];
@@ -472,6 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma::mbar_init(BAR(B_ACCEMPTY + b), CG * kEpiWarps);
     }
     tma::mbar_init(BAR(B_FIN), 1);
+    for (int i = 0; i < 2 * kEpiWarps; ++i) tma::mbar_init(BAR(B_RES + i), 1);
     tma::mbar_fence_init();
     *s_abort = 0;
   }
@@ -503,10 +599,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rank == 0) tma::mbar_expect_tx(BAR(B_FULL + s), CG * L::STAGE);
 #pragma unroll
           for (int p = 0; p < L::NP; ++p)
-            load_tile<CG, BM>(st + p * L::A, ma, amn, bar, am, kb, p);
+            load_tile<CG, L, BM>(st + p * L::A, ma, amn, bar, am, kb, p);
 #pragma unroll
           for (int p = 0; p < L::NP; ++p)
-            load_tile<CG, L::BROWS>(st + L::NP * L::A + p * L::B, mb, bmn, bar, bn, kb, p);
+            load_tile<CG, L, L::BROWS>(st + L::NP * L::A + p * L::B, mb, bmn, bar, bn, kb, p);
         }
         __syncwarp();
         ++u;
@@ -535,10 +631,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             ((bmn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
                             ((uint32_t)((BM * CG) >> 4) << 24);
         const uint64_t ka = amn ? 2048 >> 4 : 32 >> 4, kbs = bmn ? 2048 >> 4 : 32 >> 4;
-        const uint64_t da0 = operand_desc(ring, amn);
-        const uint64_t db0 = operand_desc(ring + L::NP * L::A, bmn);
+        const uint64_t da0 = operand_desc<L>(ring, amn);
+        const uint64_t db0 = operand_desc<L>(ring + L::NP * L::A, bmn);
         for (int kb = it.kb0; live && kb < it.kb1;) {
-          const int end = L::NP == 3 && kb + kChain < it.kb1 ? kb + kChain : it.kb1;
+          const int end = L::NP == 3 && kb + L::CHAIN < it.kb1 ? kb + L::CHAIN : it.kb1;
           const int buf = unit & 1;
           if (unit >= 2)
             live = warp_wait(BAR(B_ACCEMPTY + buf), (uint32_t)((unit / 2 - 1) & 1), a.limit,
@@ -561,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint64_t db = db0 + at + (uint64_t)(pj[q] * (L::B >> 4));
                 const uint32_t dq = q == 0 ? d : d + BN;
 #pragma unroll
-                for (int k = 0; k < BK / 16; ++k)
+                for (int k = 0; k < L::BK / 16; ++k)
                   mma_f16<CG>(dq, da + k * ka, db + k * kbs, id,
                               more | (q > 1 || k > 0 ? 1u : 0u));
               }
@@ -588,10 +684,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {  // ---- epilogue ----
     const int quad = warp & 3, half = warp >> 2;
-    constexpr int HC = BN / 2;  // columns of this warp
+    constexpr int HC = L::HC;  // columns of this warp
+    constexpr int NH = L::HALVES;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    float* turn = reinterpret_cast<float*>(sm + CTRL + L::ST * L::STAGE) + warp * L::TROWS * kPitch;
+    const uint32_t stg = ring + L::ST * L::STAGE + warp * L::WBUF;
+    float* turn = reinterpret_cast<float*>(sm + (stg - base));
     int unit = 0;
+    uint32_t uses0 = 0, uses1 = 0;  // residual loads issued into each half
+    bool live = true;
     auto hand_back = [&](int buf) {  // the accumulators are read
       tc::fence_before();
       __syncwarp();
@@ -609,36 +709,121 @@ __global__ void __launch_bounds__(kThreads, 1)
         column_sum<T>(a.sum, (int64_t)blockIdx.x * (kEpiWarps * 32) + threadIdx.x,
                       (int64_t)gridDim.x * (kEpiWarps * 32));
     }
-    for (int step = 0;; ++step) {
+    for (int step = 0; live; ++step) {
       const Item it = item_of<CG, BN>(a, worker, step);
       if (it.prob < 0) break;
       const Problem& p = a.p[FWD ? 0 : it.prob];
+      const Epilogue& e = p.e;
+      const CUtensorMap* map_o = it.prob == 0 ? &map_o0 : &map_o1;
       const int row0 = it.m0 + rank * BM + quad * 32, col = it.n0 + half * HC;
-      bool ok = true;
-      if constexpr (L::NP == 1) {
-        // the bias and residual of a block are loaded while the accumulators
-        // (first block) or the block before are worked on
-        Raw32<T> bias, res;
-        const Epilogue& e = p.e;
-        const int row = row0 + lane;
-        // whole aligned blocks; all lanes agree except on rows beyond m
-        auto whole = [&](int c) { return e.vec != 0 && c + 32 <= p.n; };
-        auto ahead = [&](int c) { return FWD && p.splits == 1 && whole(c) && row < p.m; };
-        auto load_bias = [&](int c) {
-          if (e.bias != nullptr) bias = load_raw32<T>(reinterpret_cast<const T*>(e.bias) + c);
-        };
-        auto load_res = [&](int c) {
-          if (e.residual != nullptr)
-            res = load_raw32<T>(reinterpret_cast<const T*>(e.residual) +
-                                (int64_t)row * e.ldr + c);
-        };
-        if (ahead(col)) {
-          load_bias(col);
-          load_res(col);
+      const bool part = p.splits > 1, inside = row0 < p.m;
+      const bool staged = part || e.vec != 0;
+      const bool keep_z = FWD && !part && staged && e.z != nullptr;
+      const bool has_res = FWD && !part && staged && e.residual != nullptr;
+      // the staging is free: the last tile's stores have read it
+      if (lane == 0) tma::bulk_wait_read_all();
+      tma::fence_proxy_async();
+      __syncwarp();
+      // residual of block g into its half (z kept: the second; else alternating)
+      auto half_of = [&](int g) { return NH == 1 ? 0 : (keep_z ? 1 : (g & 1)); };
+      auto load_res = [&](int g) {
+        const int h = half_of(g), c = col + g * L::GW;
+        if (lane == 0) {
+          const uint32_t bar = BAR(B_RES + 2 * warp + h);
+          tma::mbar_expect_tx(bar, 32 * L::ROWB);
+          load_box2(stg + h * 4096, &map_r, bar, c, row0);
         }
+        uses0 += h == 0 ? 1u : 0u;
+        uses1 += h == 0 ? 0u : 1u;
+      };
+      const bool early = has_res && inside && !(NH == 1 && keep_z);
+      if (early && col < p.n) load_res(0);
+      if (early && !keep_z && NH == 2 && HC > L::GW && col + L::GW < p.n) load_res(1);
+
+      // One block of 32 columns, c from the warp's first: v holds the sums.
+      auto finish = [&](float(&v)[32], int c) {
+        const int at = col + c;
+        if (part) {  // (rows and columns padded to whole tiles)
+          const int g = c / 32;
+          if (g >= NH) {
+            if (lane == 0) {
+              if constexpr (NH == 2)
+                bulk_wait_read_one();
+              else
+                tma::bulk_wait_read_all();
+            }
+            __syncwarp();
+          }
+          const uint32_t buf = stg + (g % NH) * 4096;
+          stage_write<float, 128>(buf, 0, v);
+          tma::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            store_box(map_o, buf, at, (int)(it.split * p.part_rows) + row0);
+            tma::bulk_commit();
+          }
+          return;
+        }
+        if (at >= p.n || !inside) return;
+        if (!staged) {
+          finish_turned<T, FWD, L::TROWS>(v, row0, at, p, turn);
+          return;
+        }
+        const int g = c / L::GW, in = c % L::GW;
+        const int h = half_of(g);
+        const bool last = in + 32 == L::GW;
+        if (in == 0 && g > 0 && (g >= NH || keep_z)) {  // this block's staging is free
+          if (lane == 0) {
+            if (NH == 2 && !keep_z)
+              bulk_wait_read_one();
+            else
+              tma::bulk_wait_read_all();
+          }
+          __syncwarp();
+          if (has_res && !(NH == 1 && keep_z)) load_res(g);
+        }
+        if constexpr (FWD) {
+          const int valid = p.n - at < 32 ? p.n - at : 32;
+          if (e.bias != nullptr) add_bias<T>(v, reinterpret_cast<const T*>(e.bias) + at, valid);
+          if (keep_z) {
+            stage_write<T, L::ROWB>(stg, in, v);
+            if (last || at + 32 >= p.n) {
+              tma::fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                store_box(&map_z, stg, at - in, row0);
+                tma::bulk_commit();
+                if constexpr (NH == 1) tma::bulk_wait_read_all();
+              }
+              __syncwarp();
+              if (NH == 1 && has_res) load_res(g);
+            }
+          }
+          if (e.z_codes != nullptr) pack32<T>(v, row0 + lane, at, p);
+          act_by(v, e.act);
+          if (has_res) {
+            if (in == 0) {
+              const uint32_t uses = h == 0 ? uses0 : uses1;
+              live = warp_wait(BAR(B_RES + 2 * warp + h), (uses - 1) & 1, a.limit, s_abort);
+            }
+            stage_add<T, L::ROWB>(stg + h * 4096, in, v);
+          }
+        }
+        stage_write<T, L::ROWB>(stg + h * 4096, in, v);
+        if (last || at + 32 >= p.n) {
+          tma::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            store_box(map_o, stg + h * 4096, at - in, row0);
+            tma::bulk_commit();
+          }
+        }
+      };
+
+      if constexpr (L::NP == 1) {
         const int buf = unit & 1;
-        ok = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
-        if (!ok) break;
+        live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
+        if (!live) break;
         tc::fence_after();
         const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
 #pragma unroll 1
@@ -646,17 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float v[32];
           tc::tmem_ld32(t + c, v);
           if (c + 32 == HC) hand_back(buf);
-          if (p.splits > 1) {
-            partial32(v, row, col + c, it.split, p);
-          } else if (whole(col + c)) {
-            if (row < p.m) finish32<T, FWD>(v, row, col + c, p, bias, res);
-          } else {
-            finish_turned<T, FWD, L::TROWS>(v, row0, col + c, p, turn);
-          }
-          if (c + 32 < HC && ahead(col + c + 32)) {
-            load_bias(col + c + 32);
-            load_res(col + c + 32);
-          }
+          finish(v, c);
         }
         ++unit;
       } else {
@@ -665,10 +840,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < HC / 32; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
-        for (int kb = it.kb0; kb < it.kb1; kb += kChain, ++unit) {
+        for (int kb = it.kb0; kb < it.kb1; kb += L::CHAIN, ++unit) {
           const int buf = unit & 1;
-          ok = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
-          if (!ok) break;
+          live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
+          if (!live) break;
           tc::fence_after();
           const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
 #pragma unroll
@@ -681,27 +856,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           hand_back(buf);
         }
-        if (!ok) break;
+        if (!live) break;
 #pragma unroll 1
         for (int c = 0; c < HC / 32; ++c) {
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = HC == 32 || c == 0 ? sum[0][i] : sum[HC / 32 - 1][i];
-          const int at = col + c * 32;
-          if (p.splits > 1) {
-            partial32(v, row0 + lane, at, it.split, p);
-          } else if (p.e.vec != 0 && at + 32 <= p.n) {
-            if (row0 + lane < p.m) {
-              Raw32<T> bias;
-              if (FWD && p.e.bias != nullptr)
-                bias = load_raw32<T>(reinterpret_cast<const T*>(p.e.bias) + at);
-              finish32<T, FWD>(v, row0 + lane, at, p, bias, bias);
-            }
-          } else {
-            finish_turned<T, FWD, L::TROWS>(v, row0, at, p, turn);
-          }
+          finish(v, 32 * c);
         }
       }
+    }
+    // no load or store of this warp's may use the staging after the block has gone
+    if (lane == 0) {
+      if (*s_abort != 0) {
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t uses = h == 0 ? uses0 : uses1;
+          if (uses > 0)
+            tma::mbar_wait_bounded(BAR(B_RES + 2 * warp + h), (uses - 1) & 1, a.limit);
+        }
+      }
+      tma::bulk_wait_read_all();
     }
   }
 
@@ -717,17 +891,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-bool encode16(CUtensorMap* map, const Operand& o, int planes, uint32_t box_rows) {
+// An operand as boxes of `inner` x `rows` elements per plane (inner 64: 128
+// bytes and their swizzle, 32: 64).
+bool encode_operand(CUtensorMap* map, const Operand& o, int planes, uint32_t inner,
+                    uint32_t rows) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = tma::encoder();
   if (fn == nullptr) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)planes};
   const cuuint64_t row = (cuuint64_t)o.ld * 2;
   const cuuint64_t strides[2] = {row, planes > 1 ? (cuuint64_t)o.plane * 2
                                                  : row * (cuuint64_t)o.rows};
-  const cuuint32_t box[3] = {64, box_rows, 1}, es[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {inner, rows, 1}, es[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box,
-            es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A row-major matrix as the epilogue's staged blocks: 32 rows of rowb bytes.
+bool encode_staged(CUtensorMap* map, const void* p, int elem, int64_t cols, int64_t rows,
+                   int64_t ld, uint32_t rowb) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = tma::encoder();
+  if (fn == nullptr) return false;
+  if (rows <= 1) ld = (cols + 7) / 8 * 8;  // one row: any legal stride
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * (cuuint64_t)elem};
+  const cuuint32_t box[2] = {rowb / (uint32_t)elem, 32}, es[2] = {1, 1};
+  return fn(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+            const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct Device {
@@ -766,19 +959,39 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
                                       (int)L::SMEM) == cudaSuccess;
   });
   if (!ready[dev]) return QRB_ERR_LAUNCH;
-  CUtensorMap ma[2], mb[2];
+  CUtensorMap ma[2], mb[2], mo[2], mr, mz;
+  constexpr int ES = sizeof(T);
   for (int i = 0; i < count; ++i) {
-    if (!encode16(&ma[i], q[i]->a, L::NP, args.p[i].amn ? BK : BM) ||
-        !encode16(&mb[i], q[i]->b, L::NP, args.p[i].bmn ? BK : L::BROWS))
-      return QRB_ERR_UNSUPPORTED;
+    const Problem& p = args.p[i];
+    const Epilogue& e = p.e;
+    bool fine = encode_operand(&ma[i], q[i]->a, L::NP, p.amn ? 64 : L::BK, p.amn ? L::BK : BM) &&
+                encode_operand(&mb[i], q[i]->b, L::NP, p.bmn ? 64 : L::BK,
+                               p.bmn ? L::BK : L::BROWS);
+    if (p.splits > 1)
+      fine = fine && encode_staged(&mo[i], p.part, 4, p.part_ld, p.part_rows * p.splits,
+                                   p.part_ld, 128);
+    else if (e.vec)
+      fine = fine && encode_staged(&mo[i], e.out, ES, p.n, p.m, e.ldo, L::ROWB);
+    else
+      mo[i] = ma[i];  // (not used)
+    if (!fine) return QRB_ERR_UNSUPPORTED;
   }
   if (count == 1) {
     ma[1] = ma[0];
     mb[1] = mb[0];
+    mo[1] = mo[0];
+  }
+  mr = mz = mo[0];
+  if (FWD && args.p[0].splits == 1 && args.p[0].e.vec) {
+    const Problem& p = args.p[0];
+    if ((p.e.residual != nullptr &&
+         !encode_staged(&mr, p.e.residual, ES, p.n, p.m, p.e.ldr, L::ROWB)) ||
+        (p.e.z != nullptr && !encode_staged(&mz, p.e.z, ES, p.n, p.m, p.e.ldz, L::ROWB)))
+      return QRB_ERR_UNSUPPORTED;
   }
   if constexpr (CG == 1) {
-    k_product<CG, BN, T, FWD><<<args.s.workers, kThreads, L::SMEM, s>>>(ma[0], mb[0], ma[1], mb[1],
-                                                                        args);
+    k_product<CG, BN, T, FWD><<<args.s.workers, kThreads, L::SMEM, s>>>(
+        ma[0], mb[0], ma[1], mb[1], mo[0], mo[1], mr, mz, args);
   } else {
     cudaLaunchConfig_t lc = {};
     cudaLaunchAttribute la[1];
@@ -792,8 +1005,8 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
     lc.stream = s;
     lc.attrs = la;
     lc.numAttrs = 1;
-    if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD>, ma[0], mb[0], ma[1], mb[1], args) !=
-        cudaSuccess) {
+    if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD>, ma[0], mb[0], ma[1], mb[1], mo[0],
+                           mo[1], mr, mz, args) != cudaSuccess) {
       (void)cudaGetLastError();
       return QRB_ERR_LAUNCH;
     }
@@ -836,8 +1049,9 @@ constexpr Cut kCuts32[] = {{2, 128}, {1, 128}, {1, 64}};
 // a clock; rows beyond a short m are not read).
 double stage_clocks(bool f32, Cut c, int64_t m) {
   const double rows = m < BM ? (double)m : BM;
-  const double mma = 2.0 * c.bn * (f32 ? 6 : 1);
-  const double load = 2.0 * (rows + c.bn / c.cg) * (f32 ? 3 : 1);
+  // (an FP32 stage is half as long)
+  const double mma = 2.0 * c.bn * (f32 ? 3 : 1);
+  const double load = 2.0 * (rows + c.bn / c.cg) * (f32 ? 1.5 : 1);
   return mma > load ? mma : load;
 }
 double item_clocks(bool f32, Cut c, int64_t m, int64_t kb) {
@@ -877,13 +1091,15 @@ double make_schedule(const int64_t* items, const double* clocks, int64_t most, S
   return length;
 }
 
-Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, Cut c, int splits) {
+int stage_values(bool f32) { return f32 ? Lay<1, 64, float>::BK : Lay<1, 64, bf16>::BK; }
+
+Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, Cut c, int bk, int splits) {
   Problem p = {};
   p.m = (int)m;
   p.n = (int)n;
   p.mt = (int)tiles_of(m, BM * c.cg);
   p.nt = (int)tiles_of(n, c.bn);
-  p.kb = (int)tiles_of(k, BK);
+  p.kb = (int)tiles_of(k, bk);
   p.splits = splits;
   p.items = p.mt * p.nt * splits;
   p.group = c.cg == 2 ? 8 : 16;
@@ -911,7 +1127,7 @@ static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
     int64_t tiles[2] = {0, 0}, kb[2] = {1, 1};
     for (int i = 0; i < count; ++i) {
       tiles[i] = tiles_of(sizes[i].m, BM * c.cg) * tiles_of(sizes[i].n, c.bn);
-      kb[i] = tiles_of(sizes[i].k, BK);
+      kb[i] = tiles_of(sizes[i].k, stage_values(f32));
       if (tiles[i] > (1 << 26)) return best;  // (refused: 26 bits of tiles)
     }
     for (int s0 = 1; s0 <= 16 && s0 <= kb[0]; ++s0) {
@@ -999,7 +1215,7 @@ int launch_products(int dtype, const Product* products, int count, const Product
     const int i = count > 1 ? (j == 0 ? plan.first : 1 - plan.first) : 0;  // longer items first
     q[j] = &products[i];
     const ProductSize& z = products[i].size;
-    args.p[j] = problem_of(products[i].kind, z.m, z.n, z.k, c, plan.splits[i]);
+    args.p[j] = problem_of(products[i].kind, z.m, z.n, z.k, c, stage_values(f32), plan.splits[i]);
     args.p[j].part = plan.splits[i] > 1 ? products[i].part : nullptr;
     args.p[j].part_rows = plan.part_rows[i];
     args.p[j].part_ld = plan.part_ld[i];
