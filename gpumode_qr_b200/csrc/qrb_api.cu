@@ -35,6 +35,9 @@ std::atomic<int64_t> g_tma_split{1024};    // two row halves from this height (0
 std::atomic<int64_t> g_tma_pair{0};        // halves on: 0 auto, 1 one CTA, 2 a CTA pair per tile
 std::atomic<int64_t> g_tma_dual{0};        // 32 reflectors: 0 auto, 1 one CTA per SM, 2 two
 std::atomic<int64_t> g_la_depth{0};        // two-level look-ahead depth: 0 auto, 1 or 2 blocks
+std::atomic<int64_t> g_linear_cut{0};      // linear products: 0 automatic, else 1000 CTAs + width
+std::atomic<int64_t> g_linear_splits{0};   // parts of a product's reduction, 0 = automatic
+std::atomic<int64_t> g_linear_rows{-1};    // most rows of the few-row kernel, -1 = automatic
 std::atomic<int64_t> g_narrow{1};          // narrow cluster kernel for the next panel's columns
 std::atomic<int64_t> g_panel_priority{1};  // look-ahead stream at the highest priority
 
@@ -469,6 +472,9 @@ bool mid_fused_enabled() { return g_mid_fused.load() != 0; }
 bool mid_fused_always() { return g_mid_fused.load() == 2; }
 int panel_rpt() { return (int)g_panel_rpt.load(); }
 int gram_tile() { return (int)g_gram_tile.load(); }
+int linear_cut() { return (int)g_linear_cut.load(); }
+int linear_splits() { return (int)g_linear_splits.load(); }
+int linear_rows() { return (int)g_linear_rows.load(); }
 int64_t host_direct_blocks() {
   const int64_t b = g_direct_blocks.load();
   return b > 0 ? b : kHostDirectBlocks;
@@ -953,6 +959,22 @@ int qrb_set_config(const char* key, int64_t value) {
     g_gram_tile.store(value);
     return QRB_OK;
   }
+  if (std::strcmp(key, "linear_cut") == 0) {
+    if (value != 0 && value != 2256 && value != 2128 && value != 1128 && value != 1064)
+      return QRB_ERR_INVALID_ARG;
+    g_linear_cut.store(value);
+    return QRB_OK;
+  }
+  if (std::strcmp(key, "linear_splits") == 0) {
+    if (value < 0 || value > 16) return QRB_ERR_INVALID_ARG;
+    g_linear_splits.store(value);
+    return QRB_OK;
+  }
+  if (std::strcmp(key, "linear_rows") == 0) {
+    if (value < -1 || value > 32) return QRB_ERR_INVALID_ARG;
+    g_linear_rows.store(value);
+    return QRB_OK;
+  }
   if (std::strcmp(key, "mid_fused") == 0) {
     if (value < 0 || value > 2) return QRB_ERR_INVALID_ARG;
     g_mid_fused.store(value);
@@ -1022,6 +1044,9 @@ int qrb_get_config(const char* key, int64_t* value) {
   if (std::strcmp(key, "two_level") == 0) { *value = g_two_level.load(); return QRB_OK; }
   if (std::strcmp(key, "panel_rpt") == 0) { *value = g_panel_rpt.load(); return QRB_OK; }
   if (std::strcmp(key, "gram_tile") == 0) { *value = g_gram_tile.load(); return QRB_OK; }
+  if (std::strcmp(key, "linear_cut") == 0) { *value = g_linear_cut.load(); return QRB_OK; }
+  if (std::strcmp(key, "linear_splits") == 0) { *value = g_linear_splits.load(); return QRB_OK; }
+  if (std::strcmp(key, "linear_rows") == 0) { *value = g_linear_rows.load(); return QRB_OK; }
   if (std::strcmp(key, "direct_blocks") == 0) { *value = qrb::host_direct_blocks(); return QRB_OK; }
   if (std::strcmp(key, "host_path") == 0) { *value = qrb::host_last_path(); return QRB_OK; }
   return QRB_ERR_INVALID_ARG;

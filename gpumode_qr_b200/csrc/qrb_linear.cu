@@ -121,6 +121,9 @@ Forward plan_forward(const qrbl_linear_args& a, Carve* c) {
   f.x = operand_of(a.dtype, f.xs, c, &f.stage_x);
   f.w = operand_of(a.dtype, f.ws, c, &f.stage_w);
   f.size.m = a.m; f.size.n = a.n; f.size.k = a.k;
+  f.size.epilogue = (a.activation > QRBL_ACT_RELU ? 1 : 0) |
+                    (a.z != nullptr || a.z_codes != nullptr ? 2 : 0) |
+                    (a.residual != nullptr ? 4 : 0);
   f.plan = plan_products(a.dtype, &f.size, 1);
   f.part = reinterpret_cast<float*>(c->take(f.plan.part_bytes[0]));
   return f;

@@ -10,6 +10,13 @@
 #include "qrb_common.cuh"
 
 namespace qrb {
+// qrb_set_config test hooks of the linear products: "linear_cut" (0 automatic,
+// else 1000 * CTAs per tile + tile width: 2256, 2128, 1128 or 1064),
+// "linear_splits" (parts of the reduction, 0 automatic) and "linear_rows" (most
+// rows of the few-row kernel, -1 automatic).
+int linear_cut();
+int linear_splits();
+int linear_rows();
 namespace lin {
 
 using bf16 = __nv_bfloat16;
@@ -441,6 +448,7 @@ enum ProductKind { kForward = 0, kGradIn = 1, kGradW = 2 };
 
 struct ProductSize {
   int64_t m = 0, n = 0, k = 0;
+  int epilogue = 0;  // extra work per value: 1 activation, 2 kept z, 4 residual
 };
 struct Product {
   int kind = kForward;

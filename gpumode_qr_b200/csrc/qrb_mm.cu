@@ -309,11 +309,12 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
   }
 }
 
-// Staged blocks: 32 rows (lane = row) of ROWB bytes with TMA's 128- or 64-byte
-// swizzle, which also spreads a warp's 16-byte accesses over the banks.
+// Staged blocks: 32 rows (lane = row) of ROWB bytes with TMA's swizzle of that
+// width, which also spreads a warp's 16-byte accesses over the banks.
 template <uint32_t ROWB>
 __device__ __forceinline__ uint32_t staged_at(uint32_t buf, int row, int unit) {
-  const int x = ROWB == 128 ? unit ^ (row & 7) : unit ^ ((row >> 1) & 3);
+  const int x = ROWB == 128 ? unit ^ (row & 7)
+                            : (ROWB == 64 ? unit ^ ((row >> 1) & 3) : unit ^ ((row >> 2) & 1));
   return buf + row * ROWB + x * 16;
 }
 template <typename T>
@@ -495,12 +496,12 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
   }
 }
 
-// The packed form of 32 columns of one row (lane = row).
-template <typename T>
-__device__ __forceinline__ void pack32(const float (&v)[32], int row, int col, const Problem& a) {
+// The packed form of 32 columns of the lane's row: codes into the staged block
+// (rows of CB bytes) from column `first`; returns the exponent.
+template <typename T, uint32_t CB>
+__device__ __forceinline__ int pack32(uint32_t buf, int first, const float (&v)[32]) {
   constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
-  const Epilogue& e = a.e;
-  float amax = 0.f;
+  float amax = 0.f;  // columns beyond the matrix are 0 (or, beside Inf or NaN, NaN)
 #pragma unroll
   for (int i = 0; i < 32; ++i) amax = max_abs_nan(amax, v[i]);
   const bool fine = finite_f(amax);
@@ -508,23 +509,13 @@ __device__ __forceinline__ void pack32(const float (&v)[32], int row, int col, c
   const int ex = block_exponent(amax, lo, hi);
   uint32_t w[8];
   encode(v, ex, fine && ex < hi, ex == hi ? 63.f : 127.f, w);
-  if (row >= a.m || col >= a.n) return;
-  int8_t* out = e.z_codes + (int64_t)row * a.n + col;  // n % 16 == 0, 16-byte aligned
-  reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  if (col + 16 < a.n) reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  e.z_exps[(int64_t)row * ((a.n + kBlk - 1) / kBlk) + col / kBlk] = (int8_t)ex;
-}
-
-// 32 values at p (of them `valid` within the row), 16-byte aligned, added.
-template <typename T>
-__device__ __forceinline__ void add_bias(float (&v)[32], const T* p, int valid) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float f[8];
-    values8<T>(load_raw8<T>(p + 8 * j, true, valid - 8 * j), f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * j + i] += f[i];
-  }
+  for (int j = 0; j < 2; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
+                     staged_at<CB>(buf, threadIdx.x & 31, first / 16 + j)),
+                 "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                 : "memory");
+  return ex;
 }
 
 template <int CG, int BN, typename T, bool FWD>
@@ -533,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
               const __grid_constant__ CUtensorMap map_o0, const __grid_constant__ CUtensorMap map_o1,
               const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_z,
+              const __grid_constant__ CUtensorMap map_q,
               const __grid_constant__ Args a) {
   using L = Lay<CG, BN, T>;
   extern __shared__ uint8_t smem_raw[];
@@ -718,7 +710,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row0 = it.m0 + rank * BM + quad * 32, col = it.n0 + half * HC;
       const bool part = p.splits > 1, inside = row0 < p.m;
       const bool staged = part || e.vec != 0;
-      const bool keep_z = FWD && !part && staged && e.z != nullptr;
+      // what is kept of z goes through the first half, y through the second
+      const bool plain_z = FWD && !part && staged && e.z != nullptr;
+      const bool packed_z = FWD && !part && staged && e.z_codes != nullptr;
+      const bool keep_z = plain_z || packed_z;
       const bool has_res = FWD && !part && staged && e.residual != nullptr;
       // the staging is free: the last tile's stores have read it
       if (lane == 0) tma::bulk_wait_read_all();
@@ -736,6 +731,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         uses0 += h == 0 ? 1u : 0u;
         uses1 += h == 0 ? 0u : 1u;
       };
+      // the bias of the warp's columns: lane l has column l of each block of 32
+      float bias[HC / 32];
+      if constexpr (FWD) {
+#pragma unroll
+        for (int i = 0; i < HC / 32; ++i) {
+          const int c = col + 32 * i + lane;
+          bias[i] = e.bias != nullptr && c < p.n && staged && !part
+                        ? to_f<T>(reinterpret_cast<const T*>(e.bias)[c])
+                        : 0.f;
+        }
+      }
+      uint32_t exps = 0;
       const bool early = has_res && inside && !(NH == 1 && keep_z);
       if (early && col < p.n) load_res(0);
       if (early && !keep_z && NH == 2 && HC > L::GW && col + L::GW < p.n) load_res(1);
@@ -783,11 +790,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (has_res && !(NH == 1 && keep_z)) load_res(g);
         }
         if constexpr (FWD) {
-          const int valid = p.n - at < 32 ? p.n - at : 32;
-          if (e.bias != nullptr) add_bias<T>(v, reinterpret_cast<const T*>(e.bias) + at, valid);
-          if (keep_z) {
+          if (e.bias != nullptr) {
+            float mine = bias[0];
+#pragma unroll
+            for (int i = 1; i < HC / 32; ++i) mine = c == 32 * i ? bias[i] : mine;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(kFull, mine, i);
+          }
+          const bool flush = last || at + 32 >= p.n;
+          if (plain_z) {
             stage_write<T, L::ROWB>(stg, in, v);
-            if (last || at + 32 >= p.n) {
+            if (flush) {
               tma::fence_proxy_async();
               __syncwarp();
               if (lane == 0) {
@@ -799,7 +812,34 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (NH == 1 && has_res) load_res(g);
             }
           }
-          if (e.z_codes != nullptr) pack32<T>(v, row0 + lane, at, p);
+          if (packed_z) {
+            const int ex = pack32<T, L::GW>(stg, in, v);
+            exps |= (uint32_t)(ex & 255) << (8 * (c / 32));
+            if (flush) {
+              tma::fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                store_box(&map_q, stg, at - in, row0);
+                tma::bulk_commit();
+                if constexpr (NH == 1) tma::bulk_wait_read_all();
+              }
+              __syncwarp();
+              if (NH == 1 && has_res) load_res(g);
+            }
+            if (c + 32 == HC || at + 32 >= p.n) {  // the row's exponents of all blocks
+              const int nblk = (p.n + kBlk - 1) / kBlk, count = c / 32 + 1;
+              int8_t* x = e.z_exps + (int64_t)(row0 + lane) * nblk + col / kBlk;
+              if (row0 + lane < p.m) {
+                if (count == 4 && (reinterpret_cast<uintptr_t>(x) & 3) == 0) {
+                  *reinterpret_cast<uint32_t*>(x) = exps;
+                } else {
+#pragma unroll
+                  for (int i = 0; i < HC / 32; ++i)
+                    if (i < count) x[i] = (int8_t)(exps >> (8 * i));
+                }
+              }
+            }
+          }
           act_by(v, e.act);
           if (has_res) {
             if (in == 0) {
@@ -913,14 +953,19 @@ bool encode_staged(CUtensorMap* map, const void* p, int elem, int64_t cols, int6
                    int64_t ld, uint32_t rowb) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = tma::encoder();
   if (fn == nullptr) return false;
-  if (rows <= 1) ld = (cols + 7) / 8 * 8;  // one row: any legal stride
+  if (rows <= 1) ld = (cols + 15) / 16 * 16;  // one row: any legal stride
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld * (cuuint64_t)elem};
   const cuuint32_t box[2] = {rowb / (uint32_t)elem, 32}, es[2] = {1, 1};
-  return fn(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-            const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const CUtensorMapDataType type = elem == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUtensorMapSwizzle swizzle = rowb == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : rowb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                  : CU_TENSOR_MAP_SWIZZLE_32B;
+  return fn(map, type, 2, const_cast<void*>(p), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct Device {
@@ -959,7 +1004,7 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
                                       (int)L::SMEM) == cudaSuccess;
   });
   if (!ready[dev]) return QRB_ERR_LAUNCH;
-  CUtensorMap ma[2], mb[2], mo[2], mr, mz;
+  CUtensorMap ma[2], mb[2], mo[2], mr, mz, mq;
   constexpr int ES = sizeof(T);
   for (int i = 0; i < count; ++i) {
     const Problem& p = args.p[i];
@@ -981,17 +1026,18 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
     mb[1] = mb[0];
     mo[1] = mo[0];
   }
-  mr = mz = mo[0];
+  mr = mz = mq = mo[0];
   if (FWD && args.p[0].splits == 1 && args.p[0].e.vec) {
     const Problem& p = args.p[0];
     if ((p.e.residual != nullptr &&
          !encode_staged(&mr, p.e.residual, ES, p.n, p.m, p.e.ldr, L::ROWB)) ||
-        (p.e.z != nullptr && !encode_staged(&mz, p.e.z, ES, p.n, p.m, p.e.ldz, L::ROWB)))
+        (p.e.z != nullptr && !encode_staged(&mz, p.e.z, ES, p.n, p.m, p.e.ldz, L::ROWB)) ||
+        (p.e.z_codes != nullptr && !encode_staged(&mq, p.e.z_codes, 1, p.n, p.m, p.n, L::GW)))
       return QRB_ERR_UNSUPPORTED;
   }
   if constexpr (CG == 1) {
     k_product<CG, BN, T, FWD><<<args.s.workers, kThreads, L::SMEM, s>>>(
-        ma[0], mb[0], ma[1], mb[1], mo[0], mo[1], mr, mz, args);
+        ma[0], mb[0], ma[1], mb[1], mo[0], mo[1], mr, mz, mq, args);
   } else {
     cudaLaunchConfig_t lc = {};
     cudaLaunchAttribute la[1];
@@ -1006,7 +1052,7 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
     lc.attrs = la;
     lc.numAttrs = 1;
     if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD>, ma[0], mb[0], ma[1], mb[1], mo[0],
-                           mo[1], mr, mz, args) != cudaSuccess) {
+                           mo[1], mr, mz, mq, args) != cudaSuccess) {
       (void)cudaGetLastError();
       return QRB_ERR_LAUNCH;
     }
@@ -1037,41 +1083,44 @@ int launch_type(int cg, int bn, bool fwd, const Product* const* q, int count, Ar
 
 int64_t tiles_of(int64_t v, int64_t t) { return (v + t - 1) / t; }
 
-// The cuts of the kernel: CTAs per tile and tile width.
+// The cuts of the kernel: CTAs per tile, tile width, and what one stage of one
+// tile takes, in microseconds, measured on a B200 over m, n, k = 360 .. 8192.
 struct Cut {
   int cg, bn;
+  double stage;
 };
-constexpr Cut kCuts16[] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
-constexpr Cut kCuts32[] = {{2, 128}, {1, 128}, {1, 64}};
+constexpr Cut kCuts16[] = {{2, 256, 0.33}, {2, 128, 0.25}, {1, 128, 0.25}, {1, 64, 0.20}};
+constexpr Cut kCuts32[] = {{2, 128, 0.65}, {1, 128, 0.72}, {1, 64, 0.53}};
 
-// Estimated SM clocks of one stage of one CTA: the larger of its MMAs (2 BN
-// clocks, shared by a pair; six times as many in FP32) and its loads (64 bytes
-// a clock; rows beyond a short m are not read).
-double stage_clocks(bool f32, Cut c, int64_t m) {
-  const double rows = m < BM ? (double)m : BM;
-  // (an FP32 stage is half as long)
-  const double mma = 2.0 * c.bn * (f32 ? 3 : 1);
-  const double load = 2.0 * (rows + c.bn / c.cg) * (f32 ? 1.5 : 1);
-  return mma > load ? mma : load;
-}
-double item_clocks(bool f32, Cut c, int64_t m, int64_t kb) {
-  return (double)kb * stage_clocks(f32, c, m) + 500.0;
+// One tile's products and its epilogue (which run beside another tile's), in
+// microseconds: a column of results takes 11 ns, 12 more with an activation, 6
+// with z kept, 5 with a residual (FP32 twice that).
+struct TileTime {
+  double main, epi;
+  double longer() const { return main > epi ? main : epi; }
+  double shorter() const { return main > epi ? epi : main; }
+};
+TileTime tile_time(bool f32, const Cut& c, const ProductSize& z, int64_t kb, bool split) {
+  const double col = split ? 0.011
+                           : 0.011 + ((z.epilogue & 1) ? 0.012 : 0) + ((z.epilogue & 2) ? 0.006 : 0) +
+                                 ((z.epilogue & 4) ? 0.005 : 0);
+  return {(double)kb * c.stage, c.bn * col * (f32 ? 2 : 1)};
 }
 
 // The schedule of `items[0]` longer and `items[1]` shorter items over `most`
-// workers, and its length in the items' clocks.
-double make_schedule(const int64_t* items, const double* clocks, int64_t most, Schedule* out) {
+// workers, and its length in the items' own times.
+double make_schedule(const int64_t* items, const double* each, int64_t most, Schedule* out) {
   const int64_t all = items[0] + items[1];
   const int64_t g = all < most ? all : most;
   Schedule s = {};
   s.workers = (int)g;
   s.q = (int)(items[0] / g);
   s.r = (int)(items[0] % g);
-  double length = (s.q + (s.r > 0 ? 1 : 0)) * clocks[0];
+  double length = (s.q + (s.r > 0 ? 1 : 0)) * each[0];
   if (items[1] > 0) {
     // the least x whose level holds every short item; y by what the one more
     // long item leaves of it
-    const double ratio = clocks[0] / clocks[1];
+    const double ratio = each[0] / each[1];
     int64_t x = (items[1] - 1) / g;
     for (;; ++x) {
       int64_t y = x - (int64_t)(ratio + 0.5);
@@ -1083,8 +1132,8 @@ double make_schedule(const int64_t* items, const double* clocks, int64_t most, S
         break;
       }
     }
-    const double late = s.q * clocks[0] + s.x * clocks[1];
-    const double early = s.r > 0 ? (s.q + 1) * clocks[0] + s.y * clocks[1] : 0;
+    const double late = s.q * each[0] + s.x * each[1];
+    const double early = s.r > 0 ? (s.q + 1) * each[0] + s.y * each[1] : 0;
     length = late > early ? late : early;
   }
   *out = s;
@@ -1093,7 +1142,7 @@ double make_schedule(const int64_t* items, const double* clocks, int64_t most, S
 
 int stage_values(bool f32) { return f32 ? Lay<1, 64, float>::BK : Lay<1, 64, bf16>::BK; }
 
-Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, Cut c, int bk, int splits) {
+Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, const Cut& c, int bk, int splits) {
   Problem p = {};
   p.m = (int)m;
   p.n = (int)n;
@@ -1110,9 +1159,9 @@ Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, Cut c, int bk, int
 
 }  // namespace
 
-// The cut with the least estimated time, in SM clocks: the schedule's length, a
-// start, and for each split product the writing and reading of its partial
-// tiles and its second launch.
+// The cut with the least estimated time: a start of 4.5 us, the schedule's
+// length, the end of the last tile, and for each split product 2.5 us for its
+// second launch and its partial sums' way out and back at 5 TB/s.
 static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
   ProductPlan best;
   const Device* d = device_info();
@@ -1121,8 +1170,12 @@ static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
   double least = -1;
   const Cut* cuts = f32 ? kCuts32 : kCuts16;
   const int ncuts = f32 ? 3 : 4;
+  const int hook_cut = linear_cut(), hook_splits = linear_splits();
   for (int ci = 0; ci < ncuts; ++ci) {
     const Cut c = cuts[ci];
+    // (a cut that FP32 does not have: its widest)
+    if (hook_cut != 0 && hook_cut != 1000 * c.cg + c.bn && !(f32 && hook_cut == 2256 && ci == 0))
+      continue;
     const int64_t workers = sms / c.cg;
     int64_t tiles[2] = {0, 0}, kb[2] = {1, 1};
     for (int i = 0; i < count; ++i) {
@@ -1131,23 +1184,27 @@ static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
       if (tiles[i] > (1 << 26)) return best;  // (refused: 26 bits of tiles)
     }
     for (int s0 = 1; s0 <= 16 && s0 <= kb[0]; ++s0) {
-      if (s0 > 1 && tiles[0] * (s0 - 1) >= workers) break;
+      if (hook_splits > 0 && s0 != hook_splits && s0 != kb[0]) continue;
+      if (hook_splits == 0 && s0 > 1 && tiles[0] * (s0 - 1) >= workers) break;
       for (int s1 = 1; s1 <= (count > 1 ? 16 : 1) && s1 <= kb[1]; ++s1) {
-        if (s1 > 1 && tiles[1] * (s1 - 1) >= workers) break;
+        if (hook_splits > 0 && count > 1 && s1 != hook_splits && s1 != kb[1]) continue;
+        if (hook_splits == 0 && s1 > 1 && tiles[1] * (s1 - 1) >= workers) break;
         const int sp[2] = {s0, s1};
-        double len[2] = {0, 0}, t = 3000.0;
+        double len[2] = {0, 0}, t = 4.5, end = 0;
         int64_t items[2] = {0, 0};
         for (int i = 0; i < count; ++i) {
+          const ProductSize& z = sizes[i];
+          const TileTime x = tile_time(f32, c, z, tiles_of(kb[i], sp[i]), sp[i] > 1);
           items[i] = tiles[i] * sp[i];
-          len[i] = item_clocks(f32, c, sizes[i].m, tiles_of(kb[i], sp[i]));
-          if (sp[i] > 1)
-            t += 6000.0 + 2.0 * sp[i] * (double)sizes[i].m * (double)sizes[i].n * 4.0 / 2500.0;
+          len[i] = x.longer();
+          if (x.shorter() > end) end = x.shorter();
+          if (sp[i] > 1) t += 2.5 + 8.0 * sp[i] * (double)z.m * (double)z.n / 5e6;
         }
         const bool swap = count > 1 && len[1] > len[0];
         const int64_t it[2] = {items[swap ? 1 : 0], count > 1 ? items[swap ? 0 : 1] : 0};
-        const double cl[2] = {len[swap ? 1 : 0], count > 1 ? len[swap ? 0 : 1] : 1.0};
+        const double each[2] = {len[swap ? 1 : 0], count > 1 ? len[swap ? 0 : 1] : 1.0};
         Schedule sc;
-        t += make_schedule(it, cl, workers, &sc);
+        t += make_schedule(it, each, workers, &sc) + end;
         if (least < 0 || t < least) {
           least = t;
           best.cg = c.cg;
@@ -1175,25 +1232,28 @@ static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
 // launch) and a model's layers repeat.
 ProductPlan plan_products(int dtype, const ProductSize* sizes, int count) {
   struct Entry {
-    int dtype = -1, count = 0, sms = 0;
+    int dtype = -1, count = 0, sms = 0, hooks = 0;
     ProductSize z[2];
     ProductPlan plan;
   };
   static thread_local Entry kept[64];
   const Device* d = device_info();
   const int sms = d != nullptr ? d->sms : 0;
+  const int hooks = linear_cut() * 32 + linear_splits();
   uint64_t h = (uint64_t)dtype * 3 + (uint64_t)count;
   for (int i = 0; i < count; ++i)
     h = (h * 1000003u + (uint64_t)sizes[i].m) * 1000003u + (uint64_t)sizes[i].n * 8191u +
         (uint64_t)sizes[i].k;
   Entry& e = kept[(h ^ (h >> 17) ^ (h >> 31)) % 64];
-  bool same = e.dtype == dtype && e.count == count && e.sms == sms;
+  bool same = e.dtype == dtype && e.count == count && e.sms == sms && e.hooks == hooks;
   for (int i = 0; i < count && same; ++i)
-    same = e.z[i].m == sizes[i].m && e.z[i].n == sizes[i].n && e.z[i].k == sizes[i].k;
+    same = e.z[i].m == sizes[i].m && e.z[i].n == sizes[i].n && e.z[i].k == sizes[i].k &&
+           e.z[i].epilogue == sizes[i].epilogue;
   if (!same) {
     e.dtype = dtype;
     e.count = count;
     e.sms = sms;
+    e.hooks = hooks;
     for (int i = 0; i < count; ++i) e.z[i] = sizes[i];
     e.plan = search_plan(dtype, sizes, count);
   }
@@ -1205,12 +1265,16 @@ int launch_products(int dtype, const Product* products, int count, const Product
   const Device* d = device_info();
   if (d == nullptr) return QRB_ERR_DEVICE;
   if (!plan.ok) return QRB_ERR_UNSUPPORTED;
-  const Cut c = {plan.cg, plan.bn};
   const bool f32 = dtype == QRBL_F32;
+  Cut c = {plan.cg, plan.bn, 1.0};
+  for (const Cut& k : kCuts16)
+    if (!f32 && k.cg == c.cg && k.bn == c.bn) c = k;
+  for (const Cut& k : kCuts32)
+    if (f32 && k.cg == c.cg && k.bn == c.bn) c = k;
   Args args = {};
   const Product* q[2] = {nullptr, nullptr};
   int64_t items[2] = {0, 0};
-  double clocks[2] = {1.0, 1.0};
+  double each[2] = {1.0, 1.0};
   for (int j = 0; j < count; ++j) {
     const int i = count > 1 ? (j == 0 ? plan.first : 1 - plan.first) : 0;  // longer items first
     q[j] = &products[i];
@@ -1220,12 +1284,15 @@ int launch_products(int dtype, const Product* products, int count, const Product
     args.p[j].part_rows = plan.part_rows[i];
     args.p[j].part_ld = plan.part_ld[i];
     args.p[j].e = products[i].e;
-    if (products[i].e.z_codes != nullptr)  // packed rows 16-byte aligned too
-      args.p[j].e.vec &= aligned16(products[i].e.z_codes) && z.n % 16 == 0;
+    // packed rows 16-byte aligned too (and z not kept both ways: one staging half)
+    if (products[i].e.z_codes != nullptr)
+      args.p[j].e.vec &= aligned16(products[i].e.z_codes) && z.n % 16 == 0 &&
+                         products[i].e.z == nullptr;
     items[j] = args.p[j].items;
-    clocks[j] = item_clocks(f32, c, z.m, tiles_of(args.p[j].kb, plan.splits[i]));
+    each[j] = tile_time(f32, c, z, tiles_of(args.p[j].kb, plan.splits[i]), plan.splits[i] > 1)
+                  .longer();
   }
-  make_schedule(items, clocks, d->sms / c.cg, &args.s);
+  make_schedule(items, each, d->sms / c.cg, &args.s);
   if (sum != nullptr) args.sum = *sum;
   args.err = d->err;
   args.limit = device_wait_limit();

@@ -228,7 +228,11 @@ void rows32(const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
 
 }  // namespace
 
-int64_t rows_most(int dtype) { return dtype == QRBL_F32 ? 8 : 32; }
+int64_t rows_most(int dtype) {
+  const int64_t most = dtype == QRBL_F32 ? 8 : 32;
+  const int hook = linear_rows();
+  return hook < 0 || hook > most ? most : hook;
+}
 
 int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
                 const Epilogue& e, cudaStream_t s) {

@@ -31,6 +31,7 @@ from . import _lib
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_NEED = frozenset(("x", "weight", "bias"))
 #: Values of a row that share one exponent in the packed form.
 PACK_BLOCK = 32
 
@@ -58,6 +59,10 @@ class PackedActivation(NamedTuple):
 
 
 def _check(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
+    if (isinstance(t, torch.Tensor) and not t.requires_grad
+            and (t.dtype in _DTYPES and t.is_cuda if like is None
+                 else t.dtype is like.dtype and t.device == like.device)):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.dtype not in _DTYPES:
@@ -75,27 +80,31 @@ def _check(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None
 
 
 def _check_packed(name: str, p: PackedActivation, like: torch.Tensor, shape: tuple) -> None:
-    if p.dtype != like.dtype:
-        raise TypeError(f"{name} was packed from {p.dtype}, the layer is {like.dtype}")
+    codes, exps, dtype = p
+    if dtype is not like.dtype:
+        raise TypeError(f"{name} was packed from {dtype}, the layer is {like.dtype}")
     want = (*shape[:-1], -(-shape[-1] // PACK_BLOCK))
-    for part, t, s in (("codes", p.codes, shape), ("exponents", p.exponents, want)):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int8:
+    for part, t, s in (("codes", codes, shape), ("exponents", exps, want)):
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int8:
             raise TypeError(f"{name}.{part} must be an int8 tensor")
         if t.device != like.device:
             raise ValueError(f"{name}.{part} must be on {like.device}, got {t.device}")
-        if tuple(t.shape) != tuple(s):
+        if t.shape != s:
             raise ValueError(f"{name}.{part} must be {tuple(s)}, got {tuple(t.shape)}")
 
 
-def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """t as [rows, cols] with unit column stride and rows that do not overlap
-    (copying only if needed)."""
-    if t.dim() != 2:
-        t = t.reshape(-1, cols) if cols else t.new_empty((t.shape[:-1].numel(), 0))
+def _rows(t: torch.Tensor, shape: torch.Size, cols: int) -> tuple[torch.Tensor, int, int]:
+    """t (of that shape) as [rows, cols] with unit column stride and rows that do
+    not overlap (copying only if needed), with its rows and row stride."""
+    if len(shape) != 2:
+        t = t.reshape(-1, cols) if cols else t.new_empty((shape[:-1].numel(), 0))
+        shape = t.shape
+    rows = shape[0]
     row, col = t.stride()
-    if (col != 1 and cols > 1) or (row < cols and t.shape[0] > 1):
+    if (col != 1 and cols > 1) or (row < cols and rows > 1):
         t = t.contiguous()
-    return t
+        row = cols
+    return t, rows, row
 
 
 def _activation(name: str) -> int:
@@ -105,28 +114,30 @@ def _activation(name: str) -> int:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {name!r}") from None
 
 
-def _raw_stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
 
 
+_current_device = torch.cuda.current_device
 if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object
+    _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
+_OK, _NEEDS_WORKSPACE = 0, 3  # QRB_OK, QRB_ERR_WORKSPACE
 
-    def _raw_stream(dev: torch.device) -> int:  # noqa: F811
-        return torch._C._cuda_getCurrentRawStream(dev.index)
 
-
-def _run(call, size, args: bytes, dev: torch.device) -> None:
-    """``call`` on ``dev``'s current stream, with the workspace it asks for."""
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _run(call, size, args, dev)
-    stream = _raw_stream(dev)
+def _run(call, size, args: bytes, like: torch.Tensor) -> None:
+    """``call`` on the current stream of ``like``'s device, with the workspace
+    it asks for."""
+    index = like.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return _run(call, size, args, like)
+    stream = _raw_stream(index)
     rc = call(args, None, 0, stream)
-    if rc == 3:  # QRB_ERR_WORKSPACE: nothing was enqueued
+    if rc == _NEEDS_WORKSPACE:  # nothing was enqueued
         need = size(args)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = like.new_empty(need, dtype=torch.uint8)
         rc = call(args, ws.data_ptr(), need, stream)
-    if rc:
+    if rc != _OK:
         _lib.check(rc)
 
 
@@ -153,9 +164,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         raise ValueError(f"x must be [..., k] and weight [n, k], got {tuple(xs)} and {tuple(ws)}")
     act = ACTIVATIONS[activation] if activation in ACTIVATIONS else _activation(activation)
     n, k = ws
-    shape = (*xs[:-1], n)
-    x2, w2 = _rows(x, k), _rows(weight, k)
-    m = x2.shape[0]
+    shape = (xs[0], n) if len(xs) == 2 else (*xs[:-1], n)
+    x2, m, ldx = _rows(x, xs, k)
+    w2, _, ldw = _rows(weight, ws, k)
     bp = rp = ldr = zp = ldz = qp = ep = 0
     if bias is not None:
         _check("bias", bias, x)
@@ -166,27 +177,27 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         bp = bias.data_ptr()
     if residual is not None:
         _check("residual", residual, x)
-        if residual.shape != shape:
-            raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
-        residual = _rows(residual, n)
-        rp, ldr = residual.data_ptr(), residual.stride(0)
+        rs = residual.shape
+        if rs != shape:
+            raise ValueError(f"residual must be {shape}, got {tuple(rs)}")
+        residual, _, ldr = _rows(residual, rs, n)
+        rp = residual.data_ptr()
     z = None
     if keep is not None:
         if keep == "plain":
-            z = x.new_empty(shape)
+            z = x.new_empty(*shape)
             zp, ldz = z.data_ptr(), n
         elif keep == "packed":
             z = _empty_packed(shape, x)
             qp, ep = z.codes.data_ptr(), z.exponents.data_ptr()
         else:
             raise ValueError(f"keep must be None, 'plain' or 'packed', got {keep!r}")
-    y = x.new_empty(shape)
+    y = x.new_empty(*shape)  # (separate ints: parsed faster than a tuple)
     if m and n:
         L = _lib.lib()
         _run(L.qrbl_linear, L.qrbl_linear_workspace_bytes,
-             _linear_args(_DTYPES[x.dtype], act, m, n, k, x2.data_ptr(), x2.stride(0),
-                          w2.data_ptr(), w2.stride(0), bp, rp, ldr, y.data_ptr(), n, zp, ldz, qp,
-                          ep), x.device)
+             _linear_args(_DTYPES[x.dtype], act, m, n, k, x2.data_ptr(), ldx, w2.data_ptr(), ldw,
+                          bp, rp, ldr, y.data_ptr(), n, zp, ldz, qp, ep), x)
     return y if keep is None else (y, z)
 
 
@@ -210,12 +221,12 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     if len(ws) != 2 or not ds or ds[-1] != ws[0]:
         raise ValueError(f"dy must be [..., n] and weight [n, k], got {tuple(ds)} and {tuple(ws)}")
     act = ACTIVATIONS[activation] if activation in ACTIVATIONS else _activation(activation)
-    if isinstance(need, str) or not set(need) <= {"x", "weight", "bias"}:
+    if isinstance(need, str) or not _NEED.issuperset(need):
         raise ValueError(f"need must name some of 'x', 'weight' and 'bias', got {need!r}")
     n, k = ws
-    lead = tuple(ds[:-1])
-    dy2, w2 = _rows(dy, n), _rows(weight, k)
-    m = dy2.shape[0]
+    lead = (ds[0],) if len(ds) == 2 else tuple(ds[:-1])
+    dy2, m, lddy = _rows(dy, ds, n)
+    w2, _, ldw = _rows(weight, ws, k)
     xp = ldx = xq = xe = zp = ldz = zq = ze = dxp = dwp = dbp = 0
     dx = dw = db = None
     if "weight" in need:
@@ -228,11 +239,12 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
             if x is None:
                 raise ValueError("x is needed for the weight's gradient")
             _check("x", x, dy)
-            if x.shape != (*lead, k):
-                raise ValueError(f"x must be {(*lead, k)}, got {tuple(x.shape)}")
-            x2 = _rows(x, k)
-            xp, ldx = x2.data_ptr(), x2.stride(0)
-        dw = dy.new_empty((n, k))
+            xs = x.shape
+            if xs != (*lead, k):
+                raise ValueError(f"x must be {(*lead, k)}, got {tuple(xs)}")
+            x2, _, ldx = _rows(x, xs, k)
+            xp = x2.data_ptr()
+        dw = dy.new_empty(n, k)
         dwp = dw.data_ptr()
     if act:
         if isinstance(z, PackedActivation):
@@ -246,36 +258,37 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
             if z is None:
                 raise ValueError(f"z is needed for the gradient of {activation!r}")
             _check("z", z, dy)
-            if z.shape != (*lead, n):
-                raise ValueError(f"z must be {(*lead, n)}, got {tuple(z.shape)}")
-            z2 = _rows(z, n)
-            zp, ldz = z2.data_ptr(), z2.stride(0)
+            zs = z.shape
+            if zs != ds:
+                raise ValueError(f"z must be {tuple(ds)}, got {tuple(zs)}")
+            z2, _, ldz = _rows(z, zs, n)
+            zp = z2.data_ptr()
     if "x" in need:
-        dx = dy.new_empty((*lead, k))
+        dx = dy.new_empty(*lead, k)
         dxp = dx.data_ptr()
     if "bias" in need:
-        db = dy.new_empty((n,))
+        db = dy.new_empty(n)
         dbp = db.data_ptr()
     L = _lib.lib()
     _run(L.qrbl_linear_backward, L.qrbl_linear_backward_workspace_bytes,
-         _backward_args(_DTYPES[dy.dtype], act, m, n, k, dy2.data_ptr(), dy2.stride(0), xp, ldx,
-                        xq, xe, w2.data_ptr(), w2.stride(0), zp, ldz, zq, ze, dxp, k, dwp, k,
-                        dbp), dy.device)
+         _backward_args(_DTYPES[dy.dtype], act, m, n, k, dy2.data_ptr(), lddy, xp, ldx, xq, xe,
+                        w2.data_ptr(), ldw, zp, ldz, zq, ze, dxp, k, dwp, k, dbp), dy)
     return dx, dw, db
 
 
 def _empty_packed(shape: tuple, like: torch.Tensor) -> PackedActivation:
-    return PackedActivation(
-        like.new_empty(shape, dtype=torch.int8),
-        like.new_empty((*shape[:-1], -(-shape[-1] // PACK_BLOCK)), dtype=torch.int8), like.dtype)
+    blocks = -(-shape[-1] // PACK_BLOCK)
+    return PackedActivation(like.new_empty(*shape, dtype=torch.int8),
+                            like.new_empty(*shape[:-1], blocks, dtype=torch.int8), like.dtype)
 
 
-def _on(dev: torch.device, call, *args) -> None:
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _on(dev, call, *args)
-    rc = call(*args, _raw_stream(dev))
-    if rc:
+def _on(like: torch.Tensor, call, *args) -> None:
+    index = like.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return _on(like, call, *args)
+    rc = call(*args, _raw_stream(index))
+    if rc != _OK:
         _lib.check(rc)
 
 
@@ -292,11 +305,12 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     _check("x", x)
     if x.dim() < 1:
         raise ValueError("x must be [..., c], got a scalar")
-    p = _empty_packed(tuple(x.shape), x)
+    shape = x.shape
+    p = _empty_packed(shape, x)
     if x.numel():
-        x2 = _rows(x, x.shape[-1])
-        _on(x.device, _lib.lib().qrbl_pack, _DTYPES[x.dtype], x2.data_ptr(), x2.stride(0),
-            x2.shape[0], x2.shape[1], p.codes.data_ptr(), p.exponents.data_ptr())
+        x2, rows, ld = _rows(x, shape, shape[-1])
+        _on(x, _lib.lib().qrbl_pack, _DTYPES[x.dtype], x2.data_ptr(), ld, rows, shape[-1],
+            p.codes.data_ptr(), p.exponents.data_ptr())
     return p
 
 
@@ -304,18 +318,19 @@ def unpack_activation(packed: PackedActivation) -> torch.Tensor:
     """The tensor that ``packed`` stands for, in the type it was packed from."""
     if not isinstance(packed, PackedActivation):
         raise TypeError(f"packed must be a PackedActivation, got {type(packed).__name__}")
-    if packed.dtype not in _DTYPES:
-        raise TypeError(f"packed.dtype must be float32, float16 or bfloat16, got {packed.dtype}")
-    codes = packed.codes
+    codes, exps, dtype = packed
+    if dtype not in _DTYPES:
+        raise TypeError(f"packed.dtype must be float32, float16 or bfloat16, got {dtype}")
     if not isinstance(codes, torch.Tensor) or not codes.is_cuda:
         raise ValueError("packed.codes must be a CUDA tensor (libqrb200 has no CPU path)")
-    if codes.dim() < 1:
+    shape = codes.shape
+    if not shape:
         raise ValueError("packed.codes must be [..., c], got a scalar")
-    x = torch.empty(codes.shape, dtype=packed.dtype, device=codes.device)
-    _check_packed("packed", packed, x, tuple(codes.shape))
+    x = codes.new_empty(*shape, dtype=dtype)
+    _check_packed("packed", packed, x, shape)
     if x.numel():
-        codes, exps = codes.contiguous(), packed.exponents.contiguous()
-        cols = x.shape[-1]
-        _on(x.device, _lib.lib().qrbl_unpack, _DTYPES[x.dtype], codes.data_ptr(),
-            exps.data_ptr(), x.numel() // cols, cols, x.data_ptr(), cols)
+        codes, exps = codes.contiguous(), exps.contiguous()
+        cols = shape[-1]
+        _on(x, _lib.lib().qrbl_unpack, _DTYPES[dtype], codes.data_ptr(), exps.data_ptr(),
+            x.numel() // cols, cols, x.data_ptr(), cols)
     return x
