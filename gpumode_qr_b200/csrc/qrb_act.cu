@@ -41,15 +41,11 @@ __device__ __forceinline__ uint2 load_codes(const int8_t* p, bool vec, int valid
     if (i < valid) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void decode8(uint2 q, float step, float (&out)[8]) {
-  float lo[4], hi[4];
-  decode4(q.x, step, lo);
-  decode4(q.y, step, hi);
+__device__ __forceinline__ void decode8f(uint2 q, float step, float (&out)[8]) {
+  f2 v[4];
+  decode8(q, step, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    out[i] = lo[i];
-    out[4 + i] = hi[i];
-  }
+  for (int i = 0; i < 4; ++i) f2_to(v[i], out[2 * i], out[2 * i + 1]);
 }
 __device__ __forceinline__ int clip(int64_t left, int most) {
   return left >= most ? most : (left > 0 ? (int)left : 0);
@@ -61,17 +57,6 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
                "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pair_of(float a, float b) {
-  if constexpr (__is_same(T, bf16)) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
 // ---------------------------------------------------------------------------
 // pack
 // ---------------------------------------------------------------------------
@@ -83,7 +68,7 @@ __global__ void __launch_bounds__(kThreads)
            int8_t* __restrict__ codes, int8_t* __restrict__ exps, int tx, int64_t nx, int vin,
            int vout) {
   constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi, V = 16;
-  const int64_t by = blockIdx.x / nx, bx = blockIdx.x - by * nx;
+  const int64_t by = blockIdx.x / (uint32_t)nx, bx = blockIdx.x % (uint32_t)nx;
   const int ty = kThreads / tx, x0 = threadIdx.x & (tx - 1), y0 = threadIdx.x / tx;
   const int64_t c = (bx * tx + x0) * V;
   const int64_t r0 = by * ty * ROWS + y0;
@@ -148,7 +133,7 @@ template <typename T, bool PACKED, bool PLANES>
 __device__ __forceinline__ void stage_block(const StageJob& j, int64_t block) {
   constexpr int V = kStageVals, ROWS = sizeof(T) == 4 ? 2 : 4;
   const StageArgs& a = j.a;
-  const int64_t by = block / j.nx, bx = block - by * j.nx;
+  const int64_t by = (uint32_t)block / (uint32_t)j.nx, bx = (uint32_t)block % (uint32_t)j.nx;
   const int ty = kThreads / j.tx, x0 = threadIdx.x & (j.tx - 1), y0 = threadIdx.x / j.tx;
   const int64_t c = (bx * j.tx + x0) * V;
   if (!j.vin) {  // rows not 16-byte aligned: one row, neighbouring threads at neighbouring values
@@ -214,7 +199,7 @@ __device__ __forceinline__ void stage_block(const StageJob& j, int64_t block) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[8];
-          decode8(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]),
+          decode8f(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]),
                   v);
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[4 * h + k] = pair_of<T>(v[2 * k], v[2 * k + 1]);
@@ -228,7 +213,7 @@ __device__ __forceinline__ void stage_block(const StageJob& j, int64_t block) {
       if (valid <= 8 * h) continue;
       float v[8];
       if constexpr (PACKED)
-        decode8(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]), v);
+        decode8f(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]), v);
       else
         values8<T>(raw[i][h], v);
       if constexpr (PLANES) {
@@ -256,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) k_unpack(StageJob j) {
 // dz = dy act'(z), and its column sums
 // ---------------------------------------------------------------------------
 // Warps of 256 columns (8 per lane), 8 warps over the rows; a block takes `rows`
-// rows of them, 2 per warp at a time, the next 2 already being loaded. Each thread sums its rows in order, then the block's warps are
+// rows of them, 2 (FP32: 1) per warp loaded together. Each thread sums its rows in order, then the block's warps are
 // added in order: the same bits every time. part[row block][col].
 struct DzJob {
   DzArgs a;
@@ -284,7 +269,15 @@ __device__ __forceinline__ void dz_rows_any(const DzJob& j, int64_t c0, int64_t 
           f[i] = to_f<T>(reinterpret_cast<const T*>(a.z)[r * a.ldz + c]);
       }
     }
-    act_grad_by(d, f, a.act);
+    f2 d2[4], f2v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      d2[i] = f2_of(d[2 * i], d[2 * i + 1]);
+      f2v[i] = f2_of(f[2 * i], f[2 * i + 1]);
+    }
+    act_grad_by(d2, f2v, a.act);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f2_to(d2[i], d[2 * i], d[2 * i + 1]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t c = c0 + (threadIdx.x & 31) + 32 * i;
@@ -300,35 +293,12 @@ __device__ __forceinline__ void dz_rows_any(const DzJob& j, int64_t c0, int64_t 
   }
 }
 
-template <typename T, bool PACKED>
-struct DzIn {  // one row's eight values of dy and z
-  Raw8<T> g, z;
-  uint2 q;
-  int e;
-};
-template <typename T, bool PACKED>
-__device__ __forceinline__ DzIn<T, PACKED> dz_load(const DzJob& j, int64_t r, int64_t c,
-                                                   int have) {
-  const DzArgs& a = j.a;
-  DzIn<T, PACKED> in;
-  in.g = load_raw8<T>(reinterpret_cast<const T*>(a.dy) + r * a.lddy + c, j.vdy, have);
-  if (a.act != QRBL_ACT_NONE) {
-    if constexpr (PACKED) {
-      in.q = load_codes(a.z_codes + r * a.n + c, j.vz, have);
-      in.e = have > 0 ? a.z_exps[r * j.nblk + c / kBlk] : 0;
-    } else {
-      in.z = load_raw8<T>(reinterpret_cast<const T*>(a.z) + r * a.ldz + c, j.vz, have);
-    }
-  }
-  return in;
-}
-
 template <typename T, bool PACKED, bool PLANES>
 __device__ __forceinline__ void dz_block(const DzJob& j, int64_t block, float (*sums)[256]) {
   constexpr int V = 8, D = sizeof(T) == 4 ? 1 : 2;  // rows loaded together
   const DzArgs& a = j.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t by = block / j.nx, bx = block - by * j.nx;
+  const int64_t by = (uint32_t)block / (uint32_t)j.nx, bx = (uint32_t)block % (uint32_t)j.nx;
   const int64_t c = (bx * 32 + lane) * V;
   const int64_t rb = by * j.rows;
   const int64_t rend = rb + j.rows < a.m ? rb + j.rows : a.m;
@@ -340,47 +310,86 @@ __device__ __forceinline__ void dz_block(const DzJob& j, int64_t block, float (*
   if (any) {
     dz_rows_any<T, PACKED, PLANES>(j, bx * 256, rb, rend, acc);
   } else if (valid > 0) {
-    DzIn<T, PACKED> cur[D], nxt[D];
-    auto load = [&](DzIn<T, PACKED>(&to)[D], int64_t r0) {
-#pragma unroll
-      for (int k = 0; k < D; ++k)
-        to[k] = dz_load<T, PACKED>(j, r0 + 8 * k, c, r0 + 8 * k < rend ? valid : 0);
-    };
-    load(cur, rb + warp);
-    for (int64_t r0 = rb + warp; r0 < rend; r0 += 8 * D) {
-      load(nxt, r0 + 8 * D);
+    f2 sum[4] = {0, 0, 0, 0};
+    // this lane's values of its first row, and the step to the warp's next
+    const int64_t r0 = rb + warp;
+    const T* pg = reinterpret_cast<const T*>(a.dy) + r0 * a.lddy + c;
+    const T* pz = reinterpret_cast<const T*>(a.z) + (PACKED ? 0 : r0 * a.ldz + c);
+    const int8_t* pq = a.z_codes + (PACKED ? r0 * a.n + c : 0);
+    const int8_t* pe = a.z_exps + (PACKED ? r0 * j.nblk + c / kBlk : 0);
+    T* pd = reinterpret_cast<T*>(a.dst);
+    if constexpr (PLANES)
+      pd = reinterpret_cast<T*>(reinterpret_cast<bf16*>(a.dst) + r0 * a.ldd + c);
+    else
+      pd += r0 * a.ldd + c;
+    const int64_t sg = 8 * a.lddy, sz = 8 * a.ldz, sq = 8 * a.n, se = 8 * j.nblk, sd = 8 * a.ldd;
+    for (int left = (int)(rend - r0); left > 0; left -= 8 * D) {
+      Raw8<T> g[D], z[D];
+      uint2 q[D];
+      int e[D];
 #pragma unroll
       for (int k = 0; k < D; ++k) {
-        const int64_t r = r0 + 8 * k;
-        if (r >= rend) break;
-        float d[V];
-        values8<T>(cur[k].g, d);
+        const int have = left > 8 * k ? valid : 0;
+        g[k] = load_raw8<T>(pg + k * sg, true, have);
         if (a.act != QRBL_ACT_NONE) {
-          float f[V];
-          if constexpr (PACKED)
-            decode8(cur[k].q, pow2f(cur[k].e), f);
-          else
-            values8<T>(cur[k].z, f);
-          act_grad_by(d, f, a.act);
+          if constexpr (PACKED) {
+            q[k] = load_codes(pq + k * sq, true, have);
+            e[k] = have > 0 ? pe[k * se] : 0;
+          } else {
+            z[k] = load_raw8<T>(pz + k * sz, true, have);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < D; ++k) {
+        if (left <= 8 * k) break;
+        float f[V];
+        f2 d[4];
+        values8<T>(g[k], f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = f2_of(f[2 * i], f[2 * i + 1]);
+        if (a.act != QRBL_ACT_NONE) {
+          f2 zv[4];
+          if constexpr (PACKED) {
+            decode8(q[k], pow2f(e[k]), zv);
+          } else {
+            values8<T>(z[k], f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) zv[i] = f2_of(f[2 * i], f[2 * i + 1]);
+          }
+          act_grad_by(d, zv, a.act);
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += d[i];
+        for (int i = 0; i < 4; ++i) sum[i] = add2(sum[i], d[i]);
         if (a.dst == nullptr) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f2_to(d[i], f[2 * i], f[2 * i + 1]);
         if constexpr (PLANES) {
-          bf16* out = reinterpret_cast<bf16*>(a.dst) + r * a.ldd + c;
+          bf16* out = reinterpret_cast<bf16*>(pd) + k * sd;
           Vec<bf16, V> p[3];
 #pragma unroll
-          for (int i = 0; i < V; ++i) split3(d[i], p[0].v[i], p[1].v[i], p[2].v[i]);
+          for (int i = 0; i < V; ++i) split3(f[i], p[0].v[i], p[1].v[i], p[2].v[i]);
 #pragma unroll
           for (int i = 0; i < 3; ++i)
             *reinterpret_cast<Vec<bf16, V>*>(out + i * a.plane) = p[i];
         } else {
-          store_n<T, V>(reinterpret_cast<T*>(a.dst) + r * a.ldd + c, j.vdst, valid, d);
+          store_n<T, V>(pd + k * sd, true, valid, f);
         }
       }
-#pragma unroll
-      for (int k = 0; k < D; ++k) cur[k] = nxt[k];
+      pg += D * sg;
+      if constexpr (PACKED) {
+        pq += D * sq;
+        pe += D * se;
+      } else {
+        pz += D * sz;
+      }
+      if constexpr (PLANES)
+        pd = reinterpret_cast<T*>(reinterpret_cast<bf16*>(pd) + D * sd);
+      else
+        pd += D * sd;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f2_to(sum[i], acc[2 * i], acc[2 * i + 1]);
   }
   if (a.part == nullptr) return;
 #pragma unroll
@@ -402,7 +411,7 @@ struct PrepArgs {
   StageJob st[2];
 };
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) k_prepare(const __grid_constant__ PrepArgs p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4) k_prepare(const __grid_constant__ PrepArgs p) {
   constexpr bool PLANES = sizeof(T) == 4;
   __shared__ float sums[8][256];
   int64_t b = blockIdx.x;

@@ -113,6 +113,16 @@ __device__ __forceinline__ void values2(uint32_t w, float& lo, float& hi) {
   }
 }
 template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+  if constexpr (__is_same(T, bf16)) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <typename T>
 __device__ __forceinline__ void values8(const Raw8<T>& r, float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -274,16 +284,20 @@ __device__ __forceinline__ void act_n(float (&v)[N]) {
     for (int i = 0; i < N; i += 2) f2_to(act2<ACT>(f2_of(v[i], v[i + 1])), v[i], v[i + 1]);
   }
 }
-template <int ACT, int N>
-__device__ __forceinline__ void act_grad_n(float (&d)[N], const float (&z)[N]) {
+template <int ACT>
+__device__ __forceinline__ f2 slope2(f2 z) {
   if constexpr (ACT == QRBL_ACT_RELU) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) d[i] *= z[i] > 0.f ? 1.f : (z[i] <= 0.f ? 0.f : z[i]);
+    float a, b;
+    f2_to(z, a, b);
+    return f2_of(a > 0.f ? 1.f : (a <= 0.f ? 0.f : a), b > 0.f ? 1.f : (b <= 0.f ? 0.f : b));
   } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 2)
-      f2_to(mul2(f2_of(d[i], d[i + 1]), act_grad2<ACT>(f2_of(z[i], z[i + 1]))), d[i], d[i + 1]);
+    return act_grad2<ACT>(z);
   }
+}
+template <int ACT, int N>
+__device__ __forceinline__ void act_grad_n(f2 (&d)[N], const f2 (&z)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) d[i] = mul2(d[i], slope2<ACT>(z[i]));
 }
 template <int N>
 __device__ __forceinline__ void act_by(float (&v)[N], int act) {
@@ -296,7 +310,7 @@ __device__ __forceinline__ void act_by(float (&v)[N], int act) {
   }
 }
 template <int N>
-__device__ __forceinline__ void act_grad_by(float (&d)[N], const float (&z)[N], int act) {
+__device__ __forceinline__ void act_grad_by(f2 (&d)[N], const f2 (&z)[N], int act) {
   switch (act) {
     case QRBL_ACT_RELU: act_grad_n<QRBL_ACT_RELU>(d, z); break;
     case QRBL_ACT_GELU: act_grad_n<QRBL_ACT_GELU>(d, z); break;
@@ -378,20 +392,29 @@ __device__ __forceinline__ float finite_amax(const float (&v)[N]) {
 __device__ __forceinline__ float value_of(int code, float step) {
   return code == kNanCode ? __uint_as_float(0x7fc00000u) : (float)code * step;
 }
-// Four codes as values. A byte q + 128 put under the exponent of 2^23 is the
-// float 2^23 + 128 + q; kNanCode (byte 0 after the flip) becomes NaN.
-__device__ __forceinline__ void decode4(uint32_t codes, float step, float (&out)[4]) {
-  const uint32_t y = codes ^ 0x80808080u;
+// Eight codes as values, two to a register pair. A byte q + 128 put under the
+// exponent of 2^23 is the float 2^23 + 128 + q; kNanCode (byte 0 after the
+// flip) becomes NaN.
+__device__ __forceinline__ void decode8(uint2 q, float step, f2 (&out)[4]) {
+  const uint32_t y[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
   const f2 off = f2_of(-8388736.f), st = f2_of(step);
 #pragma unroll
-  for (int i = 0; i < 4; i += 2)
-    f2_to(mul2(add2(f2_of(__uint_as_float(__byte_perm(y, 0x4b000000u, 0x7540 + i)),
-                          __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7541 + i))),
-                    off), st), out[i], out[i + 1]);
-  if ((y - 0x01010101u) & ~y & 0x80808080u) {
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = y[i / 2], at = 2 * (i & 1);
+    out[i] = mul2(add2(f2_of(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + at)),
+                             __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7541 + at))),
+                       off), st);
+  }
+  if ((((y[0] - 0x01010101u) & ~y[0]) | ((y[1] - 0x01010101u) & ~y[1])) & 0x80808080u) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (((y >> (8 * i)) & 255u) == 0) out[i] = __uint_as_float(0x7fc00000u);
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      f2_to(out[i], a, b);
+      const uint32_t w = y[i / 2] >> (16 * (i & 1));
+      if ((w & 255u) == 0) a = __uint_as_float(0x7fc00000u);
+      if ((w & 0xff00u) == 0) b = __uint_as_float(0x7fc00000u);
+      out[i] = f2_of(a, b);
+    }
   }
 }
 

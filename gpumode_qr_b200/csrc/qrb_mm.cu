@@ -317,16 +317,6 @@ __device__ __forceinline__ uint32_t staged_at(uint32_t buf, int row, int unit) {
                             : (ROWB == 64 ? unit ^ ((row >> 1) & 3) : unit ^ ((row >> 2) & 1));
   return buf + row * ROWB + x * 16;
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pair_of(float a, float b) {
-  if constexpr (__is_same(T, bf16)) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
 // 32 values of the lane's row from column `first` of the block.
 template <typename E, uint32_t ROWB>
 __device__ __forceinline__ void stage_write(uint32_t buf, int first, const float (&v)[32]) {
