@@ -123,7 +123,7 @@ Forward plan_forward(const qrbl_linear_args& a, Carve* c) {
   f.size.m = a.m; f.size.n = a.n; f.size.k = a.k;
   f.size.epilogue = (a.activation > QRBL_ACT_RELU ? 1 : 0) |
                     (a.z != nullptr || a.z_codes != nullptr ? 2 : 0) |
-                    (a.residual != nullptr ? 4 : 0);
+                    (a.residual != nullptr ? 4 : 0) | (a.z_codes != nullptr ? 8 : 0);
   f.plan = plan_products(a.dtype, &f.size, 1);
   f.part = reinterpret_cast<float*>(c->take(f.plan.part_bytes[0]));
   return f;

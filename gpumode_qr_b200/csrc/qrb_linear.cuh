@@ -471,7 +471,8 @@ enum ProductKind { kForward = 0, kGradIn = 1, kGradW = 2 };
 
 struct ProductSize {
   int64_t m = 0, n = 0, k = 0;
-  int epilogue = 0;  // extra work per value: 1 activation, 2 kept z, 4 residual
+  int epilogue = 0;  // extra work per value: 1 activation, 2 kept z, 4 residual;
+                     // 8: chains summed in FP32 (z kept in 8 bits)
 };
 struct Product {
   int kind = kForward;

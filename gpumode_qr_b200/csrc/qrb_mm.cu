@@ -23,9 +23,12 @@
 // holds all three planes of both operands, and the six products a_i b_j with
 // i + j <= 2 are formed from it: the main product a0 b0 in one accumulator, the
 // five small ones in another. The tensor core does not round to nearest at
-// every add, so a chain over the whole reduction would drift: every kChain
+// every add, so a chain over the whole reduction would drift: every CHAIN
 // stages (a unit) the two accumulators are read and added to FP32 sums in
-// registers.
+// registers. A 16-bit forward product whose z is kept in 8 bits sums its chains
+// the same way (SUM): its other results are rounded far above the drift, but a
+// code near a border shows it (4 times fewer codes differ from the exact ones
+// at k = 4096).
 //
 // A reduction split over several CTAs (few tiles, long k) writes FP32 partial
 // tiles that k_join adds in order: no atomics, the same bits every time.
@@ -55,12 +58,12 @@ constexpr int kPitch = 33;              // words of a row in a warp's turned blo
 
 // control block at the start of shared memory
 constexpr int B_FULL = 0, B_EMPTY = kMaxStages, B_ACCFULL = 2 * kMaxStages,
-              B_ACCEMPTY = B_ACCFULL + 2, B_FIN = B_ACCEMPTY + 2, B_RES = B_FIN + 1,
+              B_ACCEMPTY = B_ACCFULL + 4, B_FIN = B_ACCEMPTY + 4, B_RES = B_FIN + 1,
               NBAR = B_RES + 2 * kEpiWarps;
 constexpr uint32_t OFF_TMEM = NBAR * 8, OFF_ABORT = OFF_TMEM + 4, CTRL = 1024;
 static_assert(OFF_ABORT + 4 <= CTRL, "control block");
 
-template <int CG, int BN, typename T>
+template <int CG, int BN, typename T, bool SUM>
 struct Lay {
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // planes
   static constexpr int BK = NP == 3 ? 32 : 64;       // reduction values per stage
@@ -87,7 +90,10 @@ struct Lay {
   static_assert(TROWS * kPitch * 4 <= (int)WBUF && (ROWB == 64 || ROWB == 128), "staging");
   static_assert(A % 1024 == 0 && B % 1024 == 0, "swizzle atoms");
   static constexpr int ACC = NP == 3 ? 2 * BN : BN;  // TMEM columns per buffer
-  static constexpr int TMEM = 2 * ACC;
+  // accumulator buffers (SUM: as many as fit, so that the MMAs of the next tile's
+  // chains run while this tile's epilogue does)
+  static constexpr int NACC = SUM && NP == 1 ? 4 : 2;
+  static constexpr int TMEM = NACC * ACC;
   static_assert(ST >= 2 && TMEM <= 512 && TMEM >= 32, "stage ring and TMEM");
   static_assert(BROWS % 64 == 0, "MN-major atoms");
 };
@@ -508,7 +514,57 @@ __device__ __forceinline__ int pack32(uint32_t buf, int first, const float (&v)[
   return ex;
 }
 
-template <int CG, int BN, typename T, bool FWD>
+// 64 consecutive TMEM columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+      :
+        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]),
+        "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
+        "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]),
+        "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
+        "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+// sum <- sum + the N columns at t (first: <- them).
+template <int N>
+__device__ __forceinline__ void drain(uint32_t t, float (&sum)[N], bool first) {
+  float v[N];
+  if constexpr (N == 64)
+    tmem_ld64(t, v);
+  else
+    tc::tmem_ld32(t, v);
+  if (first) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      f2_to(add2(f2_of(sum[i], sum[i + 1]), f2_of(v[i], v[i + 1])), sum[i], sum[i + 1]);
+  }
+}
+
+template <int CG, int BN, typename T, bool FWD, bool SUM>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
               const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
@@ -516,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_z,
               const __grid_constant__ CUtensorMap map_q,
               const __grid_constant__ Args a) {
-  using L = Lay<CG, BN, T>;
+  using L = Lay<CG, BN, T, SUM>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = tma::smem_addr(smem_raw);
   const uint32_t pad = (1024 - (raw & 1023)) & 1023;
@@ -544,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma::mbar_init(BAR(B_FULL + s), 1);
       tma::mbar_init(BAR(B_EMPTY + s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < L::NACC; ++b) {
       tma::mbar_init(BAR(B_ACCFULL + b), 1);
       tma::mbar_init(BAR(B_ACCEMPTY + b), CG * kEpiWarps);
     }
@@ -616,10 +672,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t da0 = operand_desc<L>(ring, amn);
         const uint64_t db0 = operand_desc<L>(ring + L::NP * L::A, bmn);
         for (int kb = it.kb0; live && kb < it.kb1;) {
-          const int end = L::NP == 3 && kb + L::CHAIN < it.kb1 ? kb + L::CHAIN : it.kb1;
-          const int buf = unit & 1;
-          if (unit >= 2)
-            live = warp_wait(BAR(B_ACCEMPTY + buf), (uint32_t)((unit / 2 - 1) & 1), a.limit,
+          const int end = SUM && kb + L::CHAIN < it.kb1 ? kb + L::CHAIN : it.kb1;
+          const int buf = unit % L::NACC;
+          if (unit >= L::NACC)
+            live = warp_wait(BAR(B_ACCEMPTY + buf), (uint32_t)((unit / L::NACC - 1) & 1), a.limit,
                              s_abort);
           tc::fence_after();
           const uint32_t d = tmem + buf * L::ACC;
@@ -850,9 +906,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
 
-      if constexpr (L::NP == 1) {
-        const int buf = unit & 1;
-        live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
+      if constexpr (!SUM) {
+        const int buf = unit % L::NACC;
+        live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / L::NACC) & 1), a.limit, s_abort);
         if (!live) break;
         tc::fence_after();
         const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
@@ -865,25 +921,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++unit;
       } else {
-        float sum[HC / 32][32];
-#pragma unroll
-        for (int c = 0; c < HC / 32; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
+        float sum[HC];
         for (int kb = it.kb0; kb < it.kb1; kb += L::CHAIN, ++unit) {
-          const int buf = unit & 1;
-          live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / 2) & 1), a.limit, s_abort);
+          const int buf = unit % L::NACC;
+          live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / L::NACC) & 1), a.limit,
+                           s_abort);
           if (!live) break;
           tc::fence_after();
           const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
-#pragma unroll
-          for (int c = 0; c < HC / 32; ++c) {
-            float v[32], w[32];
-            tc::tmem_ld32(t + c * 32, v);
-            tc::tmem_ld32(t + BN + c * 32, w);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sum[c][i] += v[i] + w[i];
-          }
+          drain(t, sum, kb == it.kb0);
+          if constexpr (L::NP == 3) drain(t + BN, sum, false);
           hand_back(buf);
         }
         if (!live) break;
@@ -891,7 +938,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < HC / 32; ++c) {
           float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = HC == 32 || c == 0 ? sum[0][i] : sum[HC / 32 - 1][i];
+          for (int i = 0; i < 32; ++i) v[i] = HC == 32 || c == 0 ? sum[i] : sum[HC - 32 + i];
           finish(v, 32 * c);
         }
       }
@@ -981,15 +1028,15 @@ const Device* device_info() {
 }
 
 // The kernel for both (or one of the) products, or for a forward product.
-template <int CG, int BN, typename T, bool FWD>
+template <int CG, int BN, typename T, bool FWD, bool SUM>
 int launch_t(const Product* const* q, int count, Args& args, const Device& d, cudaStream_t s) {
-  using L = Lay<CG, BN, T>;
+  using L = Lay<CG, BN, T, SUM>;
   static std::once_flag once[64];
   static bool ready[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QRB_ERR_DEVICE;
   std::call_once(once[dev], [dev] {
-    ready[dev] = cudaFuncSetAttribute(k_product<CG, BN, T, FWD>,
+    ready[dev] = cudaFuncSetAttribute(k_product<CG, BN, T, FWD, SUM>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)L::SMEM) == cudaSuccess;
   });
@@ -1026,7 +1073,7 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
       return QRB_ERR_UNSUPPORTED;
   }
   if constexpr (CG == 1) {
-    k_product<CG, BN, T, FWD><<<args.s.workers, kThreads, L::SMEM, s>>>(
+    k_product<CG, BN, T, FWD, SUM><<<args.s.workers, kThreads, L::SMEM, s>>>(
         ma[0], mb[0], ma[1], mb[1], mo[0], mo[1], mr, mz, mq, args);
   } else {
     cudaLaunchConfig_t lc = {};
@@ -1041,7 +1088,7 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
     lc.stream = s;
     lc.attrs = la;
     lc.numAttrs = 1;
-    if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD>, ma[0], mb[0], ma[1], mb[1], mo[0],
+    if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD, SUM>, ma[0], mb[0], ma[1], mb[1], mo[0],
                            mo[1], mr, mz, mq, args) != cudaSuccess) {
       (void)cudaGetLastError();
       return QRB_ERR_LAUNCH;
@@ -1053,20 +1100,24 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
 }
 
 template <int CG, int BN, typename T>
-int launch_dir(bool fwd, const Product* const* q, int count, Args& args, const Device& d,
+int launch_dir(bool fwd, bool sum, const Product* const* q, int count, Args& args, const Device& d,
                cudaStream_t s) {
-  return fwd ? launch_t<CG, BN, T, true>(q, count, args, d, s)
-             : launch_t<CG, BN, T, false>(q, count, args, d, s);
+  constexpr bool F32 = sizeof(T) == 4;
+  if (!fwd) return launch_t<CG, BN, T, false, F32>(q, count, args, d, s);
+  if constexpr (!F32 && BN <= 128) {
+    if (sum) return launch_t<CG, BN, T, true, true>(q, count, args, d, s);
+  }
+  return launch_t<CG, BN, T, true, F32>(q, count, args, d, s);
 }
 
 template <typename T>
-int launch_type(int cg, int bn, bool fwd, const Product* const* q, int count, Args& args,
-                const Device& d, cudaStream_t s) {
-  if (cg == 1 && bn == 64) return launch_dir<1, 64, T>(fwd, q, count, args, d, s);
-  if (cg == 1 && bn == 128) return launch_dir<1, 128, T>(fwd, q, count, args, d, s);
-  if (cg == 2 && bn == 128) return launch_dir<2, 128, T>(fwd, q, count, args, d, s);
+int launch_type(int cg, int bn, bool fwd, bool sum, const Product* const* q, int count,
+                Args& args, const Device& d, cudaStream_t s) {
+  if (cg == 1 && bn == 64) return launch_dir<1, 64, T>(fwd, sum, q, count, args, d, s);
+  if (cg == 1 && bn == 128) return launch_dir<1, 128, T>(fwd, sum, q, count, args, d, s);
+  if (cg == 2 && bn == 128) return launch_dir<2, 128, T>(fwd, sum, q, count, args, d, s);
   if constexpr (sizeof(T) == 2) {
-    if (cg == 2 && bn == 256) return launch_dir<2, 256, T>(fwd, q, count, args, d, s);
+    if (cg == 2 && bn == 256) return launch_dir<2, 256, T>(fwd, sum, q, count, args, d, s);
   }
   return QRB_ERR_INVALID_ARG;
 }
@@ -1130,7 +1181,7 @@ double make_schedule(const int64_t* items, const double* each, int64_t most, Sch
   return length;
 }
 
-int stage_values(bool f32) { return f32 ? Lay<1, 64, float>::BK : Lay<1, 64, bf16>::BK; }
+int stage_values(bool f32) { return f32 ? Lay<1, 64, float, true>::BK : Lay<1, 64, bf16, false>::BK; }
 
 Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, const Cut& c, int bk, int splits) {
   Problem p = {};
@@ -1166,6 +1217,7 @@ static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
     // (a cut that FP32 does not have: its widest)
     if (hook_cut != 0 && hook_cut != 1000 * c.cg + c.bn && !(f32 && hook_cut == 2256 && ci == 0))
       continue;
+    if (c.bn > 128 && (sizes[0].epilogue & 8)) continue;  // no registers for its sums
     const int64_t workers = sms / c.cg;
     int64_t tiles[2] = {0, 0}, kb[2] = {1, 1};
     for (int i = 0; i < count; ++i) {
@@ -1251,7 +1303,7 @@ ProductPlan plan_products(int dtype, const ProductSize* sizes, int count) {
 }
 
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
-                    const ColSum* sum, cudaStream_t s) {
+                    const ColSum* cols, cudaStream_t s) {
   const Device* d = device_info();
   if (d == nullptr) return QRB_ERR_DEVICE;
   if (!plan.ok) return QRB_ERR_UNSUPPORTED;
@@ -1283,16 +1335,17 @@ int launch_products(int dtype, const Product* products, int count, const Product
                   .longer();
   }
   make_schedule(items, each, d->sms / c.cg, &args.s);
-  if (sum != nullptr) args.sum = *sum;
+  if (cols != nullptr) args.sum = *cols;
   args.err = d->err;
   args.limit = device_wait_limit();
   args.skip_mma = test_skip_mma() ? 1 : 0;
   const bool fwd = products[0].kind == kForward;
+  const bool sum = (products[0].size.epilogue & 8) != 0;
   int rc = QRB_ERR_INVALID_ARG;
   switch (dtype) {
-    case QRBL_F32: rc = launch_type<float>(c.cg, c.bn, fwd, q, count, args, *d, s); break;
-    case QRBL_F16: rc = launch_type<f16>(c.cg, c.bn, fwd, q, count, args, *d, s); break;
-    case QRBL_BF16: rc = launch_type<bf16>(c.cg, c.bn, fwd, q, count, args, *d, s); break;
+    case QRBL_F32: rc = launch_type<float>(c.cg, c.bn, fwd, sum, q, count, args, *d, s); break;
+    case QRBL_F16: rc = launch_type<f16>(c.cg, c.bn, fwd, sum, q, count, args, *d, s); break;
+    case QRBL_BF16: rc = launch_type<bf16>(c.cg, c.bn, fwd, sum, q, count, args, *d, s); break;
   }
   for (int i = 0; i < count && rc == QRB_OK; ++i)
     if (plan.splits[i] > 1)

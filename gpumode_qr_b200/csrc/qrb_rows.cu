@@ -118,17 +118,22 @@ __global__ void __launch_bounds__(kWarps * 32)
         b[u][q] = load8(x + (int64_t)tok * ldx + c, vx, tok < m ? have : 0);
       }
     }
+    // (short chains, added in FP32: the tensor core does not round its adds)
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int r = 0; r < RG; ++r)
 #pragma unroll
-      for (int r = 0; r < RG; ++r)
+      for (int q = 0; q < NT; ++q) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int q = 0; q < NT; ++q) {
-          mma16<T>(d[r][q], a[u][r][0].x, a[u][r][1].x, a[u][r][0].y, a[u][r][1].y, b[u][q].x,
+        for (int u = 0; u < U; ++u) {
+          mma16<T>(s, a[u][r][0].x, a[u][r][1].x, a[u][r][0].y, a[u][r][1].y, b[u][q].x,
                    b[u][q].y);
-          mma16<T>(d[r][q], a[u][r][0].z, a[u][r][1].z, a[u][r][0].w, a[u][r][1].w, b[u][q].z,
+          mma16<T>(s, a[u][r][0].z, a[u][r][1].z, a[u][r][0].w, a[u][r][1].w, b[u][q].z,
                    b[u][q].w);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[r][q][i] += s[i];
+      }
   }
 #pragma unroll
   for (int r = 0; r < RG; ++r)
