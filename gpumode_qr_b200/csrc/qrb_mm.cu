@@ -1211,13 +1211,13 @@ static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
   double least = -1;
   const Cut* cuts = f32 ? kCuts32 : kCuts16;
   const int ncuts = f32 ? 3 : 4;
-  const int hook_cut = linear_cut(), hook_splits = linear_splits();
+  const bool chains = f32 || (sizes[0].epilogue & 8) != 0;
+  const int hook_splits = linear_splits();
+  const int hook_cut = chains && linear_cut() == 2256 ? 2128 : linear_cut();
   for (int ci = 0; ci < ncuts; ++ci) {
     const Cut c = cuts[ci];
-    // (a cut that FP32 does not have: its widest)
-    if (hook_cut != 0 && hook_cut != 1000 * c.cg + c.bn && !(f32 && hook_cut == 2256 && ci == 0))
-      continue;
-    if (c.bn > 128 && (sizes[0].epilogue & 8)) continue;  // no registers for its sums
+    if (c.bn > 128 && chains) continue;  // no registers for its sums
+    if (hook_cut != 0 && hook_cut != 1000 * c.cg + c.bn) continue;
     const int64_t workers = sms / c.cg;
     int64_t tiles[2] = {0, 0}, kb[2] = {1, 1};
     for (int i = 0; i < count; ++i) {

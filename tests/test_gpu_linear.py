@@ -480,6 +480,84 @@ def test_offsets_beyond_32_bits():
 
 
 # ---------------------------------------------------------------------------
+# every way a product is cut
+# ---------------------------------------------------------------------------
+@pytest.fixture
+def hooks():
+    names = ("linear_cut", "linear_splits", "linear_rows")
+    old = {k: _lib.get_config(k) for k in names}
+    yield _lib.set_config
+    for k, v in old.items():
+        _lib.set_config(k, v)
+
+
+CUTS = [2256, 2128, 1128, 1064]
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("splits", [0, 3])
+@pytest.mark.parametrize("cut", CUTS)
+def test_forward_cuts(cut, splits, dt, hooks):
+    hooks("linear_cut", cut)
+    hooks("linear_splits", splits)
+    hooks("linear_rows", 0)
+    # edges of the tiles, more tiles than SMs, aligned and unaligned rows
+    for m, n, k in ((1, 40, 200), (257, 520, 200), (130, 264, 72), (131, 77, 45), (40, 24, 1000),
+                    (3000, 1064, 96), (600, 333, 520)):
+        x, w = rnd((m, k), 170, dt), rnd((n, k), 171, dt, k**-0.5)
+        b, r = rnd((n,), 172, dt), rnd((m, n), 173, dt)
+        y, z = api.linear(x, w, b, r, "silu", keep="plain")
+        check_forward(x, w, b, r, "silu", y, z)
+        check_forward(x, w, None, r, "none", api.linear(x, w, None, r))
+        y, p = api.linear(x, w, b, r, "gelu_tanh", keep="packed")
+        z64, za = check_forward(x, w, b, r, "gelu_tanh", y)
+        s = torch.ldexp(torch.ones(p.exponents.shape, dtype=torch.float64, device=DEV), p.exponents.int())
+        near(api.unpack_activation(p), z64, 0.5 * s.repeat_interleave(32, dim=1)[:, :n] + za, "packed z")
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("splits", [0, 3])
+@pytest.mark.parametrize("cut", CUTS)
+def test_backward_cuts(cut, splits, dt, hooks):
+    hooks("linear_cut", cut)
+    hooks("linear_splits", splits)
+    # either product the longer one; more tiles than SMs in one or both
+    for m, n, k in ((257, 136, 520), (1, 40, 24), (1000, 64, 1032), (64, 1000, 1032), (131, 77, 45),
+                    (2500, 1100, 1300)):
+        dy, x, w, z = (rnd((m, n), 174, dt), rnd((m, k), 175, dt), rnd((n, k), 176, dt, n**-0.5),
+                       rnd((m, n), 177, dt))
+        check_backward(dy, x.double(), w, z.double(), "silu", *api.linear_backward(dy, x, w, z, "silu"))
+        check_backward(dy, x.double(), w, None, "none", *api.linear_backward(dy, x, w))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_few_rows_and_tiles_agree(dt, hooks):
+    m = 8 if dt == FP else 32
+    for n, k in ((100, 72), (4096, 512), (33, 1000)):
+        x, w = rnd((m, k), 178, dt), rnd((n, k), 179, dt, k**-0.5)
+        b, r = rnd((n,), 180, dt), rnd((m, n), 181, dt)
+        for rows in (m, 0):
+            hooks("linear_rows", rows)
+            check_forward(x, w, b, r, "gelu", api.linear(x, w, b, r, "gelu"))
+
+
+def test_z_kept_both_ways():
+    # the C entry point may ask for z plain and packed at once
+    for m, n, k in ((200, 160, 96), (4, 64, 64)):
+        x, w = rnd((m, k), 182, BF), rnd((n, k), 183, BF, 0.1)
+        y0, z0 = api.linear(x, w, None, None, "silu", keep="plain")
+        y, z = torch.empty_like(y0), torch.empty_like(z0)
+        p = layers._empty_packed((m, n), x)
+        a = layers._linear_args(2, 4, m, n, k, x.data_ptr(), k, w.data_ptr(), k, 0, 0, 0,
+                                y.data_ptr(), n, z.data_ptr(), n, p.codes.data_ptr(),
+                                p.exponents.data_ptr())
+        assert _lib.lib().qrbl_linear(a, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+        z64, za = check_forward(x, w, None, None, "silu", y, z)
+        s = torch.ldexp(torch.ones(p.exponents.shape, dtype=torch.float64, device=DEV), p.exponents.int())
+        near(api.unpack_activation(p), z64, 0.5 * s.repeat_interleave(32, dim=1) + za, "packed z")
+
+
+# ---------------------------------------------------------------------------
 # together, streams, graphs, refusals
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("kept", ["plain", "packed"])

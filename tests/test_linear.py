@@ -164,3 +164,16 @@ def test_injected_failure_enqueues_nothing():
     _lib.set_config("fail_next", 1)
     assert _lib.lib().qrbl_linear_backward(_bwd(), None, 0, None) == 6
     assert _lib.get_config("fail_next") == 0
+
+
+@pytest.mark.parametrize("key,good,bad", [("linear_cut", (2256, 2128, 1128, 1064, 0), (1, 1256, -1)),
+                                          ("linear_splits", (1, 16, 0), (17, -1)),
+                                          ("linear_rows", (0, 32, -1), (33, -2))])
+def test_hooks(key, good, bad):
+    for v in good:
+        _lib.set_config(key, v)
+        assert _lib.get_config(key) == v
+    for v in bad:
+        with pytest.raises(_lib.QRBError):
+            _lib.set_config(key, v)
+    assert _lib.get_config(key) == good[-1]
