@@ -414,6 +414,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4) k_prepare(const __grid_constant__ PrepArgs p) {
   constexpr bool PLANES = sizeof(T) == 4;
   __shared__ float sums[8][256];
+  let_next_start();
   int64_t b = blockIdx.x;
   if (b < p.dz.blocks) {
     if (p.dz.a.z_codes != nullptr)
@@ -446,6 +447,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_join(const float* __restrict__ part, int splits, int64_t rows, int64_t ld, int64_t m,
            int64_t n, Epilogue e) {
+  wait_for_previous();
   const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * 4;
   const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int valid = r < m && c < n ? (int)(n - c < 4 ? n - c : 4) : 0;
@@ -573,14 +575,23 @@ int prepare_t(const Prepare& p, cudaStream_t s) {
 
 template <typename T>
 int join_t(const float* part, int splits, int64_t rows, int64_t ld, int64_t m, int64_t n,
-           const Epilogue& e, cudaStream_t s) {
+           const Epilogue& e, bool after_product, cudaStream_t s) {
   int tx = 8;  // a packed block stays within one warp
   while (tx * 4 < n && tx < kThreads) tx *= 2;
   const int ty = kThreads / tx;
   const int64_t gx = (m + ty - 1) / ty, gy = (n + 4 * tx - 1) / (4 * tx);
   if (gx > 0x7fffffffLL || gy > 65535) return QRB_ERR_UNSUPPORTED;
-  k_join<T><<<dim3((unsigned)gx, (unsigned)gy), dim3((unsigned)tx, (unsigned)ty), 0, s>>>(
-      part, splits, rows, ld, m, n, e);
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute early = early_start();
+  lc.gridDim = dim3((unsigned)gx, (unsigned)gy);
+  lc.blockDim = dim3((unsigned)tx, (unsigned)ty);
+  lc.stream = s;
+  lc.attrs = &early;
+  lc.numAttrs = after_product ? 1 : 0;
+  if (cudaLaunchKernelEx(&lc, k_join<T>, part, splits, rows, ld, m, n, e) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return QRB_ERR_LAUNCH;
+  }
   return launched();
 }
 
@@ -626,8 +637,8 @@ int launch_colsum(int dtype, const ColSum& c, cudaStream_t s) {
 }
 
 int launch_join(int dtype, const float* part, int splits, int64_t rows, int64_t ld, int64_t m,
-                int64_t n, const Epilogue& e, cudaStream_t s) {
-  QRBL_BY_TYPE(dtype, return join_t<T>(part, splits, rows, ld, m, n, e, s));
+                int64_t n, const Epilogue& e, bool after_product, cudaStream_t s) {
+  QRBL_BY_TYPE(dtype, return join_t<T>(part, splits, rows, ld, m, n, e, after_product, s));
 }
 
 }  // namespace lin

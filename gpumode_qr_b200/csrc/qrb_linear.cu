@@ -146,7 +146,7 @@ int forward(const qrbl_linear_args& a, void* workspace, size_t bytes, cudaStream
   };
   e.vec = rows16(a.y, a.ldy) && rows16(a.residual, a.ldr) && rows16(a.z, a.ldz) &&
           aligned16(a.bias);
-  if (a.k == 0) return launch_join(a.dtype, nullptr, 0, 0, 0, a.m, a.n, e, s);
+  if (a.k == 0) return launch_join(a.dtype, nullptr, 0, 0, 0, a.m, a.n, e, false, s);
   Carve c{reinterpret_cast<uint8_t*>(workspace)};
   const Forward f = plan_forward(a, &c);
   if (c.used > 0 && (workspace == nullptr || bytes < c.used)) return QRB_ERR_WORKSPACE;
@@ -162,7 +162,7 @@ int forward(const qrbl_linear_args& a, void* workspace, size_t bytes, cudaStream
   p.a = f.x; p.b = f.w;
   p.part = f.part;
   p.e = e;
-  return launch_products(a.dtype, &p, 1, f.plan, nullptr, s);
+  return launch_products(a.dtype, &p, 1, f.plan, nullptr, before.stages > 0, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -292,7 +292,8 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
   }
   if (b.stage_x) add_stage(&before, b.xs, b.x);
   if (b.stage_w) add_stage(&before, b.ws, b.w);
-  if ((before.has_dz || before.stages > 0) &&
+  const bool prepared = before.has_dz || before.stages > 0;
+  if (prepared &&
       (rc = launch_prepare(a.dtype, before, s)) != QRB_OK)
     return rc;
   ColSum sum;
@@ -323,7 +324,7 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
     p[j].size = b.size[j];
     p[j].part = b.part[j];
   }
-  if (i > 0) return launch_products(a.dtype, p, i, b.plan, b.db ? &sum : nullptr, s);
+  if (i > 0) return launch_products(a.dtype, p, i, b.plan, b.db ? &sum : nullptr, prepared, s);
   return b.db ? launch_colsum(a.dtype, sum, s) : QRB_OK;
 }
 

@@ -25,6 +25,24 @@ using f16 = __half;
 constexpr int kBlk = 32;         // values that share an exponent in the packed form
 constexpr int kNanCode = -128;
 
+// Programmatic dependent launch between the kernels of one call: the earlier one
+// lets the later one's blocks start (where an SM has room) once all of its own
+// have; the later one sets itself up and then waits for the earlier one's
+// results.
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// The attribute of a launch that may start before the one in front of it ends.
+inline cudaLaunchAttribute early_start() {
+  cudaLaunchAttribute a = {};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+
 // ---------------------------------------------------------------------------
 // element types
 // ---------------------------------------------------------------------------
@@ -493,18 +511,20 @@ struct ProductPlan {
 };
 struct ColSum;
 ProductPlan plan_products(int dtype, const ProductSize* sizes, int count);
-// sum (may be null): column sums finished in the same launch.
+// sum (may be null): column sums finished in the same launch. after_prepare: the
+// launch in front of it on the stream is this call's launch_prepare.
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
-                    const ColSum* sum, cudaStream_t s);
+                    const ColSum* sum, bool after_prepare, cudaStream_t s);
 // The forward product of m <= rows_most(dtype) rows, x and w read in place at
 // any alignment.
 int64_t rows_most(int dtype);
 int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
                 const Epilogue& e, cudaStream_t s);
 // out = epilogue(sum of `splits` partial sums), part[s][row][col] with rows
-// `rows` and row stride ld (splits may be 0).
+// `rows` and row stride ld (splits may be 0). after_product: the launch in front
+// of it on the stream is this call's k_product (or another join after it).
 int launch_join(int dtype, const float* part, int splits, int64_t rows, int64_t ld, int64_t m,
-                int64_t n, const Epilogue& e, cudaStream_t s);
+                int64_t n, const Epilogue& e, bool after_product, cudaStream_t s);
 
 int launch_pack(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols, int8_t* codes,
                 int8_t* exps, cudaStream_t s);
@@ -559,7 +579,7 @@ __device__ __forceinline__ void column_sum(const ColSum& c, int64_t first, int64
   for (int64_t col = first; col < c.n; col += step) {
     float s = 0.f;
 #pragma unroll 16
-    for (int64_t b = 0; b < c.blocks; ++b) s += __ldg(c.part + b * c.n + col);
+    for (int64_t b = 0; b < c.blocks; ++b) s += c.part[b * c.n + col];
     reinterpret_cast<T*>(c.out)[col] = from_f<T>(s);
   }
 }

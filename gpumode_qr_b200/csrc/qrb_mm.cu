@@ -615,6 +615,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if constexpr (CG == 2) sync_all<CG>();
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + OFF_TMEM);
+  let_next_start();     // k_join, of a split product
+  wait_for_previous();  // k_prepare, where there is one
 
   if (warp == kEpiWarps) {  // ---- loads ----
     int u = 0;  // stages issued
@@ -1029,7 +1031,7 @@ const Device* device_info() {
 
 // The kernel for both (or one of the) products, or for a forward product.
 template <int CG, int BN, typename T, bool FWD, bool SUM>
-int launch_t(const Product* const* q, int count, Args& args, const Device& d, cudaStream_t s) {
+int launch_t(const Product* const* q, int count, Args& args, bool after_prepare, cudaStream_t s) {
   using L = Lay<CG, BN, T, SUM>;
   static std::once_flag once[64];
   static bool ready[64] = {};
@@ -1072,52 +1074,50 @@ int launch_t(const Product* const* q, int count, Args& args, const Device& d, cu
         (p.e.z_codes != nullptr && !encode_staged(&mq, p.e.z_codes, 1, p.n, p.m, p.n, L::GW)))
       return QRB_ERR_UNSUPPORTED;
   }
-  if constexpr (CG == 1) {
-    k_product<CG, BN, T, FWD, SUM><<<args.s.workers, kThreads, L::SMEM, s>>>(
-        ma[0], mb[0], ma[1], mb[1], mo[0], mo[1], mr, mz, mq, args);
-  } else {
-    cudaLaunchConfig_t lc = {};
-    cudaLaunchAttribute la[1];
-    la[0].id = cudaLaunchAttributeClusterDimension;
-    la[0].val.clusterDim.x = 2;
-    la[0].val.clusterDim.y = 1;
-    la[0].val.clusterDim.z = 1;
-    lc.gridDim = dim3(2 * (unsigned)args.s.workers);
-    lc.blockDim = dim3(kThreads);
-    lc.dynamicSmemBytes = L::SMEM;
-    lc.stream = s;
-    lc.attrs = la;
-    lc.numAttrs = 1;
-    if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD, SUM>, ma[0], mb[0], ma[1], mb[1], mo[0],
-                           mo[1], mr, mz, mq, args) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return QRB_ERR_LAUNCH;
-    }
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute la[2];
+  int attrs = 0;
+  if (CG == 2) {
+    la[attrs].id = cudaLaunchAttributeClusterDimension;
+    la[attrs].val.clusterDim.x = 2;
+    la[attrs].val.clusterDim.y = 1;
+    la[attrs++].val.clusterDim.z = 1;
   }
-  (void)d;
+  if (after_prepare) la[attrs++] = early_start();
+  lc.gridDim = dim3(CG * (unsigned)args.s.workers);
+  lc.blockDim = dim3(kThreads);
+  lc.dynamicSmemBytes = L::SMEM;
+  lc.stream = s;
+  lc.attrs = la;
+  lc.numAttrs = attrs;
+  if (cudaLaunchKernelEx(&lc, k_product<CG, BN, T, FWD, SUM>, ma[0], mb[0], ma[1], mb[1], mo[0],
+                         mo[1], mr, mz, mq, args) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return QRB_ERR_LAUNCH;
+  }
   note_launches(1);
   return cudaGetLastError() == cudaSuccess ? QRB_OK : QRB_ERR_LAUNCH;
 }
 
 template <int CG, int BN, typename T>
-int launch_dir(bool fwd, bool sum, const Product* const* q, int count, Args& args, const Device& d,
+int launch_dir(bool fwd, bool sum, const Product* const* q, int count, Args& args, bool after_prepare,
                cudaStream_t s) {
   constexpr bool F32 = sizeof(T) == 4;
-  if (!fwd) return launch_t<CG, BN, T, false, F32>(q, count, args, d, s);
+  if (!fwd) return launch_t<CG, BN, T, false, F32>(q, count, args, after_prepare, s);
   if constexpr (!F32 && BN <= 128) {
-    if (sum) return launch_t<CG, BN, T, true, true>(q, count, args, d, s);
+    if (sum) return launch_t<CG, BN, T, true, true>(q, count, args, after_prepare, s);
   }
-  return launch_t<CG, BN, T, true, F32>(q, count, args, d, s);
+  return launch_t<CG, BN, T, true, F32>(q, count, args, after_prepare, s);
 }
 
 template <typename T>
 int launch_type(int cg, int bn, bool fwd, bool sum, const Product* const* q, int count,
-                Args& args, const Device& d, cudaStream_t s) {
-  if (cg == 1 && bn == 64) return launch_dir<1, 64, T>(fwd, sum, q, count, args, d, s);
-  if (cg == 1 && bn == 128) return launch_dir<1, 128, T>(fwd, sum, q, count, args, d, s);
-  if (cg == 2 && bn == 128) return launch_dir<2, 128, T>(fwd, sum, q, count, args, d, s);
+                Args& args, bool after_prepare, cudaStream_t s) {
+  if (cg == 1 && bn == 64) return launch_dir<1, 64, T>(fwd, sum, q, count, args, after_prepare, s);
+  if (cg == 1 && bn == 128) return launch_dir<1, 128, T>(fwd, sum, q, count, args, after_prepare, s);
+  if (cg == 2 && bn == 128) return launch_dir<2, 128, T>(fwd, sum, q, count, args, after_prepare, s);
   if constexpr (sizeof(T) == 2) {
-    if (cg == 2 && bn == 256) return launch_dir<2, 256, T>(fwd, sum, q, count, args, d, s);
+    if (cg == 2 && bn == 256) return launch_dir<2, 256, T>(fwd, sum, q, count, args, after_prepare, s);
   }
   return QRB_ERR_INVALID_ARG;
 }
@@ -1303,7 +1303,7 @@ ProductPlan plan_products(int dtype, const ProductSize* sizes, int count) {
 }
 
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
-                    const ColSum* cols, cudaStream_t s) {
+                    const ColSum* cols, bool after_prepare, cudaStream_t s) {
   const Device* d = device_info();
   if (d == nullptr) return QRB_ERR_DEVICE;
   if (!plan.ok) return QRB_ERR_UNSUPPORTED;
@@ -1343,14 +1343,15 @@ int launch_products(int dtype, const Product* products, int count, const Product
   const bool sum = (products[0].size.epilogue & 8) != 0;
   int rc = QRB_ERR_INVALID_ARG;
   switch (dtype) {
-    case QRBL_F32: rc = launch_type<float>(c.cg, c.bn, fwd, sum, q, count, args, *d, s); break;
-    case QRBL_F16: rc = launch_type<f16>(c.cg, c.bn, fwd, sum, q, count, args, *d, s); break;
-    case QRBL_BF16: rc = launch_type<bf16>(c.cg, c.bn, fwd, sum, q, count, args, *d, s); break;
+    case QRBL_F32: rc = launch_type<float>(c.cg, c.bn, fwd, sum, q, count, args, after_prepare, s); break;
+    case QRBL_F16: rc = launch_type<f16>(c.cg, c.bn, fwd, sum, q, count, args, after_prepare, s); break;
+    case QRBL_BF16: rc = launch_type<bf16>(c.cg, c.bn, fwd, sum, q, count, args, after_prepare, s); break;
   }
   for (int i = 0; i < count && rc == QRB_OK; ++i)
     if (plan.splits[i] > 1)
       rc = launch_join(dtype, products[i].part, plan.splits[i], plan.part_rows[i],
-                       plan.part_ld[i], products[i].size.m, products[i].size.n, products[i].e, s);
+                       plan.part_ld[i], products[i].size.m, products[i].size.n, products[i].e, true,
+                       s);
   return rc;
 }
 

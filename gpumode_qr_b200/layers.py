@@ -58,11 +58,13 @@ class PackedActivation(NamedTuple):
     dtype: torch.dtype
 
 
+_Tensor = torch.Tensor
+
+
 def _check(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
-    if (isinstance(t, torch.Tensor) and not t.requires_grad
-            and (t.dtype in _DTYPES and t.is_cuda if like is None
-                 else t.dtype is like.dtype and t.device == like.device)):
-        return
+    """Refuse what the library cannot take. (The entry points look at a plain
+    tensor's type, device and requires_grad themselves first: a call's host time
+    is most of a small layer's.)"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.dtype not in _DTYPES:
@@ -83,14 +85,26 @@ def _check_packed(name: str, p: PackedActivation, like: torch.Tensor, shape: tup
     codes, exps, dtype = p
     if dtype is not like.dtype:
         raise TypeError(f"{name} was packed from {dtype}, the layer is {like.dtype}")
+    dev = like.device
     want = (*shape[:-1], -(-shape[-1] // PACK_BLOCK))
+    if (type(codes) is _Tensor and type(exps) is _Tensor and codes.dtype is torch.int8
+            and exps.dtype is torch.int8 and codes.device == dev and exps.device == dev
+            and codes.shape == shape and exps.shape == want):
+        return
     for part, t, s in (("codes", codes, shape), ("exponents", exps, want)):
-        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int8:
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int8:
             raise TypeError(f"{name}.{part} must be an int8 tensor")
-        if t.device != like.device:
-            raise ValueError(f"{name}.{part} must be on {like.device}, got {t.device}")
+        if t.device != dev:
+            raise ValueError(f"{name}.{part} must be on {dev}, got {t.device}")
         if t.shape != s:
             raise ValueError(f"{name}.{part} must be {tuple(s)}, got {tuple(t.shape)}")
+
+
+def _contiguous(p: PackedActivation) -> tuple[torch.Tensor, torch.Tensor]:
+    codes, exps, _ = p
+    if codes.is_contiguous() and exps.is_contiguous():
+        return codes, exps
+    return codes.contiguous(), exps.contiguous()
 
 
 def _rows(t: torch.Tensor, shape: torch.Size, cols: int) -> tuple[torch.Tensor, int, int]:
@@ -157,8 +171,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     :class:`PackedActivation` (8 bits a value, written from the FP32 sums).
     Returns ``y``, or ``(y, z)`` with ``keep``.
     """
-    _check("x", x)
-    _check("weight", weight, x)
+    if type(x) is not _Tensor or x.dtype not in _DTYPES or not x.is_cuda or x.requires_grad:
+        _check("x", x)
+    dt, dev = x.dtype, x.device
+    if (type(weight) is not _Tensor or weight.dtype is not dt or weight.device != dev
+            or weight.requires_grad):
+        _check("weight", weight, x)
     xs, ws = x.shape, weight.shape
     if len(ws) != 2 or not xs or xs[-1] != ws[1]:
         raise ValueError(f"x must be [..., k] and weight [n, k], got {tuple(xs)} and {tuple(ws)}")
@@ -169,14 +187,18 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     w2, _, ldw = _rows(weight, ws, k)
     bp = rp = ldr = zp = ldz = qp = ep = 0
     if bias is not None:
-        _check("bias", bias, x)
+        if (type(bias) is not _Tensor or bias.dtype is not dt or bias.device != dev
+                or bias.requires_grad):
+            _check("bias", bias, x)
         if bias.shape != (n,):
             raise ValueError(f"bias must be ({n},), got {tuple(bias.shape)}")
         if bias.stride(0) != 1:
             bias = bias.contiguous()
         bp = bias.data_ptr()
     if residual is not None:
-        _check("residual", residual, x)
+        if (type(residual) is not _Tensor or residual.dtype is not dt or residual.device != dev
+                or residual.requires_grad):
+            _check("residual", residual, x)
         rs = residual.shape
         if rs != shape:
             raise ValueError(f"residual must be {shape}, got {tuple(rs)}")
@@ -196,7 +218,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if m and n:
         L = _lib.lib()
         _run(L.qrbl_linear, L.qrbl_linear_workspace_bytes,
-             _linear_args(_DTYPES[x.dtype], act, m, n, k, x2.data_ptr(), ldx, w2.data_ptr(), ldw,
+             _linear_args(_DTYPES[dt], act, m, n, k, x2.data_ptr(), ldx, w2.data_ptr(), ldw,
                           bp, rp, ldr, y.data_ptr(), n, zp, ldz, qp, ep), x)
     return y if keep is None else (y, z)
 
@@ -215,8 +237,12 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     type before the two products (dbias sums it unrounded); each result is
     rounded once.
     """
-    _check("dy", dy)
-    _check("weight", weight, dy)
+    if type(dy) is not _Tensor or dy.dtype not in _DTYPES or not dy.is_cuda or dy.requires_grad:
+        _check("dy", dy)
+    dt, dev = dy.dtype, dy.device
+    if (type(weight) is not _Tensor or weight.dtype is not dt or weight.device != dev
+            or weight.requires_grad):
+        _check("weight", weight, dy)
     ds, ws = dy.shape, weight.shape
     if len(ws) != 2 or not ds or ds[-1] != ws[0]:
         raise ValueError(f"dy must be [..., n] and weight [n, k], got {tuple(ds)} and {tuple(ws)}")
@@ -232,13 +258,15 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     if "weight" in need:
         if isinstance(x, PackedActivation):
             _check_packed("x", x, dy, (*lead, k))
-            xcodes, xexps = x.codes.contiguous(), x.exponents.contiguous()
+            xcodes, xexps = _contiguous(x)
             if k:
                 xq, xe = xcodes.data_ptr(), xexps.data_ptr()
         else:
             if x is None:
                 raise ValueError("x is needed for the weight's gradient")
-            _check("x", x, dy)
+            if (type(x) is not _Tensor or x.dtype is not dt or x.device != dev
+                    or x.requires_grad):
+                _check("x", x, dy)
             xs = x.shape
             if xs != (*lead, k):
                 raise ValueError(f"x must be {(*lead, k)}, got {tuple(xs)}")
@@ -252,12 +280,14 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
                 raise ValueError("relu's gradient needs z as a tensor: packed, small values lose "
                                  "their sign")
             _check_packed("z", z, dy, (*lead, n))
-            zcodes, zexps = z.codes.contiguous(), z.exponents.contiguous()
+            zcodes, zexps = _contiguous(z)
             zq, ze = zcodes.data_ptr(), zexps.data_ptr()
         else:
             if z is None:
                 raise ValueError(f"z is needed for the gradient of {activation!r}")
-            _check("z", z, dy)
+            if (type(z) is not _Tensor or z.dtype is not dt or z.device != dev
+                    or z.requires_grad):
+                _check("z", z, dy)
             zs = z.shape
             if zs != ds:
                 raise ValueError(f"z must be {tuple(ds)}, got {tuple(zs)}")
@@ -271,7 +301,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
         dbp = db.data_ptr()
     L = _lib.lib()
     _run(L.qrbl_linear_backward, L.qrbl_linear_backward_workspace_bytes,
-         _backward_args(_DTYPES[dy.dtype], act, m, n, k, dy2.data_ptr(), lddy, xp, ldx, xq, xe,
+         _backward_args(_DTYPES[dt], act, m, n, k, dy2.data_ptr(), lddy, xp, ldx, xq, xe,
                         w2.data_ptr(), ldw, zp, ldz, zq, ze, dxp, k, dwp, k, dbp), dy)
     return dx, dw, db
 
@@ -302,7 +332,8 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     upper end, which only the type's largest values reach). Inf and NaN become
     NaN and do not affect the other values.
     """
-    _check("x", x)
+    if type(x) is not _Tensor or x.dtype not in _DTYPES or not x.is_cuda or x.requires_grad:
+        _check("x", x)
     if x.dim() < 1:
         raise ValueError("x must be [..., c], got a scalar")
     shape = x.shape
@@ -329,7 +360,7 @@ def unpack_activation(packed: PackedActivation) -> torch.Tensor:
     x = codes.new_empty(*shape, dtype=dtype)
     _check_packed("packed", packed, x, shape)
     if x.numel():
-        codes, exps = codes.contiguous(), exps.contiguous()
+        codes, exps = _contiguous(packed)
         cols = shape[-1]
         _on(x, _lib.lib().qrbl_unpack, _DTYPES[dtype], codes.data_ptr(), exps.data_ptr(),
             x.numel() // cols, cols, x.data_ptr(), cols)
