@@ -41,12 +41,6 @@ __device__ __forceinline__ uint2 load_codes(const int8_t* p, bool vec, int valid
     if (i < valid) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void decode8f(uint2 q, float step, float (&out)[8]) {
-  f2 v[4];
-  decode8(q, step, v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f2_to(v[i], out[2 * i], out[2 * i + 1]);
-}
 __device__ __forceinline__ int clip(int64_t left, int most) {
   return left >= most ? most : (left > 0 ? (int)left : 0);
 }
@@ -199,7 +193,7 @@ __device__ __forceinline__ void stage_block(const StageJob& j, int64_t block) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[8];
-          decode8f(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]),
+          decode8(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), e[i],
                   v);
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[4 * h + k] = pair_of<T>(v[2 * k], v[2 * k + 1]);
@@ -213,7 +207,7 @@ __device__ __forceinline__ void stage_block(const StageJob& j, int64_t block) {
       if (valid <= 8 * h) continue;
       float v[8];
       if constexpr (PACKED)
-        decode8f(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), pow2f(e[i]), v);
+        decode8(h == 0 ? make_uint2(q[i].x, q[i].y) : make_uint2(q[i].z, q[i].w), e[i], v);
       else
         values8<T>(raw[i][h], v);
       if constexpr (PLANES) {
@@ -351,7 +345,7 @@ __device__ __forceinline__ void dz_block(const DzJob& j, int64_t block, float (*
         if (a.act != QRBL_ACT_NONE) {
           f2 zv[4];
           if constexpr (PACKED) {
-            decode8(q[k], pow2f(e[k]), zv);
+            decode8(q[k], e[k], zv);
           } else {
             values8<T>(z[k], f);
 #pragma unroll

@@ -410,28 +410,53 @@ __device__ __forceinline__ float finite_amax(const float (&v)[N]) {
 __device__ __forceinline__ float value_of(int code, float step) {
   return code == kNanCode ? __uint_as_float(0x7fc00000u) : (float)code * step;
 }
-// Eight codes as values, two to a register pair. A byte q + 128 put under the
-// exponent of 2^23 is the float 2^23 + 128 + q; kNanCode (byte 0 after the
-// flip) becomes NaN.
-__device__ __forceinline__ void decode8(uint2 q, float step, f2 (&out)[4]) {
-  const uint32_t y[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
-  const f2 off = f2_of(-8388736.f), st = f2_of(step);
+// Eight codes of a block with exponent e as values. A byte q + 128 put under the
+// exponent of 2^23 is the float 2^23 + 128 + q; one multiply-add takes the offset
+// off and scales (exactly: a power of two), as long as the scaled offset does not
+// overflow. kNanCode (byte 0 after the flip) and exponents beyond that go the
+// long way.
+constexpr int kDecodeMost = 104;
+__device__ __forceinline__ float code_float(uint32_t flipped, int i) {
+  return __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7540 + i));
+}
+__device__ __forceinline__ bool decode_long(uint32_t y0, uint32_t y1, int e) {
+  return ((((y0 - 0x01010101u) & ~y0) | ((y1 - 0x01010101u) & ~y1)) & 0x80808080u) != 0 ||
+         e > kDecodeMost;
+}
+__device__ __forceinline__ float decode_one(uint32_t flipped, int i, int e) {
+  const int code = (int)((flipped >> (8 * i)) & 255u) - 128;
+  return code == kNanCode ? __uint_as_float(0x7fc00000u) : (float)code * pow2f(e);
+}
+__device__ __forceinline__ void decode8(uint2 q, int e, float (&out)[8]) {
+  const uint32_t y0 = q.x ^ 0x80808080u, y1 = q.y ^ 0x80808080u;
+  const float step = pow2f(e), off = -8388736.f * step;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t w = y[i / 2], at = 2 * (i & 1);
-    out[i] = mul2(add2(f2_of(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + at)),
-                             __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7541 + at))),
-                       off), st);
+    out[i] = fmaf(code_float(y0, i), step, off);
+    out[4 + i] = fmaf(code_float(y1, i), step, off);
   }
-  if ((((y[0] - 0x01010101u) & ~y[0]) | ((y[1] - 0x01010101u) & ~y[1])) & 0x80808080u) {
+  if (decode_long(y0, y1, e)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float a, b;
-      f2_to(out[i], a, b);
-      const uint32_t w = y[i / 2] >> (16 * (i & 1));
-      if ((w & 255u) == 0) a = __uint_as_float(0x7fc00000u);
-      if ((w & 0xff00u) == 0) b = __uint_as_float(0x7fc00000u);
-      out[i] = f2_of(a, b);
+      out[i] = decode_one(y0, i, e);
+      out[4 + i] = decode_one(y1, i, e);
+    }
+  }
+}
+__device__ __forceinline__ void decode8(uint2 q, int e, f2 (&out)[4]) {  // as pairs
+  const uint32_t y0 = q.x ^ 0x80808080u, y1 = q.y ^ 0x80808080u;
+  const float step = pow2f(e), off = -8388736.f * step;
+  const f2 st = f2_of(step), of = f2_of(off);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    out[i] = fma2(f2_of(code_float(y0, 2 * i), code_float(y0, 2 * i + 1)), st, of);
+    out[2 + i] = fma2(f2_of(code_float(y1, 2 * i), code_float(y1, 2 * i + 1)), st, of);
+  }
+  if (decode_long(y0, y1, e)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      out[i] = f2_of(decode_one(y0, 2 * i, e), decode_one(y0, 2 * i + 1, e));
+      out[2 + i] = f2_of(decode_one(y1, 2 * i, e), decode_one(y1, 2 * i + 1, e));
     }
   }
 }
