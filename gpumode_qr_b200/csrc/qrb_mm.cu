@@ -154,17 +154,25 @@ __device__ __forceinline__ Item item_of(const Args& a, int worker, int step) {
     }
   }
   const Problem& p = a.p[it.prob];
-  const int tiles = p.mt * p.nt;
-  it.split = item / tiles;
-  const int t = item - it.split * tiles;
-  const int per = p.group * p.nt;
-  const int g = t / per, r = t - g * per;
-  const int first = g * p.group;
-  const int gm = p.mt - first < p.group ? p.mt - first : p.group;
-  it.m0 = (first + r % gm) * (BM * CG);
-  it.n0 = (r / gm) * BN;
-  it.kb0 = (int)((long long)p.kb * it.split / p.splits);
-  it.kb1 = (int)((long long)p.kb * (it.split + 1) / p.splits);
+  uint32_t t = (uint32_t)item;
+  it.split = 0;
+  it.kb0 = 0;
+  it.kb1 = p.kb;
+  if (p.splits > 1) {
+    const uint32_t tiles = (uint32_t)(p.mt * p.nt);
+    it.split = (int)(t / tiles);
+    t -= (uint32_t)it.split * tiles;
+    it.kb0 = (int)((long long)p.kb * it.split / p.splits);
+    it.kb1 = (int)((long long)p.kb * (it.split + 1) / p.splits);
+  }
+  const uint32_t per = (uint32_t)(p.group * p.nt);
+  const uint32_t g = t / per, r = t - g * per;
+  const uint32_t first = g * (uint32_t)p.group;
+  const uint32_t left = (uint32_t)p.mt - first;
+  const uint32_t gm = left < (uint32_t)p.group ? left : (uint32_t)p.group;
+  const uint32_t q = r / gm;
+  it.m0 = (int)(first + r - q * gm) * (BM * CG);
+  it.n0 = (int)q * BN;
   return it;
 }
 
@@ -497,9 +505,11 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
 template <typename T, uint32_t CB>
 __device__ __forceinline__ int pack32(uint32_t buf, int first, const float (&v)[32]) {
   constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
-  float amax = 0.f;  // columns beyond the matrix are 0 (or, beside Inf or NaN, NaN)
+  // columns beyond the matrix are 0 (or, beside Inf or NaN, NaN)
+  float part[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-  for (int i = 0; i < 32; ++i) amax = max_abs_nan(amax, v[i]);
+  for (int i = 4; i < 32; ++i) part[i & 3] = max_abs_nan(part[i & 3], v[i]);
+  float amax = max_abs_nan(max_abs_nan(part[0], part[1]), max_abs_nan(part[2], part[3]));
   const bool fine = finite_f(amax);
   if (!fine) amax = finite_amax(v);
   const int ex = block_exponent(amax, lo, hi);
@@ -763,10 +773,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool packed_z = FWD && !part && staged && e.z_codes != nullptr;
       const bool keep_z = plain_z || packed_z;
       const bool has_res = FWD && !part && staged && e.residual != nullptr;
-      // the staging is free: the last tile's stores have read it
-      if (lane == 0) tma::bulk_wait_read_all();
-      tma::fence_proxy_async();
-      __syncwarp();
+      // The staging is free once the last tile's stores have read it: awaited here
+      // for a residual that is loaded into it, else before its first use.
+      auto staging_free = [&]() {
+        if (lane == 0) tma::bulk_wait_read_all();
+        tma::fence_proxy_async();
+        __syncwarp();
+      };
+      if (has_res) staging_free();
       // residual of block g into its half (z kept: the second; else alternating)
       auto half_of = [&](int g) { return NH == 1 ? 0 : (keep_z ? 1 : (g & 1)); };
       auto load_res = [&](int g) {
@@ -798,6 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // One block of 32 columns, c from the warp's first: v holds the sums.
       auto finish = [&](float(&v)[32], int c) {
         const int at = col + c;
+        if (c == 0 && !has_res) staging_free();
         if (part) {  // (rows and columns padded to whole tiles)
           const int g = c / 32;
           if (g >= NH) {
