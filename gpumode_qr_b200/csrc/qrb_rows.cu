@@ -1,7 +1,9 @@
 // The forward product of a few rows (tokens): y = act(x W^T + b) + r with
-// m <= kRowsMost rows, bound by reading W once. One launch, no workspace: a CTA
-// takes 16 or 32 of W's rows, its eight warps interleave along k and add their
-// sums in shared memory in order, then run the epilogue.
+// m <= rows_most() rows, bound by reading W once. One launch, no workspace: a
+// CTA takes 16 of W's rows (FP32: 8; z kept in 8 bits: 32), its eight warps
+// interleave along k and add their sums in shared memory in order, then run the
+// epilogue. 1 x 4096 x 4096 BF16: 9.2 us from HBM, 3.6 TB/s (its floor 5.2 us;
+// the rest is the launch and two round trips to HBM), FP32 14.7 us, 4.6 TB/s.
 //
 // 16-bit types: W's rows are the 16-row operand of mma.sync m16n8k16 and eight
 // tokens the 8-column one, so both go from global memory straight to registers.
@@ -9,7 +11,7 @@
 // tokens the product is 1 / 100 of what either unit does while W streams in.)
 // The reduction's order is free, so lane (g, t) takes 8 consecutive values at
 // 8 t of row g, one 16-byte load, as the fragments of two MMAs; x is read the
-// same way. FP32: fused multiply-adds, four rows of W per warp.
+// same way. FP32: fused multiply-adds, eight rows of W at a time.
 #include "qrb_linear.cuh"
 
 namespace qrb {
@@ -23,6 +25,7 @@ constexpr int kStep = 32;  // reduction values of one warp step
 // not possible.
 __device__ __forceinline__ uint4 load8(const void* p, bool vec, int valid) {
   if (valid >= 8 && vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (valid <= 0) return make_uint4(0, 0, 0, 0);
   const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -82,12 +85,12 @@ __device__ __forceinline__ void finish1(float s, int tok, int64_t col, bool live
   reinterpret_cast<T*>(e.out)[(int64_t)tok * e.ldo + col] = from_f<T>(p[0]);
 }
 
-// RG groups of 16 rows of W, NT groups of 8 tokens.
-template <typename T, int RG, int NT>
+// RG groups of 16 rows of W, NT groups of 8 tokens, U steps' loads in flight.
+template <typename T, int RG, int NT, int U>
 __global__ void __launch_bounds__(kWarps * 32)
     k_rows(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int m,
            int64_t n, int64_t k, int vx, int vw, Epilogue e) {
-  constexpr int ROWS = 16 * RG, TOK = 8 * NT, U = NT == 4 ? 2 : 4;
+  constexpr int ROWS = 16 * RG, TOK = 8 * NT;
   constexpr int PITCH = ROWS + 4;  // floats of one token's sums
   __shared__ float part[kWarps][TOK][PITCH];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -158,85 +161,119 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-// FP32: 32 rows of W per CTA, four per warp and pass over k by all 32 lanes.
-template <int MT>
+// FP32: G passes of 8 rows of W per CTA; in each its eight warps interleave along
+// k, 128 values a step, up to MT tokens.
+template <int MT, int G>
 __global__ void __launch_bounds__(kWarps * 32)
     k_rows32(const float* __restrict__ x, int64_t ldx, const float* __restrict__ w, int64_t ldw,
              int m, int64_t n, int64_t k, int vx, int vw, Epilogue e) {
-  __shared__ float sums[MT][32];
+  constexpr int R = 8;
+  __shared__ float sums[kWarps][MT][R * G + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n0 = (int64_t)blockIdx.x * 32;
-  float acc[4][MT];
+  const int64_t n0 = (int64_t)blockIdx.x * R * G;
+#pragma unroll 1
+  for (int g = 0; g < G; ++g) {
+    float acc[R][MT];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int q = 0; q < MT; ++q) acc[r][q] = 0.f;
+      for (int q = 0; q < MT; ++q) acc[r][q] = 0.f;
 #pragma unroll 2
-  for (int64_t c = lane * 4; c < k; c += 128) {
-    const int have = k - c < 4 ? (int)(k - c) : 4;
-    float a[4][4];
+    for (int64_t c = warp * 128 + lane * 4; c < k; c += kWarps * 128) {
+      const int have = k - c < 4 ? (int)(k - c) : 4;
+      float a[R][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t row = n0 + warp * 4 + r;
-      load_n<float, 4>(w + row * ldw + c, vw, row < n ? have : 0, a[r]);
+      for (int r = 0; r < R; ++r) {
+        const int64_t row = n0 + g * R + r;
+        load_n<float, 4>(w + row * ldw + c, vw, row < n ? have : 0, a[r]);
+      }
+#pragma unroll
+      for (int q = 0; q < MT; ++q) {
+        float b[4];
+        load_n<float, 4>(x + (int64_t)q * ldx + c, vx, q < m ? have : 0, b);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[r][q] = fmaf(a[r][i], b[i], acc[r][q]);
+      }
     }
 #pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      float b[4];
-      load_n<float, 4>(x + (int64_t)q * ldx + c, vx, q < m ? have : 0, b);
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int q = 0; q < MT; ++q) {
+        float s = acc[r][q];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[r][q] = fmaf(a[r][i], b[i], acc[r][q]);
-    }
+        for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(kFull, s, o);
+        if (lane == 0) sums[warp][q][g * R + r] = s;
+      }
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      float s = acc[r][q];
-#pragma unroll
-      for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(kFull, s, o);
-      if (lane == 0) sums[q][warp * 4 + r] = s;
-    }
   __syncthreads();
-  for (int tok = warp; tok < m; tok += kWarps)
-    finish1<float, 32>(sums[tok][lane], tok, n0 + lane, n0 + lane < n, n, e);
+  // a warp takes 32 / (R G) tokens at a time
+  constexpr int ROWS = R * G, PER = 32 / ROWS;
+  const int row = lane % ROWS;
+  const int64_t col = n0 + row;
+  for (int t0 = warp * PER; t0 < m; t0 += kWarps * PER) {
+    const int tok = t0 + lane / ROWS;
+    float s = 0.f;
+    if (tok < MT) {
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) s += sums[v][tok][row];
+    }
+    finish1<float, ROWS>(s, tok, col, tok < m && col < n, n, e);
+  }
 }
 
-template <typename T, int RG, int NT>
+template <typename T, int RG, int NT, int U>
 void run16(const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k, int vx, int vw,
            const Epilogue& e, cudaStream_t s) {
   const int64_t grid = (n + 16 * RG - 1) / (16 * RG);
-  k_rows<T, RG, NT><<<(unsigned)grid, kWarps * 32, 0, s>>>(
+  k_rows<T, RG, NT, U><<<(unsigned)grid, kWarps * 32, 0, s>>>(
       reinterpret_cast<const T*>(x.p), x.ld, reinterpret_cast<const T*>(w.p), w.ld, (int)m, n, k,
       vx, vw, e);
 }
-template <typename T>
+// Steps in flight: what k has for one warp, at most 8 (one group of tokens), 4 or
+// 2: at 1 x 4096 x 4096 8 steps take 9.2 us against 11.0 for 4; at k = 512, where a
+// warp has 2 steps, 8 take 5.1 us and 4 take 3.3.
+template <typename T, int RG>
 void rows16(const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k, int vx, int vw,
             const Epilogue& e, cudaStream_t s) {
-  const bool wide = e.z_codes != nullptr;  // a packed block is 32 columns
-  if (m <= 8)
-    wide ? run16<T, 2, 1>(x, w, m, n, k, vx, vw, e, s) : run16<T, 1, 1>(x, w, m, n, k, vx, vw, e, s);
-  else if (m <= 16)
-    wide ? run16<T, 2, 2>(x, w, m, n, k, vx, vw, e, s) : run16<T, 1, 2>(x, w, m, n, k, vx, vw, e, s);
+  const int64_t steps = (k + kWarps * kStep - 1) / (kWarps * kStep);
+  if (m > 16)
+    run16<T, RG, 4, 2>(x, w, m, n, k, vx, vw, e, s);
+  else if (m > 8)
+    steps > 2 ? run16<T, RG, 2, 4>(x, w, m, n, k, vx, vw, e, s)
+              : run16<T, RG, 2, 2>(x, w, m, n, k, vx, vw, e, s);
+  else if (steps > 4 && RG == 1)
+    run16<T, RG, 1, RG == 1 ? 8 : 4>(x, w, m, n, k, vx, vw, e, s);
+  else if (steps > 2)
+    run16<T, RG, 1, 4>(x, w, m, n, k, vx, vw, e, s);
   else
-    wide ? run16<T, 2, 4>(x, w, m, n, k, vx, vw, e, s) : run16<T, 1, 4>(x, w, m, n, k, vx, vw, e, s);
+    run16<T, RG, 1, 2>(x, w, m, n, k, vx, vw, e, s);
 }
 template <int MT>
 void rows32(const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k, int vx, int vw,
             const Epilogue& e, cudaStream_t s) {
-  k_rows32<MT><<<(unsigned)((n + 31) / 32), kWarps * 32, 0, s>>>(
-      reinterpret_cast<const float*>(x.p), x.ld, reinterpret_cast<const float*>(w.p), w.ld, (int)m,
-      n, k, vx, vw, e);
+  const bool wide = e.z_codes != nullptr;  // a packed block is 32 columns
+  const int64_t rows = wide ? 32 : 8, grid = (n + rows - 1) / rows;
+  const float* xp = reinterpret_cast<const float*>(x.p);
+  const float* wp = reinterpret_cast<const float*>(w.p);
+  if (wide)
+    k_rows32<MT, 4><<<(unsigned)grid, kWarps * 32, 0, s>>>(xp, x.ld, wp, w.ld, (int)m, n, k, vx,
+                                                           vw, e);
+  else
+    k_rows32<MT, 1><<<(unsigned)grid, kWarps * 32, 0, s>>>(xp, x.ld, wp, w.ld, (int)m, n, k, vx,
+                                                           vw, e);
 }
 
 }  // namespace
 
-int64_t rows_most(int dtype) {
-  const int64_t most = dtype == QRBL_F32 ? 8 : 32;
+// Up to 8 rows in FP32 and 16 otherwise, 32 where k is short (4096 x 1024: 5.6 us
+// against 8.5 for tiles; 4096 x 4096: 15.9 against 13.9).
+int64_t rows_most(int dtype, int64_t k) {
+  const int64_t able = dtype == QRBL_F32 ? 8 : 32;
+  const int64_t most = dtype == QRBL_F32 ? 8 : (k <= 1024 ? 32 : 16);
   const int hook = linear_rows();
-  return hook < 0 || hook > most ? most : hook;
+  return hook < 0 ? most : (hook < able ? hook : able);
 }
 
 int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
@@ -244,6 +281,7 @@ int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_
   const int es = elem_size(dtype);
   const int vx = aligned16(x.p) && (m <= 1 || (x.ld * es) % 16 == 0);
   const int vw = aligned16(w.p) && (n <= 1 || (w.ld * es) % 16 == 0);
+  const bool wide = e.z_codes != nullptr;  // a packed block is 32 columns
   switch (dtype) {
     case QRBL_F32:
       if (m <= 1) rows32<1>(x, w, m, n, k, vx, vw, e, s);
@@ -251,8 +289,13 @@ int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_
       else if (m <= 4) rows32<4>(x, w, m, n, k, vx, vw, e, s);
       else rows32<8>(x, w, m, n, k, vx, vw, e, s);
       break;
-    case QRBL_F16: rows16<f16>(x, w, m, n, k, vx, vw, e, s); break;
-    case QRBL_BF16: rows16<bf16>(x, w, m, n, k, vx, vw, e, s); break;
+    case QRBL_F16:
+      wide ? rows16<f16, 2>(x, w, m, n, k, vx, vw, e, s) : rows16<f16, 1>(x, w, m, n, k, vx, vw, e, s);
+      break;
+    case QRBL_BF16:
+      wide ? rows16<bf16, 2>(x, w, m, n, k, vx, vw, e, s)
+           : rows16<bf16, 1>(x, w, m, n, k, vx, vw, e, s);
+      break;
     default: return QRB_ERR_INVALID_ARG;
   }
   note_launches(1);
