@@ -1,7 +1,12 @@
 // Elementwise and column-sum kernels of the linear-layer operators: the packed
 // 8-bit form, operands staged for the products, dz = dy act'(z) with the bias
-// gradient's sums, and the join of a product split along its reduction. All
-// are bound by HBM: each value is read once and written once, 8 per thread.
+// gradient's sums, and the join of a product split along its reduction. Each
+// value is read once and written once, so HBM bounds them; what keeps them from it
+// is instructions per value, hence the byte permutes instead of conversions, the
+// packed FP32 arithmetic and 16 values per access. Measured on a B200, 8192 x 4096
+// BF16: k_pack 18.6 us (5.4 TB/s), k_unpack 16.7 us (6.0 TB/s), dz with GELU from
+// packed z 39 us (4.2 TB/s: 26 instructions a value, among them two of the
+// special-function unit, which alone take 15 us), of HBM's 6.5 TB/s.
 #include "qrb_linear.cuh"
 
 namespace qrb {

@@ -144,11 +144,11 @@ int forward(const qrbl_linear_args& a, void* workspace, size_t bytes, cudaStream
   auto rows16 = [&](const void* p, int64_t ld) {
     return p == nullptr || (aligned16(p) && (a.m <= 1 || (ld * es) % 16 == 0));
   };
-  e.vec = rows16(a.y, a.ldy) && rows16(a.residual, a.ldr) && rows16(a.z, a.ldz) &&
-          aligned16(a.bias);
+  e.vec = rows16(a.y, a.ldy) && rows16(a.residual, a.ldr) && rows16(a.z, a.ldz);
   if (a.k == 0) return launch_join(a.dtype, nullptr, 0, 0, 0, a.m, a.n, e, false, s);
   Carve c{reinterpret_cast<uint8_t*>(workspace)};
   const Forward f = plan_forward(a, &c);
+  if (!f.rows && !f.plan.ok) return QRB_ERR_UNSUPPORTED;
   if (c.used > 0 && (workspace == nullptr || bytes < c.used)) return QRB_ERR_WORKSPACE;
   if (c.used > 0 && !aligned16(workspace)) return QRB_ERR_INVALID_ARG;
   if (f.rows) return launch_rows(a.dtype, f.x, f.w, a.m, a.n, a.k, e, s);
@@ -266,6 +266,7 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
   const int es = elem_size(a.dtype);
   Carve c{reinterpret_cast<uint8_t*>(workspace)};
   const Backward b = plan_backward(a, &c);
+  if (b.products > 0 && !b.plan.ok) return QRB_ERR_UNSUPPORTED;
   if (c.used > 0 && (workspace == nullptr || bytes < c.used)) return QRB_ERR_WORKSPACE;
   if (c.used > 0 && !aligned16(workspace)) return QRB_ERR_INVALID_ARG;
   if (a.m == 0 || a.n == 0) {  // sums over nothing

@@ -602,10 +602,10 @@ struct ColSum {
 template <typename T>
 __device__ __forceinline__ void column_sum(const ColSum& c, int64_t first, int64_t step) {
   for (int64_t col = first; col < c.n; col += step) {
-    float s = 0.f;
+    double s = 0;  // (there are as many sums as a long batch has blocks)
 #pragma unroll 16
     for (int64_t b = 0; b < c.blocks; ++b) s += c.part[b * c.n + col];
-    reinterpret_cast<T*>(c.out)[col] = from_f<T>(s);
+    reinterpret_cast<T*>(c.out)[col] = from_f<T>((float)s);
   }
 }
 int launch_colsum(int dtype, const ColSum& c, cudaStream_t s);

@@ -27,11 +27,25 @@
 // stages (a unit) the two accumulators are read and added to FP32 sums in
 // registers. A 16-bit forward product whose z is kept in 8 bits sums its chains
 // the same way (SUM): its other results are rounded far above the drift, but a
-// code near a border shows it (4 times fewer codes differ from the exact ones
-// at k = 4096).
+// code near a border shows it (z's relative error against exact codes 3.2e-4 ->
+// 1.0e-4 at k = 4096, an FP32 product's 1.2e-4; 8 us of 47 at 4096 x 4096 x 1024).
 //
 // A reduction split over several CTAs (few tiles, long k) writes FP32 partial
 // tiles that k_join adds in order: no atomics, the same bits every time.
+//
+// What bounds it, measured on a B200 (single launches):
+//  - long reductions: the tensor cores. dW and dx of 8192 x 4096 x 4096 BF16 in one
+//    launch 331 us = 1660 TFLOP/s (the library's burst rate is 1689), the forward
+//    product alone 181 us = 1520; back to back the card's power limit takes both to
+//    about 1200. 256 x 256 tiles on a pair: a CTA's 128 x 256 would need 96 bytes a
+//    clock from L2, more than the 64 an SM gets (719 clocks a stage; a pair 800
+//    until its MMAs were issued from uniform registers, now 580).
+//  - short reductions (k <= 1024): the epilogue. 128 columns take 3,000 clocks plain,
+//    5,500 with GELU and a residual, 8,000 with GELU and packed z, against 256 a
+//    stage for the products; 128-wide tiles then level better than 256-wide ones
+//    (plan_products).
+//  - single tiles: 1,500 clocks until the TMEM and the cluster are set up, 2,000 for
+//    the first load, then the epilogue: 8 us in all at k <= 512.
 //
 // Every wait is bounded: a timeout sets a block-wide abort flag and the device
 // error flag; the producer then waits (bounded) for its loads in flight, the
@@ -276,8 +290,8 @@ __device__ __forceinline__ bool elect_one() {
 // Block-scope acquire, also for what the other CTA of a pair announces: all that
 // passes between them is TMA and TMEM traffic, ordered by the barriers
 // themselves; a cluster-scope release or acquire would wait for this CTA's
-// global stores and drop its L1 (measured: 25,000 clocks per 128 x 256 tile
-// with GELU and packing, against 9,000 without).
+// global stores and drop its L1 (4096 x 4096 x 1024 with GELU and packed z:
+// 55.6 us against 52.4).
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, long long limit,
                                               volatile int* abort) {
   if (tma::mbar_try(bar, parity)) return true;
@@ -722,7 +736,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++unit;
         }
       }
-      if (__any_sync(kFull, *s_abort != 0)) {  // no MMA may run on into freed TMEM (a pair: fixed time as above)
+      // no MMA may run on into freed TMEM (a pair: a fixed time, as above)
+      if (__any_sync(kFull, *s_abort != 0)) {
         if constexpr (CG == 1) {
           if (elect_one()) tc::drain_mmas(BAR(B_FIN));
         } else {
@@ -1174,20 +1189,18 @@ double make_schedule(const int64_t* items, const double* each, int64_t most, Sch
   s.r = (int)(items[0] % g);
   double length = (s.q + (s.r > 0 ? 1 : 0)) * each[0];
   if (items[1] > 0) {
-    // the least x whose level holds every short item; y by what the one more
-    // long item leaves of it
-    const double ratio = each[0] / each[1];
-    int64_t x = (items[1] - 1) / g;
-    for (;; ++x) {
-      int64_t y = x - (int64_t)(ratio + 0.5);
-      if (y < 0) y = 0;
-      if (s.r == 0) y = x;
-      if (x * (g - s.r) + y * s.r >= items[1]) {
-        s.x = (int)x;
-        s.y = (int)y;
-        break;
-      }
+    // `more` rounds of short items fit beside the one more long item that the
+    // first r workers have; the least x and y = x - more (or 0) that hold all
+    const int64_t more = (int64_t)(each[0] / each[1] + 0.5), rest = g - s.r;
+    int64_t x = (items[1] + rest - 1) / rest, y = 0;
+    if (s.r == 0) {
+      y = x;
+    } else if (x > more) {
+      x = (items[1] + more * s.r + g - 1) / g;
+      y = x - more;
     }
+    s.x = (int)x;
+    s.y = (int)y;
     const double late = s.q * each[0] + s.x * each[1];
     const double early = s.r > 0 ? (s.q + 1) * each[0] + s.y * each[1] : 0;
     length = late > early ? late : early;

@@ -188,6 +188,22 @@ def test_linear_empty(dt):
     assert torch.equal(api.unpack_activation(p), api.unpack_activation(api.pack_activation(b.expand(3, 70))))
 
 
+def test_bias_at_any_alignment():
+    x, w = rnd((300, 128), 27, BF), rnd((160, 128), 28, BF, 0.1)
+    wide = rnd((400,), 29, BF)
+    for first in (0, 1, 3, 7):
+        b = wide[first:first + 160]
+        assert torch.equal(api.linear(x, w, b), api.linear(x, w, b.clone()))
+    check_forward(x, w, wide[1:161], None, "none", api.linear(x, w, wide[1:161]))
+
+
+@pytest.mark.parametrize("m,n,k", [(60_001, 64, 72), (200_000, 40, 32)])
+def test_long_batch_through_a_narrow_layer(m, n, k):
+    # one long tile of dW beside hundreds of short ones of dx; thousands of bias sums
+    dy, x, w = rnd((m, n), 48, BF), rnd((m, k), 49, BF), rnd((n, k), 50, BF)
+    check_backward(dy, x.double(), w, None, "none", *api.linear_backward(dy, x, w))
+
+
 def test_linear_non_finite_rows_stay_in_their_row():
     for dt in TYPES:
         x, w = rnd((70, 96), 20, dt), rnd((130, 96), 21, dt, 0.1)
@@ -308,6 +324,27 @@ def test_backward_far_pre_activations():
             y = api.linear(zz, eye, activation=act)
             # z * 1 is a product with zeros beside it: finite z only
             assert (y.float()[0, 3:10] - (z * want)[3:10].to(dt).float()).abs().max() < 1e-9
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=["bf16", "fp32"])
+def test_backward_packed_far_and_non_finite(dt):
+    # packed z at the ends of the exponents' range: derivative 0, 1 / 2 or 1; a
+    # block with NaN or Inf keeps the others' values; NaN stays in its row of dx
+    z = torch.zeros(4, 96, dtype=dt)
+    z[0, :32], z[0, 32:64], z[0, 64:] = 3e38, -3e38, 1e-37
+    z[1] = torch.linspace(-60, 60, 96).to(dt)
+    z[2], z[2, 40], z[2, 41] = 1.0, float("nan"), float("inf")
+    zp = api.pack_activation(z.to(DEV))
+    back = api.unpack_activation(zp).double()
+    assert back[2].isnan().sum() == 2 and (back[2][~back[2].isnan()] == 1).all()
+    dy, eye = torch.ones(4, 96, device=DEV, dtype=dt), torch.eye(96, device=DEV, dtype=dt)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        dx, _, db = api.linear_backward(dy, None, eye, zp, act, need=("x", "bias"))
+        want = act64(back, act)[1]
+        rows = [0, 1, 3]
+        near(dx[rows], want[rows], u(dt) * 1.2 + 2e-6 + 0 * want[rows])
+        assert dx[2].isnan().all()
+        assert db.isnan().sum() == 2
 
 
 @pytest.mark.parametrize("need", [c for r in range(4) for c in itertools.combinations(
