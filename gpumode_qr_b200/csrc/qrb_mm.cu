@@ -4,14 +4,16 @@
 //
 // Tiles of 128 x BN per CTA, or 256 x BN per pair of CTAs (CG = 2: one MMA over
 // both SMs, each holding 128 rows of A and half of B's columns, so a CTA loads
-// two thirds of the bytes), over a persistent grid of one CTA per SM. Ten warps:
-// 0-7 read the accumulators (warp w: TMEM lanes 32 (w & 3) .. + 31, one half of
-// the columns by w >> 2) and run the epilogue, 8 loads (one lane issues TMA
-// boxes into a ring of stages), 9 issues the MMAs (one lane, of the pair's first
-// CTA) and owns the TMEM. A stage holds 64 of the reduction's values for both
-// operands (128-byte swizzle). An operand whose reduction runs along memory rows
-// is K-major; one whose reduction runs across them (w in dz W, both operands of
-// dz^T x) is MN-major, so no operand is ever transposed in memory. Two
+// two thirds of the bytes), over a persistent grid of one CTA per SM. 16 warps (8
+// for 64 columns) read the accumulators and run the epilogue (warp w: TMEM lanes
+// 32 (w & 3) .. + 31, a quarter of the columns by w >> 2: four warps per scheduler,
+// since one's loads, waits and special functions leave most of its issue slots
+// empty), one loads (an elected lane issues TMA boxes into a ring of stages), one
+// issues the MMAs (of the pair's first CTA) and owns the TMEM. A stage holds 64 of
+// the reduction's values for both operands (128-byte swizzle). An operand whose
+// reduction runs along memory rows is K-major; one whose reduction runs across them
+// (w in dz W, both operands of dz^T x) is MN-major, so no operand is ever
+// transposed in memory. Two
 // accumulator buffers let the epilogue of one tile run beside the MMAs of the
 // next.
 //
@@ -28,7 +30,7 @@
 // registers. A 16-bit forward product whose z is kept in 8 bits sums its chains
 // the same way (SUM): its other results are rounded far above the drift, but a
 // code near a border shows it (z's relative error against exact codes 3.2e-4 ->
-// 1.0e-4 at k = 4096, an FP32 product's 1.2e-4; 8 us of 47 at 4096 x 4096 x 1024).
+// 1.0e-4 at k = 4096, an FP32 product's 1.2e-4).
 //
 // A reduction split over several CTAs (few tiles, long k) writes FP32 partial
 // tiles that k_join adds in order: no atomics, the same bits every time.
@@ -40,10 +42,9 @@
 //    about 1200. 256 x 256 tiles on a pair: a CTA's 128 x 256 would need 96 bytes a
 //    clock from L2, more than the 64 an SM gets (719 clocks a stage; a pair 800
 //    until its MMAs were issued from uniform registers, now 580).
-//  - short reductions (k <= 1024): the epilogue. 128 columns take 3,000 clocks plain,
-//    5,500 with GELU and a residual, 8,000 with GELU and packed z, against 256 a
-//    stage for the products; 128-wide tiles then level better than 256-wide ones
-//    (plan_products).
+//  - short reductions (k <= 1024): products and epilogue about equally. 4096 x 4096
+//    x 1024 with bias, GELU and a residual 32.5 us, with GELU and packed z 39 (eight
+//    epilogue warps instead of 16: 38.5 and 47).
 //  - single tiles: 1,500 clocks until the TMEM and the cluster are set up, 2,000 for
 //    the first load, then the epilogue: 8 us in all at k <= 512.
 //
@@ -64,8 +65,7 @@ namespace {
 
 constexpr int BM = 128;       // rows per CTA
 constexpr int kChainValues = 256;  // FP32: reduction values per accumulator chain
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr int kMostEpiWarps = 16;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kSmemMost = 232448;  // 227 KB
 constexpr int kPitch = 33;              // words of a row in a warp's turned block
@@ -73,7 +73,7 @@ constexpr int kPitch = 33;              // words of a row in a warp's turned blo
 // control block at the start of shared memory
 constexpr int B_FULL = 0, B_EMPTY = kMaxStages, B_ACCFULL = 2 * kMaxStages,
               B_ACCEMPTY = B_ACCFULL + 4, B_FIN = B_ACCEMPTY + 4, B_RES = B_FIN + 1,
-              NBAR = B_RES + 2 * kEpiWarps;
+              NBAR = B_RES + 2 * kMostEpiWarps;
 constexpr uint32_t OFF_TMEM = NBAR * 8, OFF_ABORT = OFF_TMEM + 4, CTRL = 1024;
 static_assert(OFF_ABORT + 4 <= CTRL, "control block");
 
@@ -87,21 +87,23 @@ struct Lay {
   static constexpr int BROWS = BN / CG;              // B's columns of one CTA
   static constexpr uint32_t A = BM * KROW, B = BROWS * KROW;
   static constexpr uint32_t STAGE = NP * (A + B);
-  // The epilogue's staging: each warp has HALVES buffers of 32 rows of up to 128
-  // bytes, from which TMA stores the results (and into which it loads the
-  // residual); unaligned matrices use the same memory to turn blocks, TROWS rows
-  // at a time.
-  static constexpr int HC = BN / 2;                  // columns of one epilogue warp
-  static constexpr int HALVES = NP == 3 ? 1 : 2;
-  static constexpr uint32_t WBUF = HALVES * 4096;
-  static constexpr int TROWS = NP == 3 ? 16 : 32;
-  static constexpr uint32_t ROWB = HC * sizeof(T) < 128 ? HC * sizeof(T) : 128;
-  static constexpr int GW = ROWB / sizeof(T);        // columns of one staged block
-  static constexpr uint32_t TURN = kEpiWarps * WBUF;
+  // EW epilogue warps, EW / 4 of them across the columns, HC columns each. Each
+  // has HALVES staging buffers for a block of 32 x 32 values (rows of ROWB bytes),
+  // from which TMA stores the results (and into which it loads the residual); a
+  // split product's FP32 blocks use both as one, unaligned matrices turn their
+  // blocks there, TROWS rows at a time.
+  static constexpr int EW = BN == 64 ? 8 : 16;
+  static constexpr int THREADS = (EW + 2) * 32;
+  static constexpr int HC = BN / (EW / 4);
+  static constexpr uint32_t ROWB = 32 * sizeof(T);
+  static constexpr uint32_t HBUF = 32 * ROWB, WBUF = 4096;
+  static constexpr int HALVES = WBUF / HBUF;
+  static constexpr int TROWS = 16;
+  static constexpr uint32_t TURN = EW * WBUF;
   static constexpr int FIT = (int)((kSmemMost - CTRL - 1024 - TURN) / STAGE);
   static constexpr int ST = FIT < kMaxStages ? FIT : kMaxStages;
   static constexpr uint32_t SMEM = 1024 + CTRL + ST * STAGE + TURN;  // 1024: base alignment
-  static_assert(TROWS * kPitch * 4 <= (int)WBUF && (ROWB == 64 || ROWB == 128), "staging");
+  static_assert(TROWS * kPitch * 4 <= (int)WBUF && HC % 32 == 0, "staging");
   static_assert(A % 1024 == 0 && B % 1024 == 0, "swizzle atoms");
   static constexpr int ACC = NP == 3 ? 2 * BN : BN;  // TMEM columns per buffer
   // accumulator buffers (SUM: as many as fit, so that the MMAs of the next tile's
@@ -345,9 +347,9 @@ __device__ __forceinline__ uint32_t staged_at(uint32_t buf, int row, int unit) {
                             : (ROWB == 64 ? unit ^ ((row >> 1) & 3) : unit ^ ((row >> 2) & 1));
   return buf + row * ROWB + x * 16;
 }
-// 32 values of the lane's row from column `first` of the block.
+// The lane's row of a block.
 template <typename E, uint32_t ROWB>
-__device__ __forceinline__ void stage_write(uint32_t buf, int first, const float (&v)[32]) {
+__device__ __forceinline__ void stage_write(uint32_t buf, const float (&v)[32]) {
   const int row = threadIdx.x & 31;
   constexpr int PER = 16 / sizeof(E);  // values of 16 bytes
 #pragma unroll
@@ -361,13 +363,13 @@ __device__ __forceinline__ void stage_write(uint32_t buf, int first, const float
         w[k] = pair_of<E>(v[PER * j + 2 * k], v[PER * j + 2 * k + 1]);
     }
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
-                     staged_at<ROWB>(buf, row, first / PER + j)),
+                     staged_at<ROWB>(buf, row, j)),
                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                  : "memory");
   }
 }
 template <typename T, uint32_t ROWB>
-__device__ __forceinline__ void stage_add(uint32_t buf, int first, float (&v)[32]) {
+__device__ __forceinline__ void stage_add(uint32_t buf, float (&v)[32]) {
   const int row = threadIdx.x & 31;
   constexpr int PER = 16 / sizeof(T);
 #pragma unroll
@@ -375,7 +377,7 @@ __device__ __forceinline__ void stage_add(uint32_t buf, int first, float (&v)[32
     uint32_t w[4];
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(staged_at<ROWB>(buf, row, first / PER + j))
+                 : "r"(staged_at<ROWB>(buf, row, j))
                  : "memory");
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -514,10 +516,10 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
   }
 }
 
-// The packed form of 32 columns of the lane's row: codes into the staged block
-// (rows of CB bytes) from column `first`; returns the exponent.
-template <typename T, uint32_t CB>
-__device__ __forceinline__ int pack32(uint32_t buf, int first, const float (&v)[32]) {
+// The packed form of the lane's row of a block: codes into the staged block (rows
+// of 32 bytes); returns the exponent.
+template <typename T>
+__device__ __forceinline__ int pack32(uint32_t buf, const float (&v)[32]) {
   constexpr int lo = ExpRange<T>::lo, hi = ExpRange<T>::hi;
   // columns beyond the matrix are 0 (or, beside Inf or NaN, NaN)
   float part[4] = {v[0], v[1], v[2], v[3]};
@@ -532,64 +534,28 @@ __device__ __forceinline__ int pack32(uint32_t buf, int first, const float (&v)[
 #pragma unroll
   for (int j = 0; j < 2; ++j)
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
-                     staged_at<CB>(buf, threadIdx.x & 31, first / 16 + j)),
+                     staged_at<32>(buf, threadIdx.x & 31, j)),
                  "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
                  : "memory");
   return ex;
 }
 
-// 64 consecutive TMEM columns of this warp's 32 lanes.
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
-  uint32_t r[64];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
-      :
-        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]),
-        "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
-        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
-        "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]),
-        "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
-        "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
-}
-// sum <- sum + the N columns at t (first: <- them).
-template <int N>
-__device__ __forceinline__ void drain(uint32_t t, float (&sum)[N], bool first) {
-  float v[N];
-  if constexpr (N == 64)
-    tmem_ld64(t, v);
-  else
-    tc::tmem_ld32(t, v);
+// sum <- sum + the 32 columns at t (first: <- them).
+__device__ __forceinline__ void drain(uint32_t t, float (&sum)[32], bool first) {
+  float v[32];
+  tc::tmem_ld32(t, v);
   if (first) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] = v[i];
+    for (int i = 0; i < 32; ++i) sum[i] = v[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i += 2)
+    for (int i = 0; i < 32; i += 2)
       f2_to(add2(f2_of(sum[i], sum[i + 1]), f2_of(v[i], v[i + 1])), sum[i], sum[i + 1]);
   }
 }
 
 template <int CG, int BN, typename T, bool FWD, bool SUM>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__((Lay<CG, BN, T, SUM>::THREADS), 1)
     k_product(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
               const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
               const __grid_constant__ CUtensorMap map_o0, const __grid_constant__ CUtensorMap map_o1,
@@ -597,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const __grid_constant__ CUtensorMap map_q,
               const __grid_constant__ Args a) {
   using L = Lay<CG, BN, T, SUM>;
+  constexpr int kEpiWarps = L::EW;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = tma::smem_addr(smem_raw);
   const uint32_t pad = (1024 - (raw & 1023)) & 1023;
@@ -748,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {  // ---- epilogue ----
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, part_of = warp >> 2;  // rows, columns
     constexpr int HC = L::HC;  // columns of this warp
     constexpr int NH = L::HALVES;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
@@ -780,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Problem& p = a.p[FWD ? 0 : it.prob];
       const Epilogue& e = p.e;
       const CUtensorMap* map_o = it.prob == 0 ? &map_o0 : &map_o1;
-      const int row0 = it.m0 + rank * BM + quad * 32, col = it.n0 + half * HC;
+      const int row0 = it.m0 + rank * BM + quad * 32, col = it.n0 + part_of * HC;
       const bool part = p.splits > 1, inside = row0 < p.m;
       const bool staged = part || e.vec != 0;
       // what is kept of z goes through the first half, y through the second
@@ -799,11 +766,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // residual of block g into its half (z kept: the second; else alternating)
       auto half_of = [&](int g) { return NH == 1 ? 0 : (keep_z ? 1 : (g & 1)); };
       auto load_res = [&](int g) {
-        const int h = half_of(g), c = col + g * L::GW;
+        const int h = half_of(g);
         if (lane == 0) {
           const uint32_t bar = BAR(B_RES + 2 * warp + h);
-          tma::mbar_expect_tx(bar, 32 * L::ROWB);
-          load_box2(stg + h * 4096, &map_r, bar, c, row0);
+          tma::mbar_expect_tx(bar, L::HBUF);
+          load_box2(stg + h * L::HBUF, &map_r, bar, col + 32 * g, row0);
         }
         uses0 += h == 0 ? 1u : 0u;
         uses1 += h == 0 ? 0u : 1u;
@@ -822,29 +789,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t exps = 0;
       const bool early = has_res && inside && !(NH == 1 && keep_z);
       if (early && col < p.n) load_res(0);
-      if (early && !keep_z && NH == 2 && HC > L::GW && col + L::GW < p.n) load_res(1);
+      if (early && !keep_z && NH == 2 && HC > 32 && col + 32 < p.n) load_res(1);
 
       // One block of 32 columns, c from the warp's first: v holds the sums.
       auto finish = [&](float(&v)[32], int c) {
         const int at = col + c;
         if (c == 0 && !has_res) staging_free();
-        if (part) {  // (rows and columns padded to whole tiles)
-          const int g = c / 32;
-          if (g >= NH) {
-            if (lane == 0) {
-              if constexpr (NH == 2)
-                bulk_wait_read_one();
-              else
-                tma::bulk_wait_read_all();
-            }
+        const int g = c / 32;
+        if (part) {  // (rows and columns padded to whole tiles; one buffer)
+          if (g > 0) {
+            if (lane == 0) tma::bulk_wait_read_all();
             __syncwarp();
           }
-          const uint32_t buf = stg + (g % NH) * 4096;
-          stage_write<float, 128>(buf, 0, v);
+          stage_write<float, 128>(stg, v);
           tma::fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            store_box(map_o, buf, at, (int)(it.split * p.part_rows) + row0);
+            store_box(map_o, stg, at, (int)(it.split * p.part_rows) + row0);
             tma::bulk_commit();
           }
           return;
@@ -854,10 +815,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           finish_turned<T, FWD, L::TROWS>(v, row0, at, p, turn);
           return;
         }
-        const int g = c / L::GW, in = c % L::GW;
-        const int h = half_of(g);
-        const bool last = in + 32 == L::GW;
-        if (in == 0 && g > 0 && (g >= NH || keep_z)) {  // this block's staging is free
+        const uint32_t ybuf = stg + half_of(g) * L::HBUF;
+        if (g > 0 && (g >= NH || keep_z)) {  // this block's staging is free
           if (lane == 0) {
             if (NH == 2 && !keep_z)
               bulk_wait_read_one();
@@ -867,6 +826,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (has_res && !(NH == 1 && keep_z)) load_res(g);
         }
+        // a kept block of z out of the first half
+        auto flush_z = [&](const CUtensorMap* map) {
+          tma::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            store_box(map, stg, at, row0);
+            tma::bulk_commit();
+            if constexpr (NH == 1) tma::bulk_wait_read_all();
+          }
+          __syncwarp();
+          if (NH == 1 && has_res) load_res(g);
+        };
         if constexpr (FWD) {
           if (e.bias != nullptr) {
             float mine = bias[0];
@@ -875,66 +846,38 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(kFull, mine, i);
           }
-          const bool flush = last || at + 32 >= p.n;
           if (plain_z) {
-            stage_write<T, L::ROWB>(stg, in, v);
-            if (flush) {
-              tma::fence_proxy_async();
-              __syncwarp();
-              if (lane == 0) {
-                store_box(&map_z, stg, at - in, row0);
-                tma::bulk_commit();
-                if constexpr (NH == 1) tma::bulk_wait_read_all();
-              }
-              __syncwarp();
-              if (NH == 1 && has_res) load_res(g);
-            }
+            stage_write<T, L::ROWB>(stg, v);
+            flush_z(&map_z);
           }
           if (packed_z) {
-            const int ex = pack32<T, L::GW>(stg, in, v);
-            exps |= (uint32_t)(ex & 255) << (8 * (c / 32));
-            if (flush) {
-              tma::fence_proxy_async();
-              __syncwarp();
-              if (lane == 0) {
-                store_box(&map_q, stg, at - in, row0);
-                tma::bulk_commit();
-                if constexpr (NH == 1) tma::bulk_wait_read_all();
-              }
-              __syncwarp();
-              if (NH == 1 && has_res) load_res(g);
-            }
+            const int ex = pack32<T>(stg, v);
+            flush_z(&map_q);
+            exps |= (uint32_t)(ex & 255) << (8 * g);
             if (c + 32 == HC || at + 32 >= p.n) {  // the row's exponents of all blocks
-              const int nblk = (p.n + kBlk - 1) / kBlk, count = c / 32 + 1;
+              const int nblk = (p.n + kBlk - 1) / kBlk;
               int8_t* x = e.z_exps + (int64_t)(row0 + lane) * nblk + col / kBlk;
               if (row0 + lane < p.m) {
-                if (count == 4 && (reinterpret_cast<uintptr_t>(x) & 3) == 0) {
-                  *reinterpret_cast<uint32_t*>(x) = exps;
-                } else {
 #pragma unroll
-                  for (int i = 0; i < HC / 32; ++i)
-                    if (i < count) x[i] = (int8_t)(exps >> (8 * i));
-                }
+                for (int i = 0; i < HC / 32; ++i)
+                  if (i <= g) x[i] = (int8_t)(exps >> (8 * i));
               }
             }
           }
           act_by(v, e.act);
           if (has_res) {
-            if (in == 0) {
-              const uint32_t uses = h == 0 ? uses0 : uses1;
-              live = warp_wait(BAR(B_RES + 2 * warp + h), (uses - 1) & 1, a.limit, s_abort);
-            }
-            stage_add<T, L::ROWB>(stg + h * 4096, in, v);
+            const int h = half_of(g);
+            const uint32_t uses = h == 0 ? uses0 : uses1;
+            live = warp_wait(BAR(B_RES + 2 * warp + h), (uses - 1) & 1, a.limit, s_abort);
+            stage_add<T, L::ROWB>(ybuf, v);
           }
         }
-        stage_write<T, L::ROWB>(stg + h * 4096, in, v);
-        if (last || at + 32 >= p.n) {
-          tma::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            store_box(map_o, stg + h * 4096, at - in, row0);
-            tma::bulk_commit();
-          }
+        stage_write<T, L::ROWB>(ybuf, v);
+        tma::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          store_box(map_o, ybuf, at, row0);
+          tma::bulk_commit();
         }
       };
 
@@ -943,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / L::NACC) & 1), a.limit, s_abort);
         if (!live) break;
         tc::fence_after();
-        const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
+        const uint32_t t = tmem + lanes + buf * L::ACC + part_of * HC;
 #pragma unroll 1
         for (int c = 0; c < HC; c += 32) {
           float v[32];
@@ -953,26 +896,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++unit;
       } else {
-        float sum[HC];
+        static_assert(!SUM || HC == 32, "one block of sums per warp");
+        float sum[32];
         for (int kb = it.kb0; kb < it.kb1; kb += L::CHAIN, ++unit) {
           const int buf = unit % L::NACC;
           live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / L::NACC) & 1), a.limit,
                            s_abort);
           if (!live) break;
           tc::fence_after();
-          const uint32_t t = tmem + lanes + buf * L::ACC + half * HC;
+          const uint32_t t = tmem + lanes + buf * L::ACC + part_of * HC;
           drain(t, sum, kb == it.kb0);
           if constexpr (L::NP == 3) drain(t + BN, sum, false);
           hand_back(buf);
         }
         if (!live) break;
-#pragma unroll 1
-        for (int c = 0; c < HC / 32; ++c) {
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = HC == 32 || c == 0 ? sum[i] : sum[HC - 32 + i];
-          finish(v, 32 * c);
-        }
+        finish(sum, 0);
       }
     }
     // no load or store of this warp's may use the staging after the block has gone
@@ -1101,7 +1039,7 @@ int launch_t(const Product* const* q, int count, Args& args, bool after_prepare,
     if ((p.e.residual != nullptr &&
          !encode_staged(&mr, p.e.residual, ES, p.n, p.m, p.e.ldr, L::ROWB)) ||
         (p.e.z != nullptr && !encode_staged(&mz, p.e.z, ES, p.n, p.m, p.e.ldz, L::ROWB)) ||
-        (p.e.z_codes != nullptr && !encode_staged(&mq, p.e.z_codes, 1, p.n, p.m, p.n, L::GW)))
+        (p.e.z_codes != nullptr && !encode_staged(&mq, p.e.z_codes, 1, p.n, p.m, p.n, 32)))
       return QRB_ERR_UNSUPPORTED;
   }
   cudaLaunchConfig_t lc = {};
@@ -1115,7 +1053,7 @@ int launch_t(const Product* const* q, int count, Args& args, bool after_prepare,
   }
   if (after_prepare) la[attrs++] = early_start();
   lc.gridDim = dim3(CG * (unsigned)args.s.workers);
-  lc.blockDim = dim3(kThreads);
+  lc.blockDim = dim3(L::THREADS);
   lc.dynamicSmemBytes = L::SMEM;
   lc.stream = s;
   lc.attrs = la;
@@ -1164,17 +1102,17 @@ constexpr Cut kCuts16[] = {{2, 256, 0.33}, {2, 128, 0.25}, {1, 128, 0.25}, {1, 6
 constexpr Cut kCuts32[] = {{2, 128, 0.65}, {1, 128, 0.72}, {1, 64, 0.53}};
 
 // One tile's products and its epilogue (which run beside another tile's), in
-// microseconds: a column of results takes 11 ns, 12 more with an activation, 6
-// with z kept, 5 with a residual (FP32 twice that).
+// microseconds: a column of results takes 9 ns, 6 more with an activation, 6 with
+// z kept, 4 with a residual (FP32 twice that).
 struct TileTime {
   double main, epi;
   double longer() const { return main > epi ? main : epi; }
   double shorter() const { return main > epi ? epi : main; }
 };
 TileTime tile_time(bool f32, const Cut& c, const ProductSize& z, int64_t kb, bool split) {
-  const double col = split ? 0.011
-                           : 0.011 + ((z.epilogue & 1) ? 0.012 : 0) + ((z.epilogue & 2) ? 0.006 : 0) +
-                                 ((z.epilogue & 4) ? 0.005 : 0);
+  const double col = split ? 0.009
+                           : 0.009 + ((z.epilogue & 1) ? 0.006 : 0) + ((z.epilogue & 2) ? 0.006 : 0) +
+                                 ((z.epilogue & 4) ? 0.004 : 0);
   return {(double)kb * c.stage, c.bn * col * (f32 ? 2 : 1)};
 }
 

@@ -17,8 +17,9 @@
  * products are formed, which keeps FP32's 24 bits; a product with an FP32 Inf
  * may give NaN instead of Inf). Every output is rounded once, to nearest even.
  *
- * Results are the same from call to call (no atomics), for a given shape,
- * alignment and device.
+ * Results are the same from call to call (no atomics), for given sizes,
+ * alignments, device and set of arguments (what is asked for beside a product can
+ * change how its reduction is cut, and so its last bits).
  */
 #ifndef QRB200_LINEAR_H
 #define QRB200_LINEAR_H
