@@ -77,7 +77,7 @@ constexpr int B_FULL = 0, B_EMPTY = kMaxStages, B_ACCFULL = 2 * kMaxStages,
 constexpr uint32_t OFF_TMEM = NBAR * 8, OFF_ABORT = OFF_TMEM + 4, CTRL = 1024;
 static_assert(OFF_ABORT + 4 <= CTRL, "control block");
 
-template <int CG, int BN, typename T, bool SUM>
+template <int CG, int BN, typename T, bool FWD, bool SUM>
 struct Lay {
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // planes
   static constexpr int BK = NP == 3 ? 32 : 64;       // reduction values per stage
@@ -98,6 +98,8 @@ struct Lay {
   static constexpr uint32_t ROWB = 32 * sizeof(T);
   static constexpr uint32_t HBUF = 32 * ROWB, WBUF = 4096;
   static constexpr int HALVES = WBUF / HBUF;
+  // without a residual or z, two blocks side by side as one box of 128-byte rows
+  static constexpr bool PAIRED = !FWD && sizeof(T) == 2 && HC == 64;
   static constexpr int TROWS = 16;
   static constexpr uint32_t TURN = EW * WBUF;
   static constexpr int FIT = (int)((kSmemMost - CTRL - 1024 - TURN) / STAGE);
@@ -349,7 +351,7 @@ __device__ __forceinline__ uint32_t staged_at(uint32_t buf, int row, int unit) {
 }
 // The lane's row of a block.
 template <typename E, uint32_t ROWB>
-__device__ __forceinline__ void stage_write(uint32_t buf, const float (&v)[32]) {
+__device__ __forceinline__ void stage_write(uint32_t buf, const float (&v)[32], int unit = 0) {
   const int row = threadIdx.x & 31;
   constexpr int PER = 16 / sizeof(E);  // values of 16 bytes
 #pragma unroll
@@ -363,7 +365,7 @@ __device__ __forceinline__ void stage_write(uint32_t buf, const float (&v)[32]) 
         w[k] = pair_of<E>(v[PER * j + 2 * k], v[PER * j + 2 * k + 1]);
     }
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
-                     staged_at<ROWB>(buf, row, j)),
+                     staged_at<ROWB>(buf, row, unit + j)),
                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                  : "memory");
   }
@@ -555,14 +557,14 @@ __device__ __forceinline__ void drain(uint32_t t, float (&sum)[32], bool first) 
 }
 
 template <int CG, int BN, typename T, bool FWD, bool SUM>
-__global__ void __launch_bounds__((Lay<CG, BN, T, SUM>::THREADS), 1)
+__global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
     k_product(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
               const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
               const __grid_constant__ CUtensorMap map_o0, const __grid_constant__ CUtensorMap map_o1,
               const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_z,
               const __grid_constant__ CUtensorMap map_q,
               const __grid_constant__ Args a) {
-  using L = Lay<CG, BN, T, SUM>;
+  using L = Lay<CG, BN, T, FWD, SUM>;
   constexpr int kEpiWarps = L::EW;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = tma::smem_addr(smem_raw);
@@ -586,19 +588,12 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, SUM>::THREADS), 1)
       tma::prefetch_map(&map_b1);
     }
   }
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < L::ST; ++s) {
-      tma::mbar_init(BAR(B_FULL + s), 1);
-      tma::mbar_init(BAR(B_EMPTY + s), 1);
-    }
-    for (int b = 0; b < L::NACC; ++b) {
-      tma::mbar_init(BAR(B_ACCFULL + b), 1);
-      tma::mbar_init(BAR(B_ACCEMPTY + b), CG * kEpiWarps);
-    }
-    tma::mbar_init(BAR(B_FIN), 1);
-    for (int i = 0; i < 2 * kEpiWarps; ++i) tma::mbar_init(BAR(B_RES + i), 1);
+  if (threadIdx.x < NBAR) {  // one barrier per thread
+    const int i = (int)threadIdx.x;
+    const bool acc_empty = i >= B_ACCEMPTY && i < B_FIN;
+    tma::mbar_init(BAR(i), acc_empty ? CG * kEpiWarps : 1);
     tma::mbar_fence_init();
-    *s_abort = 0;
+    if (i == 0) *s_abort = 0;
   }
   if (warp == kEpiWarps + 1) tmem_alloc<CG>(base + OFF_TMEM, L::TMEM);
   tc::fence_before();
@@ -815,6 +810,18 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, SUM>::THREADS), 1)
           finish_turned<T, FWD, L::TROWS>(v, row0, at, p, turn);
           return;
         }
+        if constexpr (L::PAIRED) {
+          stage_write<T, 128>(stg, v, 4 * g);
+          if (g == 1 || at + 32 >= p.n) {
+            tma::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              store_box(map_o, stg, col, row0);
+              tma::bulk_commit();
+            }
+          }
+          return;
+        }
         const uint32_t ybuf = stg + half_of(g) * L::HBUF;
         if (g > 0 && (g >= NH || keep_z)) {  // this block's staging is free
           if (lane == 0) {
@@ -1000,7 +1007,7 @@ const Device* device_info() {
 // The kernel for both (or one of the) products, or for a forward product.
 template <int CG, int BN, typename T, bool FWD, bool SUM>
 int launch_t(const Product* const* q, int count, Args& args, bool after_prepare, cudaStream_t s) {
-  using L = Lay<CG, BN, T, SUM>;
+  using L = Lay<CG, BN, T, FWD, SUM>;
   static std::once_flag once[64];
   static bool ready[64] = {};
   int dev = 0;
@@ -1023,7 +1030,8 @@ int launch_t(const Product* const* q, int count, Args& args, bool after_prepare,
       fine = fine && encode_staged(&mo[i], p.part, 4, p.part_ld, p.part_rows * p.splits,
                                    p.part_ld, 128);
     else if (e.vec)
-      fine = fine && encode_staged(&mo[i], e.out, ES, p.n, p.m, e.ldo, L::ROWB);
+      fine = fine && encode_staged(&mo[i], e.out, ES, p.n, p.m, e.ldo,
+                                   L::PAIRED ? 128 : L::ROWB);
     else
       mo[i] = ma[i];  // (not used)
     if (!fine) return QRB_ERR_UNSUPPORTED;
@@ -1147,7 +1155,7 @@ double make_schedule(const int64_t* items, const double* each, int64_t most, Sch
   return length;
 }
 
-int stage_values(bool f32) { return f32 ? Lay<1, 64, float, true>::BK : Lay<1, 64, bf16, false>::BK; }
+int stage_values(bool f32) { return f32 ? Lay<1, 64, float, true, true>::BK : Lay<1, 64, bf16, true, false>::BK; }
 
 Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, const Cut& c, int bk, int splits) {
   Problem p = {};
