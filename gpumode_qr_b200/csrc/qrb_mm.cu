@@ -13,9 +13,8 @@
 // the reduction's values for both operands (128-byte swizzle). An operand whose
 // reduction runs along memory rows is K-major; one whose reduction runs across them
 // (w in dz W, both operands of dz^T x) is MN-major, so no operand is ever
-// transposed in memory. Two
-// accumulator buffers let the epilogue of one tile run beside the MMAs of the
-// next.
+// transposed in memory. Two accumulator buffers let the epilogue of one tile run
+// beside the MMAs of the next.
 //
 // One launch takes one product or two independent ones (dx and dW): each CTA
 // or pair runs its share of the longer tiles first, then as many of the shorter
@@ -37,9 +36,9 @@
 //
 // What bounds it, measured on a B200 (single launches):
 //  - long reductions: the tensor cores. dW and dx of 8192 x 4096 x 4096 BF16 in one
-//    launch 331 us = 1660 TFLOP/s (the library's burst rate is 1689), the forward
-//    product alone 181 us = 1520; back to back the card's power limit takes both to
-//    about 1200. 256 x 256 tiles on a pair: a CTA's 128 x 256 would need 96 bytes a
+//    launch 340 us = 1617 TFLOP/s (a library product's burst rate is 1689), the
+//    forward product alone 181 us = 1520; back to back the card's power limit takes
+//    both to about 1300. 256 x 256 tiles on a pair: a CTA's 128 x 256 would need 96 bytes a
 //    clock from L2, more than the 64 an SM gets (719 clocks a stage; a pair 800
 //    until its MMAs were issued from uniform registers, now 580).
 //  - short reductions (k <= 1024): products and epilogue about equally. 4096 x 4096

@@ -14,10 +14,10 @@ operators around that gradient:
 
 All run on the caller's current stream, allocate only their outputs and scratch
 (from torch's caching allocator), can be captured into a CUDA graph, and give
-the same bits every time (for the same sizes, layouts and arguments). They are plain functions, like the rest of the
-library: autograd does not record them, and arguments that require a gradient
-are refused while gradients are enabled (call them under ``torch.no_grad()``
-or from an ``autograd.Function``).
+the same bits every time (for the same sizes, layouts and arguments). They are
+plain functions, like the rest of the library: autograd does not record them,
+and arguments that require a gradient are refused while gradients are enabled
+(call them under ``torch.no_grad()`` or from an ``autograd.Function``).
 """
 
 from __future__ import annotations

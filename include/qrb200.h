@@ -278,6 +278,13 @@ QRB_API int qrb_gram_geqrf_f32(const float* G, int64_t strideG_b, int64_t stride
  *   "sync_check"  1: every compute call synchronises its stream and reports
  *                 asynchronous kernel faults as QRB_ERR_LAUNCH and device-side
  *                 wait timeouts as QRB_ERR_DEVICE_WAIT (debug mode).
+ *   "linear_cut", "linear_splits", "linear_rows"  the linear-layer operators
+ *                 (qrb200_linear.h): the product's cut, 0 (default) = chosen by
+ *                 size, else 1000 * CTAs per tile + tile width (2256, 2128, 1128
+ *                 or 1064; FP32 takes no 2256); the parts its reduction is split
+ *                 in, 0 (default) = chosen by size, else 1..16; the most rows of
+ *                 the few-row kernel, -1 (default) = chosen by size, else 0..32.
+ *                 They change results' last bits (test only).
  *   "larfb_kind"  trailing update of the blocked route: -1 (default) =
  *                 automatic (3 where it applies, else 0); 0 = FP32 FFMA;
  *                 1 = tcgen05 3xTF32 for both products with operands staged
