@@ -114,6 +114,8 @@ def _rows(t: torch.Tensor, shape: torch.Size, cols: int) -> tuple[torch.Tensor, 
         t = t.reshape(-1, cols) if cols else t.new_empty((shape[:-1].numel(), 0))
         shape = t.shape
     rows = shape[0]
+    if cols == 1:  # a column of a conjugate's .imag is stored negated (wider ones are copied)
+        t = t.resolve_neg()
     row, col = t.stride()
     if (col != 1 and cols > 1) or (row < cols and rows > 1):
         t = t.contiguous()
@@ -193,7 +195,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         if bias.shape != (n,):
             raise ValueError(f"bias must be ({n},), got {tuple(bias.shape)}")
         if bias.stride(0) != 1:
-            bias = bias.contiguous()
+            bias = bias.contiguous().resolve_neg()
         bp = bias.data_ptr()
     if residual is not None:
         if (type(residual) is not _Tensor or residual.dtype is not dt or residual.device != dev

@@ -197,6 +197,20 @@ def test_bias_at_any_alignment():
     check_forward(x, w, wide[1:161], None, "none", api.linear(x, w, wide[1:161]))
 
 
+def test_negated_views():
+    """``c.conj().imag`` is a real tensor whose memory holds the values negated."""
+    c = torch.complex(rnd((5, 3), 90, FP), rnd((5, 3), 91, FP))
+    for cols in (1, 3):
+        x, w = c[:, :cols].conj().imag, rnd((4, cols), 92, FP)
+        assert x.is_neg()
+        check_forward(x, w, None, None, "none", api.linear(x, w))
+        p = api.pack_activation(x)
+        assert torch.equal(p.codes, api.pack_activation(x.clone()).codes)
+    b = c[:1, 0].conj().imag
+    w = rnd((1, 3), 93, FP)
+    check_forward(c.real, w, b, None, "none", api.linear(c.real, w, b))
+
+
 @pytest.mark.parametrize("m,n,k", [(60_001, 64, 72), (200_000, 40, 32)])
 def test_long_batch_through_a_narrow_layer(m, n, k):
     # one long tile of dW beside hundreds of short ones of dx; thousands of bias sums
