@@ -140,17 +140,18 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a 
 _OK, _NEEDS_WORKSPACE = 0, 3  # QRB_OK, QRB_ERR_WORKSPACE
 
 
-def _run(call, size, args: bytes, like: torch.Tensor) -> None:
+def _run(call, size, args: bytes, like: torch.Tensor, likely: bool = False) -> None:
     """``call`` on the current stream of ``like``'s device, with the workspace
-    it asks for."""
+    it asks for (``likely`` some: asked first)."""
     index = like.get_device()
     if index != _current_device():
         with torch.cuda.device(index):
-            return _run(call, size, args, like)
+            return _run(call, size, args, like, likely)
     stream = _raw_stream(index)
-    rc = call(args, None, 0, stream)
+    need = size(args) if likely else 0
+    rc = _NEEDS_WORKSPACE if need else call(args, None, 0, stream)
     if rc == _NEEDS_WORKSPACE:  # nothing was enqueued
-        need = size(args)
+        need = need or size(args)
         ws = like.new_empty(need, dtype=torch.uint8)
         rc = call(args, ws.data_ptr(), need, stream)
     if rc != _OK:
@@ -304,7 +305,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     L = _lib.lib()
     _run(L.qrbl_linear_backward, L.qrbl_linear_backward_workspace_bytes,
          _backward_args(_DTYPES[dt], act, m, n, k, dy2.data_ptr(), lddy, xp, ldx, xq, xe,
-                        w2.data_ptr(), ldw, zp, ldz, zq, ze, dxp, k, dwp, k, dbp), dy)
+                        w2.data_ptr(), ldw, zp, ldz, zq, ze, dxp, k, dwp, k, dbp), dy, True)
     return dx, dw, db
 
 
