@@ -110,7 +110,7 @@ struct Forward {
 };
 Forward plan_forward(const qrbl_linear_args& a, Carve* c) {
   Forward f;
-  f.rows = a.m <= rows_most(a.dtype, a.k);
+  f.rows = takes_rows(a.dtype, a.m, a.n, a.k, a.z_codes != nullptr);
   if (f.rows) {
     f.x.p = a.x; f.x.ld = a.ldx;
     f.w.p = a.w; f.w.ld = a.ldw;

@@ -540,9 +540,9 @@ ProductPlan plan_products(int dtype, const ProductSize* sizes, int count);
 // launch in front of it on the stream is this call's launch_prepare.
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
                     const ColSum* sum, bool after_prepare, cudaStream_t s);
-// The forward product of m <= rows_most(dtype, k) rows, x and w read in place at
-// any alignment.
-int64_t rows_most(int dtype, int64_t k);
+// The forward product of few rows (where takes_rows), x and w read in place at any
+// alignment.
+bool takes_rows(int dtype, int64_t m, int64_t n, int64_t k, bool packed);
 int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
                 const Epilogue& e, cudaStream_t s);
 // out = epilogue(sum of `splits` partial sums), part[s][row][col] with rows

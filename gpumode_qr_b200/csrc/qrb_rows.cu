@@ -1,9 +1,9 @@
-// The forward product of a few rows (tokens): y = act(x W^T + b) + r with
-// m <= rows_most() rows, bound by reading W once. One launch, no workspace: a
+// The forward product of a few rows (tokens): y = act(x W^T + b) + r where
+// takes_rows(), bound by reading W once. One launch, no workspace: a
 // CTA takes 16 of W's rows (FP32: 8; z kept in 8 bits: 32), its eight warps
 // interleave along k and add their sums in shared memory in order, then run the
 // epilogue. 1 x 4096 x 4096 BF16: 9.2 us from HBM, 3.6 TB/s (its floor 5.2 us;
-// the rest is the launch and two round trips to HBM), FP32 14.7 us, 4.6 TB/s.
+// the rest is the launch and two round trips to HBM), FP32 14.8 us, 4.5 TB/s.
 //
 // 16-bit types: W's rows are the 16-row operand of mma.sync m16n8k16 and eight
 // tokens the 8-column one, so both go from global memory straight to registers.
@@ -11,7 +11,10 @@
 // tokens the product is 1 / 100 of what either unit does while W streams in.)
 // The reduction's order is free, so lane (g, t) takes 8 consecutive values at
 // 8 t of row g, one 16-byte load, as the fragments of two MMAs; x is read the
-// same way. FP32: fused multiply-adds, eight rows of W at a time.
+// same way. FP32: fused multiply-adds, eight rows of W at a time, two CTAs on an SM;
+// more tokens in groups of four or eight over the grid, each of which reads W
+// again from L2 (8 x 4096 x 4096: 26.6 us; with five shuffles for each of a warp's 64
+// sums and one CTA on an SM 42.8).
 #include "qrb_linear.cuh"
 
 namespace qrb {
@@ -161,16 +164,19 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-// FP32: G passes of 8 rows of W per CTA; in each its eight warps interleave along
-// k, 128 values a step, up to MT tokens.
+// FP32: G passes of 8 rows of W per CTA and MT tokens (of blockIdx.y's group); in
+// each its eight warps interleave along k, 128 values a step.
 template <int MT, int G>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, 2)
     k_rows32(const float* __restrict__ x, int64_t ldx, const float* __restrict__ w, int64_t ldw,
              int m, int64_t n, int64_t k, int vx, int vw, Epilogue e) {
   constexpr int R = 8;
   __shared__ float sums[kWarps][MT][R * G + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n0 = (int64_t)blockIdx.x * R * G;
+  const int tok0 = (int)blockIdx.y * MT;
+  x += (int64_t)tok0 * ldx;
+  m -= tok0;
 #pragma unroll 1
   for (int g = 0; g < G; ++g) {
     float acc[R][MT];
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int q = 0; q < MT; ++q) acc[r][q] = 0.f;
-#pragma unroll 2
+#pragma unroll(MT == 8 ? 1 : 2)
     for (int64_t c = warp * 128 + lane * 4; c < k; c += kWarps * 128) {
       const int have = k - c < 4 ? (int)(k - c) : 4;
       float a[R][4];
@@ -197,29 +203,46 @@ __global__ void __launch_bounds__(kWarps * 32)
           for (int i = 0; i < 4; ++i) acc[r][q] = fmaf(a[r][i], b[i], acc[r][q]);
       }
     }
+    // the warp's sums of each of the R MT accumulators: a step over half the lanes
+    // also halves the accumulators a lane still holds, of which it keeps those of
+    // its side, so 64 take 62 shuffles instead of 320
+    constexpr int N = R * MT;
+    float(&v)[N] = *reinterpret_cast<float(*)[N]>(&acc[0][0]);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int o = 16, left = N; o > 0; o /= 2) {
+      const bool up = (lane & o) != 0;
+      if (left > 1) {
+        left /= 2;
 #pragma unroll
-      for (int q = 0; q < MT; ++q) {
-        float s = acc[r][q];
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(kFull, s, o);
-        if (lane == 0) sums[warp][q][g * R + r] = s;
+        for (int i = 0; i < N / 2; ++i) {
+          if (i >= left) break;
+          const float mine = up ? v[i + left] : v[i], other = up ? v[i] : v[i + left];
+          v[i] = mine + __shfl_xor_sync(kFull, other, o);
+        }
+      } else {
+        v[0] += __shfl_xor_sync(kFull, v[0], o);
       }
+    }
+    constexpr int EACH = N > 32 ? N / 32 : 1, SAME = N < 32 ? 32 / N : 1;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int at = lane / SAME * EACH + j;
+      if (lane % SAME == 0) sums[warp][at % MT][g * R + at / MT] = v[j];
+    }
   }
   __syncthreads();
   // a warp takes 32 / (R G) tokens at a time
   constexpr int ROWS = R * G, PER = 32 / ROWS;
   const int row = lane % ROWS;
   const int64_t col = n0 + row;
-  for (int t0 = warp * PER; t0 < m; t0 += kWarps * PER) {
+  for (int t0 = warp * PER; t0 < MT; t0 += kWarps * PER) {
     const int tok = t0 + lane / ROWS;
     float s = 0.f;
     if (tok < MT) {
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) s += sums[v][tok][row];
     }
-    finish1<float, ROWS>(s, tok, col, tok < m && col < n, n, e);
+    finish1<float, ROWS>(s, tok0 + tok, col, tok < MT && tok < m && col < n, n, e);
   }
 }
 
@@ -250,30 +273,47 @@ void rows16(const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
   else
     run16<T, RG, 1, 2>(x, w, m, n, k, vx, vw, e, s);
 }
+// Whether groups of four tokens give no more CTAs than fit (two on each of 148
+// SMs): faster than groups of eight then (8 x 1024 x 1024: 3.4 us against 5.0), slower
+// where they read W twice as often in more waves (8 x 4096 x 4096: 32.3 against 26.6).
+bool at_once(int64_t m, int64_t n, bool wide) {
+  const int64_t rows = wide ? 32 : 8;
+  return (n + rows - 1) / rows * ((m + 3) / 4) <= 2 * 148;
+}
 template <int MT>
 void rows32(const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k, int vx, int vw,
             const Epilogue& e, cudaStream_t s) {
   const bool wide = e.z_codes != nullptr;  // a packed block is 32 columns
-  const int64_t rows = wide ? 32 : 8, grid = (n + rows - 1) / rows;
+  const int64_t rows = wide ? 32 : 8;
+  const dim3 grid((unsigned)((n + rows - 1) / rows), (unsigned)((m + MT - 1) / MT));
   const float* xp = reinterpret_cast<const float*>(x.p);
   const float* wp = reinterpret_cast<const float*>(w.p);
   if (wide)
-    k_rows32<MT, 4><<<(unsigned)grid, kWarps * 32, 0, s>>>(xp, x.ld, wp, w.ld, (int)m, n, k, vx,
+    k_rows32<MT, 4><<<grid, kWarps * 32, 0, s>>>(xp, x.ld, wp, w.ld, (int)m, n, k, vx,
                                                            vw, e);
   else
-    k_rows32<MT, 1><<<(unsigned)grid, kWarps * 32, 0, s>>>(xp, x.ld, wp, w.ld, (int)m, n, k, vx,
+    k_rows32<MT, 1><<<grid, kWarps * 32, 0, s>>>(xp, x.ld, wp, w.ld, (int)m, n, k, vx,
                                                            vw, e);
 }
 
 }  // namespace
 
-// Up to 8 rows in FP32 and 16 otherwise, 32 where k is short (4096 x 1024: 5.6 us
-// against 8.5 for tiles; 4096 x 4096: 15.9 against 13.9).
-int64_t rows_most(int dtype, int64_t k) {
-  const int64_t able = dtype == QRBL_F32 ? 8 : 32;
-  const int64_t most = dtype == QRBL_F32 ? 8 : (k <= 1024 ? 32 : 16);
+// 16-bit types: up to 16 rows, 32 where k is short (32 x 4096 x 1024: 5.6 us
+// against 8.5 for tiles; 32 x 4096 x 4096: 15.9 against 13.9). FP32: up to 8 rows, and
+// more where the groups' estimate, in microseconds, is below the tiles', most of
+// which is W's three planes being written and read back (32 x 1024 x 1024: 9.9
+// against 13.0, 48: 13.7 against 13.2; 16 x 4096 x 4096: 51.6 against 68.7, 24: 74.5
+// against 68.2; 64 x 1024 x 256: 15.3 against 11.5). With z packed a CTA's four passes
+// over k follow one another, which few columns do not hide (4 x 64 x 8192: 38.1
+// against 16.8).
+bool takes_rows(int dtype, int64_t m, int64_t n, int64_t k, bool packed) {
   const int hook = linear_rows();
-  return hook < 0 ? most : (hook < able ? hook : able);
+  if (hook >= 0) return m <= hook;
+  if (dtype != QRBL_F32) return m <= (k <= 1024 ? 32 : 16);
+  const double tiles = 10.0 + 3.4e-6 * (double)n * (double)k;
+  if (m > 128 || (packed && 5.0 + 0.004 * (double)k > tiles)) return false;
+  const double groups = (double)((n + 7) / 8 * ((m + 7) / 8));
+  return m <= 8 || 1.3 + groups * (0.0128 + 8e-6 * (double)k) < tiles;
 }
 
 int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_t n, int64_t k,
@@ -286,7 +326,7 @@ int launch_rows(int dtype, const Operand& x, const Operand& w, int64_t m, int64_
     case QRBL_F32:
       if (m <= 1) rows32<1>(x, w, m, n, k, vx, vw, e, s);
       else if (m <= 2) rows32<2>(x, w, m, n, k, vx, vw, e, s);
-      else if (m <= 4) rows32<4>(x, w, m, n, k, vx, vw, e, s);
+      else if (m <= 4 || at_once(m, n, wide)) rows32<4>(x, w, m, n, k, vx, vw, e, s);
       else rows32<8>(x, w, m, n, k, vx, vw, e, s);
       break;
     case QRBL_F16:

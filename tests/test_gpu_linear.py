@@ -245,7 +245,7 @@ def test_linear_in_place_residual():
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=IDS)
-@pytest.mark.parametrize("m,n,k", [(3, 40, 64), (130, 100, 72), (16, 48, 4096)])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 64), (130, 100, 72), (16, 48, 4096), (21, 70, 128)])
 def test_rows_and_columns_outside_stay_as_they_were(m, n, k, dt):
     # outputs inside larger buffers: only [m, n] is written
     L, s = _lib.lib(), torch.cuda.current_stream().cuda_stream
@@ -590,6 +590,23 @@ def test_few_rows_and_tiles_agree(dt, hooks):
         for rows in (m, 0):
             hooks("linear_rows", rows)
             check_forward(x, w, b, r, "gelu", api.linear(x, w, b, r, "gelu"))
+
+
+@pytest.mark.parametrize("m,n,k", [(9, 512, 256), (13, 2048, 1024), (32, 70, 999), (33, 1000, 257),
+                                   (64, 128, 128), (127, 33, 40), (128, 40, 8)])
+def test_fp32_tokens_in_groups(m, n, k):
+    """More than eight rows in FP32: groups of four or eight over the grid, the last one cut."""
+    x, w = rnd((m, k), 182, FP), rnd((n, k), 183, FP, k**-0.5)
+    b, r = rnd((n,), 184, FP), rnd((m, n), 185, FP)
+    y, z = api.linear(x, w, b, r, "gelu", keep="plain")
+    check_forward(x, w, b, r, "gelu", y, z)
+    y, p = api.linear(x, w, b, r, "gelu", keep="packed")
+    z64, z_err = check_forward(x, w, b, r, "gelu", y)
+    half = torch.ldexp(torch.full(p.exponents.shape, 0.5, dtype=torch.float64, device=DEV),
+                       p.exponents.int()).repeat_interleave(32, dim=1)[:, :n]
+    near(api.unpack_activation(p), z64, half + z_err, "packed z")
+    one = torch.cat([api.linear(x[i:i + 1], w, b, r[i:i + 1], "gelu") for i in (0, m // 2, m - 1)])
+    check_forward(x[[0, m // 2, m - 1]], w, b, r[[0, m // 2, m - 1]], "gelu", one)
 
 
 def test_z_kept_both_ways():
