@@ -241,8 +241,9 @@ __global__ void __launch_bounds__(kThreads) k_unpack(StageJob j) {
 // dz = dy act'(z), and its column sums
 // ---------------------------------------------------------------------------
 // Warps of 256 columns (8 per lane), 8 warps over the rows; a block takes `rows`
-// rows of them, 2 (FP32: 1) per warp loaded together. Each thread sums its rows in order, then the block's warps are
-// added in order: the same bits every time. part[row block][col].
+// rows of them, 2 (FP32: 1) per warp loaded together. Each thread sums its rows in
+// order, then the block's warps are added in order: the same bits every time.
+// part[row block][col].
 struct DzJob {
   DzArgs a;
   int64_t nx = 1, blocks = 0, nblk = 0;

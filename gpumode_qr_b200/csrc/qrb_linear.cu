@@ -252,11 +252,13 @@ Backward plan_backward(const qrbl_linear_backward_args& a, Carve* c) {
   return b;
 }
 
+// (in one piece where it is one: a pitch ends at 2^31 bytes)
 int zero_rows(void* p, int64_t ld, int64_t rows, int64_t cols, int es, cudaStream_t s) {
-  return cudaMemset2DAsync(p, (size_t)(rows <= 1 ? cols : ld) * es, 0, (size_t)cols * es,
-                           (size_t)rows, s) == cudaSuccess
-             ? QRB_OK
-             : QRB_ERR_LAUNCH;
+  const size_t row = (size_t)cols * es;
+  const cudaError_t e = rows <= 1 || ld == cols
+                            ? cudaMemsetAsync(p, 0, row * (size_t)rows, s)
+                            : cudaMemset2DAsync(p, (size_t)ld * es, 0, row, (size_t)rows, s);
+  return e == cudaSuccess ? QRB_OK : QRB_ERR_LAUNCH;
 }
 
 int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, cudaStream_t s) {

@@ -408,6 +408,13 @@ def test_backward_empty(dt):
     assert (dw == 0).all() and (db == 0).all()
 
 
+def test_backward_of_nothing_through_a_wide_layer():
+    k = 2**29 + 24  # one row of dW is more than 2^31 bytes
+    w = torch.empty(1, k, device=DEV)
+    dw = api.linear_backward(w.new_empty(0, 1), w.new_empty(0, k), w, need=("weight",))[1]
+    assert dw.shape == (1, k) and not dw.any()
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_gradients_against_differences(act):
     # central differences of the FP64 formula's loss sum(y * c) around the FP32 inputs
