@@ -415,7 +415,8 @@ struct PrepArgs {
   StageJob st[2];
 };
 template <typename T>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4) k_prepare(const __grid_constant__ PrepArgs p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4)
+    k_prepare(const __grid_constant__ PrepArgs p) {
   constexpr bool PLANES = sizeof(T) == 4;
   __shared__ float sums[8][256];
   let_next_start();

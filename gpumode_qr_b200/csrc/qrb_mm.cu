@@ -1154,7 +1154,9 @@ double make_schedule(const int64_t* items, const double* each, int64_t most, Sch
   return length;
 }
 
-int stage_values(bool f32) { return f32 ? Lay<1, 64, float, true, true>::BK : Lay<1, 64, bf16, true, false>::BK; }
+int stage_values(bool f32) {
+  return f32 ? Lay<1, 64, float, true, true>::BK : Lay<1, 64, bf16, true, false>::BK;
+}
 
 Problem problem_of(int kind, int64_t m, int64_t n, int64_t k, const Cut& c, int bk, int splits) {
   Problem p = {};

@@ -134,9 +134,9 @@ def _raw_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
-_current_device = torch.cuda.current_device
-if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object
-    _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
+# the same index and handle without the lazy start (a CUDA tensor is there) and the Stream object
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 _OK, _NEEDS_WORKSPACE = 0, 3  # QRB_OK, QRB_ERR_WORKSPACE
 
 

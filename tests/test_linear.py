@@ -131,8 +131,8 @@ def test_sizes_workspaces_and_empty_calls():
     big = (1 << 30) + 1
     assert L.qrbl_linear(_fwd(k=big, ldx=big, ldw=big), None, 0, None) == 2
     assert L.qrbl_linear_backward(_bwd(m=big), None, 0, None) == 2
-    # an operand that is not 16-byte aligned, or FP32, is staged: a workspace is required
-    for a in (_fwd(m=64, x=P + 2), _fwd(m=64, ldx=33), _fwd(m=64, dtype=0)):
+    # an operand that is not 16-byte aligned, or FP32 of many rows, is staged: a workspace is required
+    for a in (_fwd(m=64, x=P + 2), _fwd(m=64, ldx=33), _fwd(m=200, dtype=0)):
         need = L.qrbl_linear_workspace_bytes(a)
         assert need > 0
         assert L.qrbl_linear(a, None, need, None) == 3
