@@ -51,7 +51,8 @@
 // error flag; the producer then waits (bounded) for its loads in flight, the
 // MMA warp for its MMAs, and the TMEM is freed. In a pair each CTA's waits for
 // the other are bounded the same way, and both reach the closing cluster
-// barrier before either exits.
+// barrier before either exits; by then each loading warp has seen every stage
+// released, so no commit's arrival is still on its way to either.
 #include <mutex>
 
 #include "qrb_linear.cuh"
@@ -633,6 +634,13 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
         ++u;
       }
     }
+    // The last stages' releases are waited for as well: the MMA warp's commits arrive
+    // on this CTA's barriers from outside its threads (a pair's second CTA gets them
+    // from the first one), and separate commits' arrivals need not land in order, so
+    // the accumulators being ready does not say that these are in. None may reach
+    // shared memory that this CTA has given back.
+    for (int v = u > L::ST ? u - L::ST : 0; live && v < u; ++v)
+      live = warp_wait(BAR(B_EMPTY + v % L::ST), (uint32_t)((v / L::ST) & 1), a.limit, s_abort);
     if (__any_sync(kFull, *s_abort != 0)) {  // no load may land after the block has gone
       if constexpr (CG == 1) {
         for (int v = u > L::ST ? u - L::ST : 0; v < u; ++v)

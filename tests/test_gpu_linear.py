@@ -785,3 +785,24 @@ def test_withheld_products_time_out_and_the_next_call_works():
             _lib.set_config(k, v)
         _lib.set_config("device_error", 0)
     assert torch.equal(api.linear(x, w), want)
+
+
+@pytest.mark.parametrize("cut", CUTS)
+def test_products_leave_nothing_in_flight(cut, hooks):
+    """Products of fewer, as many and more stages than the ring holds, each followed at
+    once by kernels that use the same SMs' shared memory: the same bits every time."""
+    hooks("linear_cut", cut)
+    hooks("linear_rows", 0)
+    G = rnd((4, 128, 128), 190, FP)
+    s0 = api.gram(G)
+    for k in (64, 192, 256, 512, 1000):
+        x, w, dy = rnd((520, k), 191, BF), rnd((264, k), 192, BF, k**-0.5), rnd((520, 264), 193, BF)
+        y0, g0 = api.linear(x, w), api.linear_backward(dy, x, w)
+        check_forward(x, w, None, None, "none", y0)
+        check_backward(dy, x.double(), w, None, "none", *g0)
+        runs = []
+        for _ in range(40):
+            runs += [(api.linear(x, w), api.gram(G), api.linear_backward(dy, x, w), api.gram(G))]
+        for y, s, g, t in runs:
+            assert torch.equal(y, y0) and torch.equal(s, s0) and torch.equal(t, s0)
+            assert all(torch.equal(p, q) for p, q in zip(g, g0))
