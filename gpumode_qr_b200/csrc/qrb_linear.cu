@@ -107,6 +107,7 @@ struct Forward {
   ProductSize size;
   ProductPlan plan;
   float* part = nullptr;
+  float* chains = nullptr;
 };
 Forward plan_forward(const qrbl_linear_args& a, Carve* c) {
   Forward f;
@@ -126,6 +127,7 @@ Forward plan_forward(const qrbl_linear_args& a, Carve* c) {
                     (a.residual != nullptr ? 4 : 0) | (a.z_codes != nullptr ? 8 : 0);
   f.plan = plan_products(a.dtype, &f.size, 1);
   f.part = reinterpret_cast<float*>(c->take(f.plan.part_bytes[0]));
+  if (f.plan.chain_bytes > 0) f.chains = reinterpret_cast<float*>(c->take(f.plan.chain_bytes));
   return f;
 }
 
@@ -162,7 +164,7 @@ int forward(const qrbl_linear_args& a, void* workspace, size_t bytes, cudaStream
   p.a = f.x; p.b = f.w;
   p.part = f.part;
   p.e = e;
-  return launch_products(a.dtype, &p, 1, f.plan, nullptr, before.stages > 0, s);
+  return launch_products(a.dtype, &p, 1, f.plan, f.chains, nullptr, before.stages > 0, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -208,6 +210,7 @@ struct Backward {
   int products = 0;
   ProductPlan plan;
   float* part[2] = {nullptr, nullptr};
+  float* chains = nullptr;
   float* colsum = nullptr;
   int64_t colsum_blocks = 0;
 };
@@ -248,6 +251,7 @@ Backward plan_backward(const qrbl_linear_backward_args& a, Carve* c) {
     b.plan = plan_products(a.dtype, b.size, b.products);
     for (int i = 0; i < b.products; ++i)
       b.part[i] = reinterpret_cast<float*>(c->take(b.plan.part_bytes[i]));
+    if (b.plan.chain_bytes > 0) b.chains = reinterpret_cast<float*>(c->take(b.plan.chain_bytes));
   }
   return b;
 }
@@ -327,7 +331,8 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
     p[j].size = b.size[j];
     p[j].part = b.part[j];
   }
-  if (i > 0) return launch_products(a.dtype, p, i, b.plan, b.db ? &sum : nullptr, prepared, s);
+  if (i > 0)
+    return launch_products(a.dtype, p, i, b.plan, b.chains, b.db ? &sum : nullptr, prepared, s);
   return b.db ? launch_colsum(a.dtype, sum, s) : QRB_OK;
 }
 

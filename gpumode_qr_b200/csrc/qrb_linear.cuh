@@ -533,13 +533,15 @@ struct ProductPlan {
   int splits[2] = {1, 1};
   int64_t part_rows[2] = {0, 0}, part_ld[2] = {0, 0};
   size_t part_bytes[2] = {0, 0};
+  size_t chain_bytes = 0;  // 16-bit reductions longer than an accumulator chain
 };
 struct ColSum;
 ProductPlan plan_products(int dtype, const ProductSize* sizes, int count);
-// sum (may be null): column sums finished in the same launch. after_prepare: the
-// launch in front of it on the stream is this call's launch_prepare.
+// chains: the plan's chain_bytes of workspace (null where it has none). sum (may be
+// null): column sums finished in the same launch. after_prepare: the launch in front
+// of it on the stream is this call's launch_prepare.
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
-                    const ColSum* sum, bool after_prepare, cudaStream_t s);
+                    float* chains, const ColSum* sum, bool after_prepare, cudaStream_t s);
 // The forward product of few rows (where takes_rows), x and w read in place at any
 // alignment.
 bool takes_rows(int dtype, int64_t m, int64_t n, int64_t k, bool packed);

@@ -27,9 +27,15 @@
 // every add, so a chain over the whole reduction would drift: every CHAIN
 // stages (a unit) the two accumulators are read and added to FP32 sums in
 // registers. A 16-bit forward product whose z is kept in 8 bits sums its chains
-// the same way (SUM): its other results are rounded far above the drift, but a
-// code near a border shows it (z's relative error against exact codes 3.2e-4 ->
-// 1.0e-4 at k = 4096, an FP32 product's 1.2e-4).
+// the same way (SUM): a code near a border shows the drift (z's relative error
+// against exact codes 3.2e-4 -> 1.0e-4 at k = 4096, an FP32 product's 1.2e-4).
+// Other 16-bit results are rounded above the drift of a chain of 8192 values:
+// each 16 of them cost at most 2^-23 of the sum, so a chain 2^-14, an eighth of
+// FP16's half step (measured on a long batch of one sign 5e-5; without an end to
+// the chain 1.5e-3 at 262,144 values, three half steps, and growing with them).
+// Longer reductions are read out every 8192 values and added in FP32 to this
+// warp's part of a buffer in the workspace, beside the next chain's MMAs: their
+// 256-column tiles leave no registers for the sums.
 //
 // A reduction split over several CTAs (few tiles, long k) writes FP32 partial
 // tiles that k_join adds in order: no atomics, the same bits every time.
@@ -64,7 +70,8 @@ namespace lin {
 namespace {
 
 constexpr int BM = 128;       // rows per CTA
-constexpr int kChainValues = 256;  // FP32: reduction values per accumulator chain
+constexpr int kChainValues = 256;  // sums in registers: reduction values per accumulator chain
+constexpr int kLongChain = 8192;   // sums in the workspace: the same
 constexpr int kMostEpiWarps = 16;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kSmemMost = 232448;  // 227 KB
@@ -83,7 +90,8 @@ struct Lay {
   static constexpr int BK = NP == 3 ? 32 : 64;       // reduction values per stage
   static constexpr uint32_t KROW = BK * 2;           // bytes of a K-major row
   static constexpr uint32_t ATOM = BK * 128;         // MN-major box: BK rows of 128 bytes
-  static constexpr int CHAIN = kChainValues / BK;    // FP32: stages per accumulator chain
+  // stages per accumulator chain
+  static constexpr int CHAIN = (SUM ? kChainValues : kLongChain) / BK;
   static constexpr int BROWS = BN / CG;              // B's columns of one CTA
   static constexpr uint32_t A = BM * KROW, B = BROWS * KROW;
   static constexpr uint32_t STAGE = NP * (A + B);
@@ -141,6 +149,7 @@ struct Args {
   Problem p[2];
   Schedule s;
   ColSum sum;       // column sums to finish beside the products (out null: none)
+  float* chains;    // sums of long reductions' chains, BM x BN per CTA (null: none is long)
   int* err;
   long long limit;
   int skip_mma;     // test hook: withhold the MMAs, so that the waits run out
@@ -556,6 +565,23 @@ __device__ __forceinline__ void drain(uint32_t t, float (&sum)[32], bool first) 
   }
 }
 
+// The lane's 32 sums in the workspace, lanes at neighbouring 16 bytes.
+__device__ __forceinline__ void keep(float4* p, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    p[32 * i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+__device__ __forceinline__ void add_kept(const float4* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 u = p[32 * i];
+    v[4 * i] += u.x;
+    v[4 * i + 1] += u.y;
+    v[4 * i + 2] += u.z;
+    v[4 * i + 3] += u.w;
+  }
+}
+
 template <int CG, int BN, typename T, bool FWD, bool SUM>
 __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
     k_product(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0,
@@ -667,7 +693,7 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
         const uint64_t da0 = operand_desc<L>(ring, amn);
         const uint64_t db0 = operand_desc<L>(ring + L::NP * L::A, bmn);
         for (int kb = it.kb0; live && kb < it.kb1;) {
-          const int end = SUM && kb + L::CHAIN < it.kb1 ? kb + L::CHAIN : it.kb1;
+          const int end = kb + L::CHAIN < it.kb1 ? kb + L::CHAIN : it.kb1;
           const int buf = unit % L::NACC;
           if (unit >= L::NACC)
             live = warp_wait(BAR(B_ACCEMPTY + buf), (uint32_t)((unit / L::NACC - 1) & 1), a.limit,
@@ -896,19 +922,33 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
       };
 
       if constexpr (!SUM) {
-        const int buf = unit % L::NACC;
-        live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / L::NACC) & 1), a.limit, s_abort);
-        if (!live) break;
-        tc::fence_after();
-        const uint32_t t = tmem + lanes + buf * L::ACC + part_of * HC;
+        // this lane's sums of the chains before the last: four columns each 32 apart
+        float4* kept = reinterpret_cast<float4*>(a.chains) +
+                       ((size_t)blockIdx.x * kEpiWarps + warp) * (HC * 8) + lane;
+        int kb = it.kb0;
+        do {
+          const int buf = unit % L::NACC;
+          live = warp_wait(BAR(B_ACCFULL + buf), (uint32_t)((unit / L::NACC) & 1), a.limit,
+                           s_abort);
+          if (!live) break;
+          tc::fence_after();
+          const uint32_t t = tmem + lanes + buf * L::ACC + part_of * HC;
+          const bool last = kb + L::CHAIN >= it.kb1;
 #pragma unroll 1
-        for (int c = 0; c < HC; c += 32) {
-          float v[32];
-          tc::tmem_ld32(t + c, v);
-          if (c + 32 == HC) hand_back(buf);
-          finish(v, c);
-        }
-        ++unit;
+          for (int c = 0; c < HC; c += 32) {
+            float v[32];
+            tc::tmem_ld32(t + c, v);
+            if (c + 32 == HC) hand_back(buf);
+            if (kb > it.kb0) add_kept(kept + 8 * c, v);
+            if (last)
+              finish(v, c);
+            else
+              keep(kept + 8 * c, v);
+          }
+          kb += L::CHAIN;
+          ++unit;
+        } while (live && kb < it.kb1);
+        if (!live) break;
       } else {
         static_assert(!SUM || HC == 32, "one block of sums per warp");
         float sum[32];
@@ -1248,6 +1288,17 @@ static ProductPlan search_plan(int dtype, const ProductSize* sizes, int count) {
     best.part_bytes[i] =
         (size_t)best.splits[i] * best.part_rows[i] * best.part_ld[i] * sizeof(float);
   }
+  if (!chains && least >= 0) {
+    int64_t items = 0;
+    bool some = false;
+    for (int i = 0; i < count; ++i) {
+      items += tiles_of(sizes[i].m, BM * best.cg) * tiles_of(sizes[i].n, best.bn) * best.splits[i];
+      some |= tiles_of(tiles_of(sizes[i].k, stage_values(f32)), best.splits[i]) >
+              kLongChain / stage_values(f32);
+    }
+    const int64_t workers = items < sms / best.cg ? items : sms / best.cg;
+    if (some) best.chain_bytes = (size_t)workers * best.cg * BM * best.bn * sizeof(float);
+  }
   best.ok = least >= 0;
   return best;
 }
@@ -1286,7 +1337,7 @@ ProductPlan plan_products(int dtype, const ProductSize* sizes, int count) {
 }
 
 int launch_products(int dtype, const Product* products, int count, const ProductPlan& plan,
-                    const ColSum* cols, bool after_prepare, cudaStream_t s) {
+                    float* chains, const ColSum* cols, bool after_prepare, cudaStream_t s) {
   const Device* d = device_info();
   if (d == nullptr) return QRB_ERR_DEVICE;
   if (!plan.ok) return QRB_ERR_UNSUPPORTED;
@@ -1319,6 +1370,7 @@ int launch_products(int dtype, const Product* products, int count, const Product
   }
   make_schedule(items, each, d->sms / c.cg, &args.s);
   if (cols != nullptr) args.sum = *cols;
+  args.chains = chains;
   args.err = d->err;
   args.limit = device_wait_limit();
   args.skip_mma = test_skip_mma() ? 1 : 0;

@@ -13,7 +13,9 @@
  *
  * Types: QRBL_F32, QRBL_F16 or QRBL_BF16 for every matrix and vector of one
  * call. Products accumulate in FP32 (FP16 and BF16 operands on the tensor
- * cores as they are; FP32 operands as three BF16 parts whose six largest
+ * cores as they are, whose own sums, which do not round to nearest, are taken
+ * out and added in FP32 after at most 8192 values: an error of at most 2^-14 of
+ * the terms' magnitudes at any length; FP32 operands as three BF16 parts whose six largest
  * products are formed, which keeps FP32's 24 bits; a product with an FP32 Inf
  * may give NaN instead of Inf). Every output is rounded once, to nearest even.
  *

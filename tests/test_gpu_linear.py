@@ -806,3 +806,49 @@ def test_products_leave_nothing_in_flight(cut, hooks):
         for y, s, g, t in runs:
             assert torch.equal(y, y0) and torch.equal(s, s0) and torch.equal(t, s0)
             assert all(torch.equal(p, q) for p, q in zip(g, g0))
+
+
+def long_acc(k):
+    """A 16-bit product's sum at any length: chains of at most 8192 values (16 to an MMA,
+    fewer than 16 adds within the last), added in FP32, each add half a step."""
+    return STEP * (8192 / 16 + 18) + STEP / 2 * (k / 8192 + 1)
+
+
+@pytest.mark.parametrize("dt", [BF, HF], ids=IDS[:2])
+@pytest.mark.parametrize("cut,splits", [(0, 0), (2256, 1), (2128, 1), (1128, 1), (1064, 1), (2256, 3)])
+def test_long_reductions_do_not_drift(cut, splits, dt, hooks):
+    """Terms of one sign, so that every truncated add would pull the same way."""
+    hooks("linear_cut", cut)
+    hooks("linear_splits", splits)
+    hooks("linear_rows", 0)
+    m, n, k = 600_011, 136, 264
+    g = torch.Generator(device=DEV).manual_seed(194)
+    one = lambda *s: ((torch.rand(*s, device=DEV, generator=g) + 0.5) * m**-0.5).to(dt)  # noqa: E731
+    dy, x, w = one(m, n), one(m, k), rnd((n, k), 195, dt)
+    dx, dw, _ = api.linear_backward(dy, x, w, need=("x", "weight"))
+    want = dy.double().mT @ x.double()
+    near(dw, want, (u(dt) * 1.0001 + long_acc(m) * (1 + u(dt))) * want, "dw")
+    check_backward(dy[:1000], None, w, None, "none", dx[:1000], None, None)
+    # forward, the long axis as k, rows of z beside it (no activation)
+    a, b = dy.t().contiguous(), x.t().contiguous()
+    y = api.linear(a, b)
+    near(y, want, (u(dt) * 1.0001 + long_acc(m) * (1 + u(dt))) * want, "y")
+
+
+@pytest.mark.parametrize("k", [8191, 8192, 8193, 16_384, 16_385, 24_640])
+def test_reductions_about_a_chain_are_exact(k, hooks):
+    """Small whole numbers: every partial sum is exact in FP32, so no value may be lost or
+    counted twice where one chain ends and the next begins."""
+    hooks("linear_splits", 1)
+    hooks("linear_rows", 0)
+    g = torch.Generator(device=DEV).manual_seed(k)
+    whole = lambda *s: torch.randint(-2, 3, s, device=DEV, generator=g).to(BF)  # noqa: E731
+    ld = (k + 7) // 8 * 8
+    for m, n in ((40, 72), (300, 520), (4000, 1100)):  # more tiles than SMs in the last
+        x, w = whole(m, ld)[:, :k], whole(n, ld)[:, :k]
+        want = (x.float() @ w.float().mT).to(BF)
+        for cut in (0, *CUTS):
+            hooks("linear_cut", cut)
+            assert torch.equal(api.linear(x, w), want)
+            assert torch.equal(api.linear_backward(x.t(), w.t(), w.new_zeros(m, n), need=("weight",))[1],
+                               want)
