@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4)
 // out[col] = sum over the blocks of part[block][col].
 template <typename T>
 __global__ void __launch_bounds__(128) k_colsum(ColSum c) {
-  column_sum<T>(c, (int64_t)blockIdx.x * 128 + threadIdx.x, (int64_t)gridDim.x * 128);
+  column_sum<T>(c, (int64_t)blockIdx.x * 4 + threadIdx.x / 32, (int64_t)gridDim.x * 4);
 }
 
 // ---------------------------------------------------------------------------
@@ -633,7 +633,7 @@ int colsum_rows(int64_t m, int64_t n) {
 }
 
 int launch_colsum(int dtype, const ColSum& c, cudaStream_t s) {
-  const int64_t gx = (c.n + 127) / 128;
+  const int64_t gx = (c.n * c.slices + 127) / 128;
   const unsigned grid = (unsigned)(gx < 65535 ? gx : 65535);
   QRBL_BY_TYPE(dtype, {
     k_colsum<T><<<grid, 128, 0, s>>>(c);

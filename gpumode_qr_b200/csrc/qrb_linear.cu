@@ -308,6 +308,7 @@ int backward(const qrbl_linear_backward_args& a, void* workspace, size_t bytes, 
   sum.blocks = b.colsum_blocks;
   sum.n = a.n;
   sum.out = a.dbias;
+  sum.slices = colsum_slices(b.colsum_blocks, a.n);
   auto rows16 = [&](const void* p, int64_t ld, int64_t rows) {
     return aligned16(p) && (rows <= 1 || (ld * es) % 16 == 0);
   };

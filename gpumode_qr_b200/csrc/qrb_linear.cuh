@@ -600,15 +600,32 @@ struct ColSum {
   const float* part = nullptr;
   int64_t blocks = 0, n = 0;
   void* out = nullptr;
+  int slices = 1;  // lanes of a warp that share a column, a power of two
 };
+// A warp takes 32 / slices columns: lane (slice, column) adds every slices-th block's
+// sum in order, then the slices are added in a fixed tree, all in 64 bits (there are
+// as many sums as a long batch has blocks).
 template <typename T>
-__device__ __forceinline__ void column_sum(const ColSum& c, int64_t first, int64_t step) {
-  for (int64_t col = first; col < c.n; col += step) {
-    double s = 0;  // (there are as many sums as a long batch has blocks)
+__device__ __forceinline__ void column_sum(const ColSum& c, int64_t warp, int64_t warps) {
+  const int lane = threadIdx.x & 31, wide = 32 / c.slices, slice = lane / wide;
+  for (int64_t c0 = warp * wide; c0 < c.n; c0 += warps * wide) {
+    const int64_t col = c0 + lane % wide;
+    double s = 0;
+    if (col < c.n) {
 #pragma unroll 16
-    for (int64_t b = 0; b < c.blocks; ++b) s += c.part[b * c.n + col];
-    reinterpret_cast<T*>(c.out)[col] = from_f<T>((float)s);
+      for (int64_t b = slice; b < c.blocks; b += c.slices) s += c.part[b * c.n + col];
+    }
+    for (int o = wide; o < 32; o *= 2) s += __shfl_xor_sync(kFull, s, o);
+    if (slice == 0 && col < c.n) reinterpret_cast<T*>(c.out)[col] = from_f<T>((float)s);
   }
+}
+// As many slices as leave each lane 16 sums, which it loads together, or as fill half
+// the card's lanes. Whole backward calls, BF16, k = 64, with one lane a column and so:
+// 20,000 x 64 25.0 and 13.6 us, 1,000,000 x 64 565 and 277, 8192 x 1024 21.3 and 16.1.
+inline int colsum_slices(int64_t blocks, int64_t n) {
+  int s = 1;
+  while (s < 32 && blocks > 16 * s && n * s <= 148 * 256) s *= 2;
+  return s;
 }
 int launch_colsum(int dtype, const ColSum& c, cudaStream_t s);
 

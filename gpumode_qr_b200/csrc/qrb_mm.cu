@@ -765,9 +765,9 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
       }
     };
     if constexpr (!FWD) {
-      if (a.sum.out != nullptr)
-        column_sum<T>(a.sum, (int64_t)blockIdx.x * (kEpiWarps * 32) + threadIdx.x,
-                      (int64_t)gridDim.x * (kEpiWarps * 32));
+      if (a.sum.out != nullptr)  // over the blocks first: no tile waits long for it
+        column_sum<T>(a.sum, (int64_t)warp * gridDim.x + blockIdx.x,
+                      (int64_t)gridDim.x * kEpiWarps);
     }
     for (int step = 0; live; ++step) {
       const Item it = item_of<CG, BN>(a, worker, step);

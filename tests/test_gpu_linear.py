@@ -852,3 +852,25 @@ def test_reductions_about_a_chain_are_exact(k, hooks):
             assert torch.equal(api.linear(x, w), want)
             assert torch.equal(api.linear_backward(x.t(), w.t(), w.new_zeros(m, n), need=("weight",))[1],
                                want)
+
+
+@pytest.mark.parametrize("n", [32, 200])
+def test_bias_sums_of_a_long_batch_hold_nothing_up(n, hooks):
+    """The sums are added beside the products' tiles: with the waits bounded by 300,000
+    clocks (150 us) none runs out over 15,626 blocks' sums of each column."""
+    m, k = 2_000_003, 64
+    g = torch.Generator(device=DEV).manual_seed(196)
+    dy = torch.randint(-2, 3, (m, n), device=DEV, generator=g).to(BF)
+    x, w = rnd((m, k), 197, BF), rnd((n, k), 198, BF)
+    want = dy.double().sum(0).to(BF)
+    limits = {"wait_limit": 300_000, "sync_check": 1}
+    old = {key: _lib.get_config(key) for key in limits}
+    try:
+        for key, v in limits.items():
+            _lib.set_config(key, v)
+        got = [api.linear_backward(dy, x, w)[2], api.linear_backward(dy, x, w, need=("bias",))[2]]
+    finally:
+        for key, v in old.items():
+            _lib.set_config(key, v)
+        _lib.set_config("device_error", 0)
+    assert all(torch.equal(db, want) for db in got)
