@@ -250,6 +250,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     if len(ws) != 2 or not ds or ds[-1] != ws[0]:
         raise ValueError(f"dy must be [..., n] and weight [n, k], got {tuple(ds)} and {tuple(ws)}")
     act = ACTIVATIONS[activation] if activation in ACTIVATIONS else _activation(activation)
+    if type(need) is not tuple and not isinstance(need, str):
+        need = tuple(need)  # an iterator gives its names once
     if isinstance(need, str) or not _NEED.issuperset(need):
         raise ValueError(f"need must name some of 'x', 'weight' and 'bias', got {need!r}")
     n, k = ws

@@ -874,3 +874,15 @@ def test_bias_sums_of_a_long_batch_hold_nothing_up(n, hooks):
             _lib.set_config(key, v)
         _lib.set_config("device_error", 0)
     assert all(torch.equal(db, want) for db in got)
+
+
+@pytest.mark.parametrize("need", [("x", "bias"), ("weight",), ()])
+def test_need_may_be_any_iterable(need):
+    dy, x, w = rnd((20, 24), 199, BF), rnd((20, 16), 200, BF), rnd((24, 16), 201, BF)
+    want = api.linear_backward(dy, x, w, need=need)
+    assert [g is not None for g in want] == [name in need for name in ("x", "weight", "bias")]
+    for given in (list(need), set(need), iter(need), (name for name in need), dict.fromkeys(need)):
+        for g, h in zip(api.linear_backward(dy, x, w, need=given), want):
+            assert h is None if g is None else torch.equal(g, h)
+    with pytest.raises(ValueError, match="need"):
+        api.linear_backward(dy, x, w, need=iter(("x", "y")))
