@@ -183,7 +183,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     xs, ws = x.shape, weight.shape
     if len(ws) != 2 or not xs or xs[-1] != ws[1]:
         raise ValueError(f"x must be [..., k] and weight [n, k], got {tuple(xs)} and {tuple(ws)}")
-    act = ACTIVATIONS[activation] if activation in ACTIVATIONS else _activation(activation)
+    known = type(activation) is str and activation in ACTIVATIONS
+    act = ACTIVATIONS[activation] if known else _activation(activation)
     n, k = ws
     shape = (xs[0], n) if len(xs) == 2 else (*xs[:-1], n)
     x2, m, ldx = _rows(x, xs, k)
@@ -249,7 +250,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     ds, ws = dy.shape, weight.shape
     if len(ws) != 2 or not ds or ds[-1] != ws[0]:
         raise ValueError(f"dy must be [..., n] and weight [n, k], got {tuple(ds)} and {tuple(ws)}")
-    act = ACTIVATIONS[activation] if activation in ACTIVATIONS else _activation(activation)
+    known = type(activation) is str and activation in ACTIVATIONS
+    act = ACTIVATIONS[activation] if known else _activation(activation)
     if type(need) is not tuple and not isinstance(need, str):
         need = tuple(need)  # an iterator gives its names once
     if isinstance(need, str) or not _NEED.issuperset(need):

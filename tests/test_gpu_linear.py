@@ -886,3 +886,12 @@ def test_need_may_be_any_iterable(need):
             assert h is None if g is None else torch.equal(g, h)
     with pytest.raises(ValueError, match="need"):
         api.linear_backward(dy, x, w, need=iter(("x", "y")))
+
+
+@pytest.mark.parametrize("act", [["gelu"], {"gelu": 1}, {"gelu"}, 2, b"gelu"])
+def test_activations_that_are_no_names_are_refused(act):
+    x, w = rnd((4, 8), 202, BF), rnd((6, 8), 203, BF)
+    with pytest.raises(ValueError, match="activation must be one of"):
+        api.linear(x, w, activation=act)
+    with pytest.raises(ValueError, match="activation must be one of"):
+        api.linear_backward(rnd((4, 6), 204, BF), x, w, x, act)
