@@ -17,7 +17,8 @@ All run on the caller's current stream, allocate only their outputs and scratch
 the same bits every time (for the same sizes, layouts and arguments). They are
 plain functions, like the rest of the library: autograd does not record them,
 and arguments that require a gradient are refused while gradients are enabled
-(call them under ``torch.no_grad()`` or from an ``autograd.Function``).
+(call them under ``torch.no_grad()`` or from an ``autograd.Function``), as are
+arguments with a tangent of forward-mode differentiation, which would be lost.
 """
 
 from __future__ import annotations
@@ -26,6 +27,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 
@@ -79,6 +81,18 @@ def _check(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, but autograd does not record this call: "
                            "use torch.no_grad() and linear_backward")
+
+
+def _refuse_tangents(**tensors) -> None:
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has a tangent, but forward-mode differentiation does not "
+                               "pass through this call: give its primal (unpack_dual)")
+
+
+def _differentiating() -> bool:
+    """Whether forward-mode differentiation is on (its level read without a call)."""
+    return getattr(_forward_ad, "_current_level", 0) >= 0
 
 
 def _check_packed(name: str, p: PackedActivation, like: torch.Tensor, shape: tuple) -> None:
@@ -185,6 +199,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         raise ValueError(f"x must be [..., k] and weight [n, k], got {tuple(xs)} and {tuple(ws)}")
     known = type(activation) is str and activation in ACTIVATIONS
     act = ACTIVATIONS[activation] if known else _activation(activation)
+    if _differentiating():
+        _refuse_tangents(x=x, weight=weight, bias=bias, residual=residual)
     n, k = ws
     shape = (xs[0], n) if len(xs) == 2 else (*xs[:-1], n)
     x2, m, ldx = _rows(x, xs, k)
@@ -256,6 +272,9 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
         need = tuple(need)  # an iterator gives its names once
     if isinstance(need, str) or not _NEED.issuperset(need):
         raise ValueError(f"need must name some of 'x', 'weight' and 'bias', got {need!r}")
+    if _differentiating():
+        _refuse_tangents(dy=dy, weight=weight, x=x if "weight" in need else None,
+                         z=z if act else None)
     n, k = ws
     lead = (ds[0],) if len(ds) == 2 else tuple(ds[:-1])
     dy2, m, lddy = _rows(dy, ds, n)
@@ -343,6 +362,8 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
         _check("x", x)
     if x.dim() < 1:
         raise ValueError("x must be [..., c], got a scalar")
+    if _differentiating():
+        _refuse_tangents(x=x)
     shape = x.shape
     p = _empty_packed(shape, x)
     if x.numel():

@@ -895,3 +895,28 @@ def test_activations_that_are_no_names_are_refused(act):
         api.linear(x, w, activation=act)
     with pytest.raises(ValueError, match="activation must be one of"):
         api.linear_backward(rnd((4, 6), 204, BF), x, w, x, act)
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as forward_ad
+
+    x, w, b, r = rnd((4, 8), 205, FP), rnd((6, 8), 206, FP), rnd((6,), 207, FP), rnd((4, 6), 208, FP)
+    want = api.linear(x, w, b, r)
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: api.linear(dual(x), w), lambda: api.linear(x, dual(w)),
+                     lambda: api.linear(x, w, dual(b)), lambda: api.linear(x, w, b, dual(r)),
+                     lambda: api.linear_backward(dual(r), x, w),
+                     lambda: api.linear_backward(r, dual(x), w),
+                     lambda: api.linear_backward(r, x, dual(w)),
+                     lambda: api.linear_backward(r, x, w, dual(r), "gelu"),
+                     lambda: api.pack_activation(dual(x))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        # tensors without one, packed ones among them, are taken
+        assert torch.equal(api.linear(x, w, b, r), want)
+        assert torch.equal(api.linear(forward_ad.unpack_dual(dual(x)).primal, w, b, r), want)
+        api.linear_backward(r, api.pack_activation(x), w)
+        api.linear_backward(r, dual(x), w, dual(r), need=("x",))  # neither is read
+    with pytest.raises(RuntimeError, match="tangent"):
+        torch.func.jvp(lambda t: api.linear(t, w), (x,), (x,))
