@@ -128,7 +128,7 @@ def _rows(t: torch.Tensor, shape: torch.Size, cols: int) -> tuple[torch.Tensor, 
         t = t.reshape(-1, cols) if cols else t.new_empty((shape[:-1].numel(), 0))
         shape = t.shape
     rows = shape[0]
-    if cols == 1:  # a column of a conjugate's .imag is stored negated (wider ones are copied)
+    if t.is_neg():  # a conjugate's .imag is stored negated
         t = t.resolve_neg()
     row, col = t.stride()
     if (col != 1 and cols > 1) or (row < cols and rows > 1):
@@ -212,7 +212,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             _check("bias", bias, x)
         if bias.shape != (n,):
             raise ValueError(f"bias must be ({n},), got {tuple(bias.shape)}")
-        if bias.stride(0) != 1:
+        if bias.stride(0) != 1 or bias.is_neg():
             bias = bias.contiguous().resolve_neg()
         bp = bias.data_ptr()
     if residual is not None:

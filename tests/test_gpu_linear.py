@@ -920,3 +920,16 @@ def test_tangents_are_refused():
         api.linear_backward(r, dual(x), w, dual(r), need=("x",))  # neither is read
     with pytest.raises(RuntimeError, match="tangent"):
         torch.func.jvp(lambda t: api.linear(t, w), (x,), (x,))
+
+
+def test_negated_views_with_unit_stride():
+    c = torch.complex(rnd((6, 8), 209, FP), rnd((6, 8), 210, FP)).conj().imag
+    x, w = c.as_strided((5, 4), (8, 1)), rnd((6, 4), 211, FP)  # elements of both parts, all negated
+    one = c[0, 0].reshape(1)
+    assert x.is_neg() and x.stride(1) == 1 and one.is_neg() and one.stride() == (1,)
+    check_forward(x, w, None, None, "none", api.linear(x, w))
+    check_forward(w, x, None, w[:, :1].expand(6, 5), "none", api.linear(w, x, None, w[:, :1].expand(6, 5)))
+    check_forward(x, w[:1], one, x[:, :1], "none", api.linear(x, w[:1], one, x[:, :1]))
+    check_backward(x, rnd((5, 3), 212, FP).double(), rnd((4, 3), 213, FP), x.double(), "silu",
+                   *api.linear_backward(x, rnd((5, 3), 212, FP), rnd((4, 3), 213, FP), x, "silu"))
+    assert torch.equal(api.pack_activation(x).codes, api.pack_activation(x.clone()).codes)
