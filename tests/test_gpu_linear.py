@@ -933,3 +933,33 @@ def test_negated_views_with_unit_stride():
     check_backward(x, rnd((5, 3), 212, FP).double(), rnd((4, 3), 213, FP), x.double(), "silu",
                    *api.linear_backward(x, rnd((5, 3), 212, FP), rnd((4, 3), 213, FP), x, "silu"))
     assert torch.equal(api.pack_activation(x).codes, api.pack_activation(x.clone()).codes)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(60_001, 64, 72), (200_000, 40, 32), (100_003, 256, 264)])
+def test_long_batch_is_exact_in_whole_numbers(m, n, k, dt):
+    """Products and sums of whole numbers up to 2 are exact below 2^24, in every type's
+    operands, so dW, db and dx are the exact sums rounded once: no row of the batch may
+    be lost, counted twice or added to another."""
+    g = torch.Generator(device=DEV).manual_seed(m)
+    whole = lambda *s: torch.randint(-2, 3, s, device=DEV, generator=g).to(dt)  # noqa: E731
+    dy, x, w = whole(m, n), whole(m, k), whole(n, k)
+    dx, dw, db = api.linear_backward(dy, x, w)
+    assert torch.equal(dw, (dy.double().mT @ x.double()).to(dt))
+    assert torch.equal(db, dy.double().sum(0).to(dt))
+    assert torch.equal(dx, (dy.double() @ w.double()).to(dt))
+
+
+@pytest.mark.parametrize("products", [True, False])
+def test_block_sums_of_the_bias_are_joined_in_64_bits(products):
+    """Rows of c = (1 + 2^-17) 2^j / 128: a block of 8, 32 or 128 of them has an exact FP32
+    sum ((2^17 + 1) i with i <= 128 takes 24 bits), and thousands of blocks an exact FP64
+    sum; joined in FP32, each add beyond 128 blocks would lose 2^-17."""
+    m, n, k = 1_000_003, 48, 16
+    c = (1 + 2.0**-17) / 128 * 2.0 ** (torch.arange(n, dtype=torch.float64, device=DEV) % 5)
+    c = c * (1 - 2 * (torch.arange(n, device=DEV) % 2))
+    dy = c.float().expand(m, n).contiguous()
+    assert torch.equal(dy[0].double(), c)
+    x, w = rnd((m, k), 214, FP), rnd((n, k), 215, FP)
+    db = api.linear_backward(dy, x, w, need=("x", "weight", "bias") if products else ("bias",))[2]
+    assert torch.equal(db, (m * c).float())
