@@ -289,7 +289,6 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
-// Bounded: false on a timeout (which sets *abort) or once *abort is set.
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t pred;
@@ -300,6 +299,7 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(pred));
   return pred != 0;
 }
+// Bounded: false on a timeout (which sets *abort) or once *abort is set.
 // Block-scope acquire, also for what the other CTA of a pair announces: all that
 // passes between them is TMA and TMEM traffic, ordered by the barriers
 // themselves; a cluster-scope release or acquire would wait for this CTA's
@@ -417,10 +417,6 @@ __device__ __forceinline__ void load_box2(uint32_t dst, const CUtensorMap* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
-// At most one of this thread's stores still reads shared memory.
-__device__ __forceinline__ void bulk_wait_read_one() {
-  asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-}
 
 // A warp's block of 32 columns of up to eight rows, packed (lane = column).
 template <typename T>
@@ -456,7 +452,7 @@ __device__ __forceinline__ void pack_rows(const float (&p)[8], int64_t row, int 
 // rows at a time, so that every access is consecutive elements of one row,
 // whatever their alignment: blocks that are cut by the matrix's edge or whose
 // rows are not 16-byte aligned.
-template <typename T, bool FWD, int TROWS>
+template <typename T, bool FWD, bool SUM, int TROWS>
 __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, int col,
                                               const Problem& a, float* turn) {
   if (row0 >= a.m || col >= a.n) return;
@@ -512,7 +508,9 @@ __device__ __forceinline__ void finish_turned(const float (&v)[32], int row0, in
           for (int k = 0; k < 8; ++k)
             if (k < left) z[k * e.ldz] = from_f<T>(p[k]);
         }
-        if (e.z_codes != nullptr) pack_rows<T>(p, row0g, left, live, col, a);
+        if constexpr (SUM) {
+          if (e.z_codes != nullptr) pack_rows<T>(p, row0g, left, live, col, a);
+        }
         act_by(p, e.act);
 #pragma unroll
         for (int k = 0; k < 8; ++k) p[k] += q[k];
@@ -746,6 +744,7 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
     const int quad = warp & 3, part_of = warp >> 2;  // rows, columns
     constexpr int HC = L::HC;  // columns of this warp
     constexpr int NH = L::HALVES;
+    static_assert(HC == 32 || NH == 2, "a block's staging is free or waited for once");
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t stg = ring + L::ST * L::STAGE + warp * L::WBUF;
     float* turn = reinterpret_cast<float*>(sm + (stg - base));
@@ -780,7 +779,7 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
       const bool staged = part || e.vec != 0;
       // what is kept of z goes through the first half, y through the second
       const bool plain_z = FWD && !part && staged && e.z != nullptr;
-      const bool packed_z = FWD && !part && staged && e.z_codes != nullptr;
+      const bool packed_z = FWD && SUM && !part && staged && e.z_codes != nullptr;
       const bool keep_z = plain_z || packed_z;
       const bool has_res = FWD && !part && staged && e.residual != nullptr;
       // The staging is free once the last tile's stores have read it: awaited here
@@ -814,7 +813,6 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
                         : 0.f;
         }
       }
-      uint32_t exps = 0;
       const bool early = has_res && inside && !(NH == 1 && keep_z);
       if (early && col < p.n) load_res(0);
       if (early && !keep_z && NH == 2 && HC > 32 && col + 32 < p.n) load_res(1);
@@ -840,7 +838,7 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
         }
         if (at >= p.n || !inside) return;
         if (!staged) {
-          finish_turned<T, FWD, L::TROWS>(v, row0, at, p, turn);
+          finish_turned<T, FWD, SUM, L::TROWS>(v, row0, at, p, turn);
           return;
         }
         if constexpr (L::PAIRED) {
@@ -856,15 +854,10 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
           return;
         }
         const uint32_t ybuf = stg + half_of(g) * L::HBUF;
-        if (g > 0 && (g >= NH || keep_z)) {  // this block's staging is free
-          if (lane == 0) {
-            if (NH == 2 && !keep_z)
-              bulk_wait_read_one();
-            else
-              tma::bulk_wait_read_all();
-          }
+        if (g > 0 && keep_z) {  // (the second and last block) its staging is free
+          if (lane == 0) tma::bulk_wait_read_all();
           __syncwarp();
-          if (has_res && !(NH == 1 && keep_z)) load_res(g);
+          if (has_res) load_res(g);
         }
         // a kept block of z out of the first half
         auto flush_z = [&](const CUtensorMap* map) {
@@ -890,18 +883,13 @@ __global__ void __launch_bounds__((Lay<CG, BN, T, FWD, SUM>::THREADS), 1)
             stage_write<T, L::ROWB>(stg, v);
             flush_z(&map_z);
           }
-          if (packed_z) {
-            const int ex = pack32<T>(stg, v);
-            flush_z(&map_q);
-            exps |= (uint32_t)(ex & 255) << (8 * g);
-            if (c + 32 == HC || at + 32 >= p.n) {  // the row's exponents of all blocks
-              const int nblk = (p.n + kBlk - 1) / kBlk;
-              int8_t* x = e.z_exps + (int64_t)(row0 + lane) * nblk + col / kBlk;
-              if (row0 + lane < p.m) {
-#pragma unroll
-                for (int i = 0; i < HC / 32; ++i)
-                  if (i <= g) x[i] = (int8_t)(exps >> (8 * i));
-              }
+          if constexpr (SUM) {  // (one block of 32 columns a warp)
+            if (packed_z) {
+              const int ex = pack32<T>(stg, v);
+              flush_z(&map_q);
+              if (row0 + lane < p.m)
+                e.z_exps[(int64_t)(row0 + lane) * ((p.n + kBlk - 1) / kBlk) + at / kBlk] =
+                    (int8_t)ex;
             }
           }
           act_by(v, e.act);
