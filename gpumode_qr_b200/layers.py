@@ -24,6 +24,7 @@ arguments with a tangent of forward-mode differentiation, which would be lost.
 from __future__ import annotations
 
 import struct
+from types import SimpleNamespace
 from typing import NamedTuple
 
 import torch
@@ -90,11 +91,6 @@ def _refuse_tangents(**tensors) -> None:
                                "pass through this call: give its primal (unpack_dual)")
 
 
-def _differentiating() -> bool:
-    """Whether forward-mode differentiation is on (its level read without a call)."""
-    return getattr(_forward_ad, "_current_level", 0) >= 0
-
-
 def _check_packed(name: str, p: PackedActivation, like: torch.Tensor, shape: tuple) -> None:
     codes, exps, dtype = p
     if dtype is not like.dtype:
@@ -130,6 +126,8 @@ def _rows(t: torch.Tensor, shape: torch.Size, cols: int) -> tuple[torch.Tensor, 
     rows = shape[0]
     if t.is_neg():  # a conjugate's .imag is stored negated
         t = t.resolve_neg()
+    if t.is_contiguous():
+        return t, rows, cols
     row, col = t.stride()
     if (col != 1 and cols > 1) or (row < cols and rows > 1):
         t = t.contiguous()
@@ -137,11 +135,8 @@ def _rows(t: torch.Tensor, shape: torch.Size, cols: int) -> tuple[torch.Tensor, 
     return t, rows, row
 
 
-def _activation(name: str) -> int:
-    try:
-        return ACTIVATIONS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {name!r}") from None
+def _no_activation(name) -> ValueError:
+    return ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {name!r}")
 
 
 def _raw_stream(index: int) -> int:
@@ -151,6 +146,8 @@ def _raw_stream(index: int) -> int:
 # the same index and handle without the lazy start (a CUDA tensor is there) and the Stream object
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+# forward-mode differentiation is on where its level is not negative, read without a call
+_level = _forward_ad if hasattr(_forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
 _OK, _NEEDS_WORKSPACE = 0, 3  # QRB_OK, QRB_ERR_WORKSPACE
 
 
@@ -197,9 +194,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     xs, ws = x.shape, weight.shape
     if len(ws) != 2 or not xs or xs[-1] != ws[1]:
         raise ValueError(f"x must be [..., k] and weight [n, k], got {tuple(xs)} and {tuple(ws)}")
-    known = type(activation) is str and activation in ACTIVATIONS
-    act = ACTIVATIONS[activation] if known else _activation(activation)
-    if _differentiating():
+    try:
+        act = ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise _no_activation(activation) from None
+    if _level._current_level >= 0:
         _refuse_tangents(x=x, weight=weight, bias=bias, residual=residual)
     n, k = ws
     shape = (xs[0], n) if len(xs) == 2 else (*xs[:-1], n)
@@ -236,7 +235,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             raise ValueError(f"keep must be None, 'plain' or 'packed', got {keep!r}")
     y = x.new_empty(*shape)  # (separate ints: parsed faster than a tuple)
     if m and n:
-        L = _lib.lib()
+        L = _lib._lib or _lib.lib()
         _run(L.qrbl_linear, L.qrbl_linear_workspace_bytes,
              _linear_args(_DTYPES[dt], act, m, n, k, x2.data_ptr(), ldx, w2.data_ptr(), ldw,
                           bp, rp, ldr, y.data_ptr(), n, zp, ldz, qp, ep), x)
@@ -266,13 +265,15 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     ds, ws = dy.shape, weight.shape
     if len(ws) != 2 or not ds or ds[-1] != ws[0]:
         raise ValueError(f"dy must be [..., n] and weight [n, k], got {tuple(ds)} and {tuple(ws)}")
-    known = type(activation) is str and activation in ACTIVATIONS
-    act = ACTIVATIONS[activation] if known else _activation(activation)
+    try:
+        act = ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise _no_activation(activation) from None
     if type(need) is not tuple and not isinstance(need, str):
         need = tuple(need)  # an iterator gives its names once
     if isinstance(need, str) or not _NEED.issuperset(need):
         raise ValueError(f"need must name some of 'x', 'weight' and 'bias', got {need!r}")
-    if _differentiating():
+    if _level._current_level >= 0:
         _refuse_tangents(dy=dy, weight=weight, x=x if "weight" in need else None,
                          z=z if act else None)
     n, k = ws
@@ -325,7 +326,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     if "bias" in need:
         db = dy.new_empty(n)
         dbp = db.data_ptr()
-    L = _lib.lib()
+    L = _lib._lib or _lib.lib()
     _run(L.qrbl_linear_backward, L.qrbl_linear_backward_workspace_bytes,
          _backward_args(_DTYPES[dt], act, m, n, k, dy2.data_ptr(), lddy, xp, ldx, xq, xe,
                         w2.data_ptr(), ldw, zp, ldz, zq, ze, dxp, k, dwp, k, dbp), dy, True)
@@ -362,7 +363,7 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
         _check("x", x)
     if x.dim() < 1:
         raise ValueError("x must be [..., c], got a scalar")
-    if _differentiating():
+    if _level._current_level >= 0:
         _refuse_tangents(x=x)
     shape = x.shape
     p = _empty_packed(shape, x)
