@@ -42,8 +42,8 @@
 //
 // What bounds it, measured on a B200 (single launches):
 //  - long reductions: the tensor cores. dW and dx of 8192 x 4096 x 4096 BF16 in one
-//    launch 340 us = 1617 TFLOP/s (a library product's burst rate is 1689), the
-//    forward product alone 181 us = 1520; back to back the card's power limit takes
+//    launch 332 us = 1656 TFLOP/s (a library product's burst rate is 1689), the
+//    forward product alone 178 us = 1544; back to back the card's power limit takes
 //    both to about 1300. 256 x 256 tiles on a pair: a CTA's 128 x 256 would need 96 bytes a
 //    clock from L2, more than the 64 an SM gets (719 clocks a stage; a pair 800
 //    until its MMAs were issued from uniform registers, now 580).

@@ -178,7 +178,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     ``[..., n]``, all float32, float16 or bfloat16 (one type) on one CUDA device,
     any strides. ``activation`` is ``"none"``, ``"relu"``, ``"gelu"``,
     ``"gelu_tanh"`` or ``"silu"``. Sums are FP32 (FP32 inputs keep their 24
-    bits: no TF32); y is rounded once.
+    bits: no TF32; below 2^-110 they lose low ones); y is rounded once. An Inf
+    among FP32 inputs may give NaN where the product is Inf: whether it does
+    depends on the number of rows.
 
     ``keep`` also returns the pre-activation ``z = x @ weight.T + bias`` for
     :func:`linear_backward`: ``"plain"`` as a tensor like y, ``"packed"`` as a
@@ -254,7 +256,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor | PackedActivation | None,
     ``need`` names the gradients to compute; the others are None. The residual's
     gradient is ``dy`` itself. ``dz = dy * act'(z)`` is rounded to the layer's
     type before the two products (dbias sums it unrounded); each result is
-    rounded once.
+    rounded once. An Inf among FP32 inputs may give NaN, as in :func:`linear`.
+    Packed x is read back into the call's workspace in the layer's type.
     """
     if type(dy) is not _Tensor or dy.dtype not in _DTYPES or not dy.is_cuda or dy.requires_grad:
         _check("dy", dy)

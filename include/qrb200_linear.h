@@ -14,10 +14,11 @@
  * Types: QRBL_F32, QRBL_F16 or QRBL_BF16 for every matrix and vector of one
  * call. Products accumulate in FP32 (FP16 and BF16 operands on the tensor
  * cores as they are, whose own sums, which do not round to nearest, are taken
- * out and added in FP32 after at most 8192 values: an error of at most 2^-14 of
- * the terms' magnitudes at any length; FP32 operands as three BF16 parts whose six largest
- * products are formed, which keeps FP32's 24 bits; a product with an FP32 Inf
- * may give NaN instead of Inf). Every output is rounded once, to nearest even.
+ * out and added in FP32 after at most 8192 values: they add at most 2^-14 of
+ * the terms' magnitudes to FP32's own roundings, at any length; FP32 operands as three BF16 parts
+ * whose six largest products are formed, which keeps FP32's 24 bits of
+ * operands above 2^-110 in magnitude; a product with an FP32 Inf may give NaN
+ * instead of Inf). Every output is rounded once, to nearest even.
  *
  * Results are the same from call to call (no atomics), for given sizes,
  * alignments, device and set of arguments (what is asked for beside a product can
@@ -72,10 +73,11 @@ typedef struct {
 } qrbl_linear_args;
 
 /* Bytes of device workspace (16-byte aligned) qrbl_linear takes for these
- * arguments: operands that the tensor memory accelerator cannot read in place
- * (rows or base not 16-byte aligned; FP32 parts) and the partial sums of a
- * product split along k. A function of the arguments' sizes, strides,
- * alignments and of which pointers are given. 0 for invalid arguments. */
+ * arguments: operands that the tensor memory accelerator cannot read in
+ * place (rows or base not 16-byte aligned; FP32 parts), the partial sums of
+ * a product split along its reduction and the sums of a reduction longer
+ * than 8192. A function of the arguments' sizes, strides, alignments and of
+ * which pointers are given. 0 for invalid arguments. */
 QRB_API size_t qrbl_linear_workspace_bytes(const qrbl_linear_args* args);
 QRB_API int qrbl_linear(const qrbl_linear_args* args, void* workspace, size_t workspace_bytes,
                         void* stream);
